@@ -11,6 +11,7 @@ from __future__ import annotations
 import glob
 import os
 import shutil
+import subprocess
 import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -36,6 +37,25 @@ def sources() -> list[str]:
     )
 
 
+def cxx_library_flags() -> list[str]:
+    """Link the process's own C++ library.  A compiler whose folder holds only
+    ``libstdc++.a`` links a second copy in, and an error message with a number
+    in it then ends the process inside the other copy's stream."""
+    cxx = os.environ.get("CXX", "c++")
+
+    def found(name: str) -> bool:
+        try:
+            path = subprocess.run([cxx, f"-print-file-name={name}"], capture_output=True,
+                                  text=True, check=True).stdout.strip()
+        except (OSError, subprocess.CalledProcessError):
+            return False
+        return os.path.isabs(path)
+
+    if not found("libstdc++.so") and found("libstdc++.so.6"):
+        return ["-l:libstdc++.so.6"]
+    return []
+
+
 def build(verbose: bool = False) -> str:
     from torch.utils import cpp_extension
 
@@ -47,7 +67,7 @@ def build(verbose: bool = False) -> str:
         extra_cflags=CXX_FLAGS,
         extra_cuda_cflags=NVCC_FLAGS,
         extra_include_paths=[CSRC],
-        extra_ldflags=["-lrt"],
+        extra_ldflags=["-lrt"] + cxx_library_flags(),
         build_directory=BUILD_DIR,
         with_cuda=True,
         is_python_module=True,
