@@ -17,12 +17,17 @@ Ops here:
   calculate_cdf, encode_fast_new, decode_fast_prefsum,
   rotary_embedding_k_fused, rotary_embedding_k_fused_layers (every layer in one
   launch), layerwise_prefill_dma_copy, get_gpu_pci_bus_id.
+Operators of a serving step on the paged cache (not in the reference):
+  build_slot_mapping (block tables and slots from request lengths),
+  rotary_embedding, rotary_embedding_and_cache (fresh rows, K/V to their pages),
+  shared_prefix_attention (a batch over one prefix), position_attention
+  (CacheBlend's recomputed rows over all keys).
 The reference's raw-pointer call signatures are in ``lmcache_ascend_b200.c_ops``.
 """
 
 from __future__ import annotations
 
-from typing import Tuple, List, Optional, Sequence
+from typing import Tuple, List, NamedTuple, Optional, Sequence, Union
 
 import torch
 
@@ -551,6 +556,210 @@ def rotary_embedding_k_fused_layers(old_positions, new_positions, keys, head_siz
     for k in keys:
         rotary_embedding_k_fused(old_positions, new_positions, k, head_size, cos_sin_cache,
                                  is_neox, slot_mapping)
+
+
+# ----------------------------------------------------- serving-step operators
+class SlotMapping(NamedTuple):
+    """The new tokens of a step, packed request after request."""
+
+    slot_mapping: torch.Tensor     # [num_tokens] slot of each token, -1: none
+    positions: torch.Tensor        # [num_tokens] position in its request
+    request_ids: torch.Tensor      # [num_tokens] int32 request, -1 behind the last one
+    query_start_loc: torch.Tensor  # [batch + 1] int32 first token of each request
+    seq_lens: torch.Tensor         # [batch] int32 context + new tokens
+    taken: torch.Tensor            # [batch + 1] int32 free blocks used before each request
+
+
+def build_slot_mapping(context_lens: torch.Tensor, new_lens: torch.Tensor,
+                       block_tables: torch.Tensor, block_size: int, num_tokens: int,
+                       free_blocks: Optional[torch.Tensor] = None,
+                       num_blocks: Optional[int] = None, dtype: torch.dtype = torch.int64,
+                       status: Optional[torch.Tensor] = None) -> SlotMapping:
+    """Slots and positions of a step's new tokens from the request lengths, in
+    one launch and without a host synchronisation (capturable).
+
+    ``context_lens`` / ``new_lens`` (int32 or int64 [batch]): tokens a request
+    holds and gets.  ``block_tables`` (int32 [>= batch, width]): its blocks.
+    With ``free_blocks`` (int32) the blocks missing for the new tokens are taken
+    from it in request order and written to ``block_tables``; ``taken[-1]`` of
+    them are used up.  Without it the tables hold every block already.
+    ``num_tokens``: rows of the outputs; rows behind the last request get slot
+    -1, position 0 and request -1.
+
+    A token has slot -1 when its block is missing: the free list or the table
+    row is too short, or the block id is not in [0, ``num_blocks``).  These, and
+    lengths below zero (taken as zero) or more than ``num_tokens`` tokens (cut),
+    are reported in ``status`` (a ``DeviceStatus`` tensor).
+    """
+    if dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"slots are int32 or int64, not {dtype}")
+    if num_blocks is None:
+        num_blocks = ((1 << 31) - 1) // (block_size if dtype == torch.int32 else 1)
+    if block_tables.is_cuda:
+        return SlotMapping(*native().build_slot_mapping(
+            context_lens, new_lens, block_tables, block_size, num_tokens, free_blocks,
+            num_blocks, dtype == torch.int64, status))
+    if context_lens.dim() != 1 or new_lens.shape != context_lens.shape:
+        raise ValueError("context_lens and new_lens must be [batch]")
+    if block_tables.dim() != 2 or block_tables.shape[0] < context_lens.numel():
+        raise ValueError("block_tables must be [>= batch, width]")
+    if block_size < 1 or num_tokens < 0:
+        raise ValueError("bad block_size or num_tokens")
+    return SlotMapping(*R.build_slot_mapping_ref(context_lens, new_lens, block_tables, block_size,
+                                                 num_tokens, free_blocks, num_blocks, dtype))
+
+
+def rotary_embedding(positions: torch.Tensor, query: torch.Tensor,
+                     key: Optional[torch.Tensor], head_size: int, cos_sin_cache: torch.Tensor,
+                     is_neox: bool = True, query_out: Optional[torch.Tensor] = None,
+                     key_out: Optional[torch.Tensor] = None,
+                     status: Optional[torch.Tensor] = None
+                     ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Rotate fresh ``query`` and ``key`` rows ([T, heads * D] or [T, heads, D],
+    any row stride) to ``positions``; returns (query, key) rotated, in new
+    tensors or in ``query_out`` / ``key_out`` (which may be the inputs).
+
+    The first ``cos_sin_cache.shape[1]`` elements of each head are rotated, the
+    others pass through.  ``cos_sin_cache``: one row of cosines and sines per
+    position (``reference.make_cos_sin_cache`` / ``make_scaled_cos_sin_cache``).
+    A position outside the table gives a zero row and is reported in ``status``.
+    """
+    if query.is_cuda:
+        if query_out is None:
+            query_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+        if key is not None and key_out is None:
+            key_out = torch.empty(key.shape, dtype=key.dtype, device=key.device)
+        native().rotary_embedding_and_cache(positions, query, key, None, None, None, None,
+                                            head_size, cos_sin_cache, is_neox, query_out, key_out,
+                                            status)
+        return query_out, key_out
+
+    def turn(x, out):
+        if x is None:
+            return None
+        y = R.rotary_embedding_ref(positions, x, head_size, cos_sin_cache, is_neox).to(x.dtype)
+        return y if out is None else out.copy_(y)
+
+    return turn(query, query_out), turn(key, key_out)
+
+
+def rotary_embedding_and_cache(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor,
+                               value: torch.Tensor, key_cache: torch.Tensor,
+                               value_cache: torch.Tensor, slot_mapping: torch.Tensor,
+                               head_size: int, cos_sin_cache: torch.Tensor, is_neox: bool = True,
+                               query_out: Optional[torch.Tensor] = None,
+                               key_out: Optional[torch.Tensor] = None,
+                               status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`rotary_embedding` that also writes the rotated keys and the values
+    to their pages: row t to slot ``slot_mapping[t]`` (int32 or int64, -1: not
+    written) of ``key_cache`` / ``value_cache`` [blocks, block size, KV heads, D]
+    (any strides with contiguous heads).  Returns the rotated queries; the
+    rotated keys are also kept when ``key_out`` is given.
+
+    Rows of equal slots overwrite one another in no fixed order.  A slot past
+    the cache, or a position outside the table, writes nothing to the pages and
+    is reported in ``status``."""
+    if query.is_cuda:
+        if query_out is None:
+            query_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+        native().rotary_embedding_and_cache(positions, query, key, value, key_cache, value_cache,
+                                            slot_mapping, head_size, cos_sin_cache, is_neox,
+                                            query_out, key_out, status)
+        return query_out
+    q, k = rotary_embedding(positions, query, key, head_size, cos_sin_cache, is_neox, query_out,
+                            key_out)
+    for rows, cache in ((k, key_cache), (value, value_cache)):
+        R.write_cache_ref(positions, rows, cache, slot_mapping, cos_sin_cache.shape[0])
+    return q
+
+
+def _attention_result(query, out, lse, return_lse):
+    out = out.to(query.dtype)
+    return (out, lse.float()) if return_lse else out
+
+
+def shared_prefix_attention(query: torch.Tensor, key_cache: torch.Tensor,
+                            value_cache: torch.Tensor, prefix_blocks: torch.Tensor,
+                            prefix_len: int, block_tables: torch.Tensor, seq_lens: torch.Tensor,
+                            scale: Optional[float] = None, softcap: float = 0.0,
+                            alibi_slopes: Optional[torch.Tensor] = None,
+                            return_lse: bool = False, status: Optional[torch.Tensor] = None
+                            ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """Attention of a batch whose requests share their first ``prefix_len``
+    tokens, read once for all of them.
+
+    ``query`` [B, H, D], or [B, q_len, H, D] for the last q_len tokens of each
+    request.  ``key_cache`` / ``value_cache`` [blocks, block size, KV heads, D].
+    ``prefix_blocks`` (int32): the shared blocks.  ``block_tables`` (int32
+    [>= B, width]) and ``seq_lens`` (int32 [B]): each request's own blocks and
+    tokens behind the prefix, the queries' own keys included.  Query i of a
+    request of n own tokens sees the whole prefix and its own keys 0 ..
+    n - q_len + i.  Scores are ``scale`` (default D^-0.5) times q.k, then
+    ``softcap * tanh(x / softcap)`` (0: no cap), then ``-alibi_slopes[h]`` times
+    the distance (fp32 [H]).
+
+    Returns [B, ..., H, D] and, with ``return_lse``, the fp32 log of each row's
+    sum.  A row that sees no key is zero with -inf.  Keys in a block outside the
+    cache, or past the end of a table row, are left out and reported in
+    ``status``.  On the device: bfloat16 or float16, D of 64 or 128, 16-byte
+    aligned cache rows.
+    """
+    if scale is None:
+        scale = query.shape[-1] ** -0.5
+    if query.is_cuda:
+        out, lse = native().shared_prefix_attention(
+            query, key_cache, value_cache, prefix_blocks, prefix_len, block_tables, seq_lens,
+            scale, softcap, alibi_slopes, return_lse, status)
+        return (out, lse) if return_lse else out
+    if query.dim() not in (3, 4) or query.shape[-2] % key_cache.shape[2]:
+        raise ValueError("query must be [B, H, D] or [B, q_len, H, D] with whole head groups")
+    if prefix_len < 0 or prefix_blocks.numel() * key_cache.shape[1] < prefix_len:
+        raise ValueError("prefix_blocks do not hold the prefix")
+    out, lse = R.shared_prefix_attention_ref(query, key_cache, value_cache, prefix_blocks,
+                                             prefix_len, block_tables, seq_lens, scale, softcap,
+                                             alibi_slopes)
+    return _attention_result(query, out, lse, return_lse)
+
+
+def position_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+                       q_positions: torch.Tensor, k_positions: Optional[torch.Tensor] = None,
+                       scale: Optional[float] = None, softcap: float = 0.0,
+                       alibi_slopes: Optional[torch.Tensor] = None,
+                       q_documents: Optional[torch.Tensor] = None,
+                       k_documents: Optional[torch.Tensor] = None,
+                       q_prefix_lens: Optional[torch.Tensor] = None, causal: bool = True,
+                       return_lse: bool = False
+                       ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """Attention of rows at any positions over keys at any positions: the rows
+    CacheBlend recomputes over the blended keys, or packed documents.
+
+    ``query`` [Tq, H, D] at ``q_positions``; ``key`` / ``value`` [Tk, KV heads, D]
+    at ``k_positions`` (int32 or int64; default 0, 1, 2, ...), in any order.  A
+    row sees a key when the key's position is at most its own (unless not
+    ``causal``) or below its ``q_prefix_lens`` (int32 [Tq]), and, with
+    ``q_documents`` / ``k_documents`` (int32), both are in the same document;
+    a negative document marks a padding row.  Scores as in
+    :func:`shared_prefix_attention`.
+
+    Returns [Tq, H, D] and, with ``return_lse``, the fp32 log of each row's sum;
+    a row that sees no key is zero with -inf.  On the device: bfloat16 or
+    float16, D of 64 or 128.
+    """
+    if scale is None:
+        scale = query.shape[-1] ** -0.5
+    if query.is_cuda:
+        out, lse = native().position_attention(
+            query, key, value, q_positions, k_positions, scale, softcap, alibi_slopes,
+            q_documents, k_documents, q_prefix_lens, causal, return_lse)
+        return (out, lse) if return_lse else out
+    if query.dim() != 3 or key.dim() != 3 or query.shape[1] % key.shape[1]:
+        raise ValueError("query [Tq, H, D] and key [Tk, KV heads, D] with whole head groups")
+    if (q_documents is None) != (k_documents is None):
+        raise ValueError("q_documents and k_documents go together")
+    out, lse = R.position_attention_ref(query, key, value, q_positions, k_positions, scale,
+                                        softcap, alibi_slopes, q_documents, k_documents,
+                                        q_prefix_lens, causal)
+    return _attention_result(query, out, lse, return_lse)
 
 
 # ----------------------------------------------------------------- misc

@@ -1,0 +1,112 @@
+// What the attention kernels share: their arguments, the score, and the row
+// that one warp computes by the definition.
+//
+// For a query row and the keys it sees
+//   x_j = scale * q . k_j,   x_j = cap * tanh(x_j / cap)      (cap > 0)
+//   x_j = x_j - slope_h * |p - p_j|                            (distance bias)
+//   o = sum_j exp(x_j - lse) v_j,   lse = log sum_j exp(x_j)
+// with every sum and statistic in fp32 and one rounding of o to the row's type.
+// A row that sees no key is zero with lse = -inf.  Keys it does not see are
+// never multiplied by a zero weight: whatever their rows hold stays out.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include "common.cuh"
+#include "serving_ops.h"
+
+namespace lmc {
+
+static_assert(sizeof(DeviceStatus) == kDeviceStatusBytes, "status layout");
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+template <typename T>
+__device__ __forceinline__ float2 pair_to_float(uint32_t w);
+template <>
+__device__ __forceinline__ float2 pair_to_float<__nv_bfloat16>(uint32_t w) {
+  return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162 *>(&w));
+}
+template <>
+__device__ __forceinline__ float2 pair_to_float<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<__half2 *>(&w));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pair_from_float(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pair_from_float<__nv_bfloat16>(float a, float b) {
+  __nv_bfloat162 w = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t *>(&w);
+}
+template <>
+__device__ __forceinline__ uint32_t pair_from_float<__half>(float a, float b) {
+  __half2 w = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t *>(&w);
+}
+
+// One query row on one warp; lane l holds elements [l D/32, (l + 1) D/32).
+template <typename T, int D>
+struct WarpRow {
+  static constexpr int E = D / 32;
+  float q[E], o[E], m, l;
+
+  __device__ __forceinline__ void load(const T *p, float *f) const {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(p + (threadIdx.x & 31) * E);
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      const float2 v = pair_to_float<T>(w[i]);
+      f[2 * i] = v.x, f[2 * i + 1] = v.y;
+    }
+  }
+
+  __device__ __forceinline__ void start(const T *row) {
+    load(row, q);
+#pragma unroll
+    for (int i = 0; i < E; ++i) o[i] = 0.f;
+    m = -INFINITY;
+    l = 0.f;
+  }
+
+  // bias is subtracted after the cap
+  __device__ __forceinline__ void add(const T *k, const T *v, float scale, float cap,
+                                      float bias) {
+    float kf[E], vf[E];
+    load(k, kf);
+    load(v, vf);
+    float x = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) x += q[i] * kf[i];
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) x += __shfl_xor_sync(0xffffffffu, x, s);
+    x *= scale;
+    if (cap > 0.f) x = cap * tanhf(x / cap);
+    x = (x - bias) * kLog2e;
+    const float top = fmaxf(m, x);
+    if (top == -INFINITY) return;  // a score of -inf before any other
+    const float keep = exp2f(m - top), w = exp2f(x - top);
+    m = top;
+    l = l * keep + w;
+#pragma unroll
+    for (int i = 0; i < E; ++i) o[i] = o[i] * keep + w * vf[i];
+  }
+
+  __device__ __forceinline__ void finish(T *row, float *lse) const {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint32_t *w = reinterpret_cast<uint32_t *>(row + (threadIdx.x & 31) * E);
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i)
+      w[i] = pair_from_float<T>(o[2 * i] * inv, o[2 * i + 1] * inv);
+    if (lse != nullptr && (threadIdx.x & 31) == 0)
+      *lse = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+  }
+};
+
+__device__ __forceinline__ long long position_at(const void *p, bool is_long, int i) {
+  return is_long ? static_cast<const long long *>(p)[i]
+                 : static_cast<long long>(static_cast<const int *>(p)[i]);
+}
+
+}  // namespace lmc

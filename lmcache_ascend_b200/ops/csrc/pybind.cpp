@@ -85,6 +85,32 @@ void rotary_embedding_k_fused_layers(const at::Tensor &old_positions,
                                      const std::vector<at::Tensor> &keys, int64_t head_size,
                                      const at::Tensor &cos_sin_cache, bool is_neox,
                                      const c10::optional<at::Tensor> &slot_mapping);
+// slot_kernels.cu
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>
+build_slot_mapping(const at::Tensor &context_lens, const at::Tensor &new_lens,
+                   at::Tensor &block_tables, int64_t block_size, int64_t num_tokens,
+                   const c10::optional<at::Tensor> &free_blocks, int64_t num_blocks,
+                   bool long_slots, const c10::optional<at::Tensor> &status);
+// rope_cache_kernels.cu
+void rotary_embedding_and_cache(
+    const at::Tensor &positions, const at::Tensor &query, const c10::optional<at::Tensor> &key,
+    const c10::optional<at::Tensor> &value, const c10::optional<at::Tensor> &key_cache,
+    const c10::optional<at::Tensor> &value_cache, const c10::optional<at::Tensor> &slot_mapping,
+    int64_t head_size, const at::Tensor &cos_sin_cache, bool is_neox, at::Tensor &query_out,
+    const c10::optional<at::Tensor> &key_out, const c10::optional<at::Tensor> &status);
+// attention_kernels.cu
+std::tuple<at::Tensor, c10::optional<at::Tensor>> shared_prefix_attention(
+    const at::Tensor &query, const at::Tensor &key_cache, const at::Tensor &value_cache,
+    const at::Tensor &prefix_blocks, int64_t prefix_len, const at::Tensor &block_tables,
+    const at::Tensor &own_lens, double scale, double softcap,
+    const c10::optional<at::Tensor> &alibi_slopes, bool return_lse,
+    const c10::optional<at::Tensor> &status);
+std::tuple<at::Tensor, c10::optional<at::Tensor>> position_attention(
+    const at::Tensor &query, const at::Tensor &key, const at::Tensor &value,
+    const at::Tensor &q_positions, const c10::optional<at::Tensor> &k_positions, double scale,
+    double softcap, const c10::optional<at::Tensor> &alibi_slopes,
+    const c10::optional<at::Tensor> &q_documents, const c10::optional<at::Tensor> &k_documents,
+    const c10::optional<at::Tensor> &q_prefix_lens, bool causal, bool return_lse);
 // dma.cu
 void dma_copy_batch(const at::Tensor &dsts, const at::Tensor &srcs, const at::Tensor &sizes);
 double dma_copy_batch_timed(const at::Tensor &dsts, const at::Tensor &srcs,
@@ -209,6 +235,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rotary_embedding_k_fused", &rotary_embedding_k_fused, py::arg("old_positions"),
         py::arg("new_positions"), py::arg("key"), py::arg("head_size"),
         py::arg("cos_sin_cache"), py::arg("is_neox"), py::arg("slot_mapping") = py::none());
+
+  m.def("build_slot_mapping", &build_slot_mapping);
+  m.def("rotary_embedding_and_cache", &rotary_embedding_and_cache);
+  m.def("shared_prefix_attention", &shared_prefix_attention);
+  m.def("position_attention", &position_attention);
 
   m.def("layerwise_prefill_dma_copy", &dma_copy_batch);
   m.def("layerwise_prefill_dma_copy_diagnose", &dma_copy_batch_timed);

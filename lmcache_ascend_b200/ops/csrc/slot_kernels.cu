@@ -1,0 +1,215 @@
+// Block tables and slot maps from request lengths, on the device, in one launch.
+//
+// Request b holds c_b tokens in its pages and gets n_b new ones.  With pages of
+// `bs` slots it has ceil(c_b / bs) pages and needs ceil((c_b + n_b) / bs); the
+// missing ones come from the free list in request order:
+//   off_b = sum_{i<b} (need_i - have_i),  table[b, have_b + j] = free[off_b + j].
+// The new tokens of all requests are packed: token t of request b (start_b =
+// sum_{i<b} n_i) has position p = c_b + t - start_b and slot
+//   page(b, p / bs) * bs + p % bs.
+//
+// Two prefix sums over the requests and then independent work per token and
+// per new page.  No block waits for another: every block sums the lengths
+// itself (8 bytes a request, from L2), keeps one partial sum per thread in
+// shared memory, and takes an even share of the tokens, of the new pages and
+// of the requests.  A token's page is read from the table only in columns the
+// request had before, and from the free list otherwise, so no block depends on
+// table entries written by another.  Bound by the launch for a decode batch and
+// by the 20 bytes written per token for prompts.
+#include <algorithm>
+
+#include "common.cuh"
+#include "serving_ops.h"
+
+namespace lmc {
+namespace {
+
+constexpr int kSlotThreads = 512;
+constexpr int kTokensPerBlock = 2048;
+
+enum SlotWhere : int { kWhereLength = 1, kWhereTable = 2, kWhereFree = 3, kWhereTotal = 4 };
+
+struct Need {
+  long long tokens, pages;
+};
+
+// Pages of `tokens` slots (< 2^32: two lengths below 2^31), in 32-bit divisions.
+__device__ __forceinline__ long long pages_of(long long tokens, int block_size) {
+  const unsigned t = static_cast<unsigned>(tokens), bs = static_cast<unsigned>(block_size);
+  return t / bs + (t % bs != 0);
+}
+
+template <typename LT>
+__device__ __forceinline__ long long length_of(const void *p, int b) {
+  const long long v = static_cast<long long>(static_cast<const LT *>(p)[b]);
+  // a length below zero counts as zero; one past 2^31 - 1 as that
+  return v < 0 ? 0 : (v > 0x7fffffffll ? 0x7fffffffll : v);
+}
+
+template <typename LT>
+__device__ __forceinline__ Need need_of(const SlotArgs &a, int b) {
+  const long long c = length_of<LT>(a.ctx, b), n = length_of<LT>(a.fresh, b);
+  return {n, a.grow ? pages_of(c + n, a.block_size) - pages_of(c, a.block_size) : 0};
+}
+
+// Exclusive prefix of the request sums at each thread's segment of requests.
+struct Sums {
+  long long tokens[kSlotThreads + 1];
+  long long pages[kSlotThreads + 1];
+};
+
+// Largest i with v[i] <= x (v ascending, v[0] = 0 <= x).
+__device__ __forceinline__ int last_leq(const long long *v, int n, long long x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (v[mid] <= x)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+template <typename LT, typename OT>
+__global__ void __launch_bounds__(kSlotThreads) slot_mapping_kernel(SlotArgs a) {
+  __shared__ Sums s;
+  __shared__ long long warp_tok[kSlotThreads / 32], warp_pg[kSlotThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int seg = (a.batch + kSlotThreads - 1) / kSlotThreads;
+  const int b0 = min(a.batch, tid * seg), b1 = min(a.batch, b0 + seg);
+  Need mine = {0, 0};
+  for (int b = b0; b < b1; ++b) {
+    const Need n = need_of<LT>(a, b);
+    mine.tokens += n.tokens;
+    mine.pages += n.pages;
+  }
+  long long ti = mine.tokens, pi = mine.pages;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, ti, o), y = __shfl_up_sync(0xffffffffu, pi, o);
+    if (lane >= o) ti += x, pi += y;
+  }
+  if (lane == 31) warp_tok[warp] = ti, warp_pg[warp] = pi;
+  __syncthreads();
+  long long tb = 0, pb = 0;
+  for (int w = 0; w < warp; ++w) tb += warp_tok[w], pb += warp_pg[w];
+  s.tokens[tid] = tb + ti - mine.tokens;
+  s.pages[tid] = pb + pi - mine.pages;
+  if (tid == kSlotThreads - 1) s.tokens[kSlotThreads] = tb + ti, s.pages[kSlotThreads] = pb + pi;
+  __syncthreads();
+  const long long total_tokens = s.tokens[kSlotThreads], total_pages = s.pages[kSlotThreads];
+
+  // --- per request: this block's share is written by the threads that summed it
+  const int share = (a.batch + gridDim.x - 1) / gridDim.x;
+  const int r0 = blockIdx.x * share, r1 = min(a.batch, r0 + share);
+  if (b0 < r1 && b1 > r0) {
+    long long t = s.tokens[tid], p = s.pages[tid];
+    for (int b = b0; b < b1; ++b) {
+      const Need n = need_of<LT>(a, b);
+      if (b >= r0 && b < r1) {
+        const long long c = length_of<LT>(a.ctx, b);
+        a.start[b] = static_cast<int>(t);
+        a.taken[b] = static_cast<int>(p);
+        a.seq_lens[b] = static_cast<int>(min(c + n.tokens, 0x7fffffffll));
+        if (static_cast<long long>(static_cast<const LT *>(a.ctx)[b]) != c ||
+            static_cast<long long>(static_cast<const LT *>(a.fresh)[b]) != n.tokens)
+          report_status(a.status, kStatusBadIndex, kWhereLength, b, 0);
+        if (b == a.batch - 1) {
+          a.start[a.batch] = static_cast<int>(t + n.tokens);
+          a.taken[a.batch] = static_cast<int>(p + n.pages);
+        }
+      }
+      t += n.tokens;
+      p += n.pages;
+    }
+  }
+  if (blockIdx.x == 0 && tid == 0) {
+    if (a.batch == 0) a.start[0] = 0, a.taken[0] = 0;
+    if (total_tokens > a.num_tokens)
+      report_status(a.status, kStatusBadIndex, kWhereTotal, total_tokens, a.num_tokens);
+    if (total_pages > a.num_free)
+      report_status(a.status, kStatusBadIndex, kWhereFree, total_pages, a.num_free);
+  }
+
+  // --- new pages into the tables
+  for (long long j = static_cast<long long>(blockIdx.x) * kSlotThreads + tid; j < total_pages;
+       j += static_cast<long long>(gridDim.x) * kSlotThreads) {
+    const int g = last_leq(s.pages, kSlotThreads, j);
+    int b = g * seg;
+    long long p = s.pages[g];
+    long long n = need_of<LT>(a, b).pages;
+    while (j >= p + n) {
+      p += n;
+      n = need_of<LT>(a, ++b).pages;
+    }
+    const long long c = length_of<LT>(a.ctx, b);
+    const long long col = pages_of(c, a.block_size) + (j - p);
+    if (col < a.width)
+      a.tables[b * a.table_stride + col] = j < a.num_free ? a.free_blocks[j] : -1;
+    else
+      report_status(a.status, kStatusBadIndex, kWhereTable, b, col);
+  }
+
+  // --- tokens
+  OT *slots = static_cast<OT *>(a.slots);
+  OT *positions = static_cast<OT *>(a.positions);
+  const long long t0 = static_cast<long long>(blockIdx.x) * kTokensPerBlock;
+  const long long t1 = min(a.num_tokens, t0 + kTokensPerBlock);
+  for (long long t = t0 + tid; t < t1; t += kSlotThreads) {
+    if (t >= total_tokens) {  // rows behind the last request
+      slots[t] = -1;
+      positions[t] = 0;
+      a.request_ids[t] = -1;
+      continue;
+    }
+    const int g = last_leq(s.tokens, kSlotThreads, t);
+    int b = g * seg;
+    long long start = s.tokens[g], pages = s.pages[g];
+    Need n = need_of<LT>(a, b);
+    while (t >= start + n.tokens) {
+      start += n.tokens;
+      pages += n.pages;
+      n = need_of<LT>(a, ++b);
+    }
+    const long long c = length_of<LT>(a.ctx, b);
+    const long long pos = c + (t - start);
+    const long long col = static_cast<unsigned>(pos) / static_cast<unsigned>(a.block_size);
+    const long long have = pages_of(c, a.block_size);
+    long long page = -1;
+    if (col >= a.width) {
+      report_status(a.status, kStatusBadIndex, kWhereTable, b, col);
+    } else if (a.grow && col >= have) {
+      const long long j = pages + (col - have);
+      if (j < a.num_free) page = a.free_blocks[j];
+    } else {
+      page = a.tables[b * a.table_stride + col];
+    }
+    long long slot = -1;
+    if (page >= 0 && page < a.num_blocks)
+      slot = page * a.block_size + (pos - col * a.block_size);
+    else if (col < a.width)
+      report_status(a.status, kStatusBadSlot, b, page, a.num_blocks);
+    slots[t] = static_cast<OT>(slot);
+    positions[t] = static_cast<OT>(pos);
+    a.request_ids[t] = b;
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_slot_mapping(const SlotArgs &a, bool long_lens, bool long_slots,
+                                cudaStream_t stream) {
+  const unsigned grid = static_cast<unsigned>(
+      std::max(1ll, (a.num_tokens + kTokensPerBlock - 1) / kTokensPerBlock));
+#define LMC_SLOTS(LT, OT) slot_mapping_kernel<LT, OT><<<grid, kSlotThreads, 0, stream>>>(a)
+  if (!long_lens) {
+    if (long_slots) LMC_SLOTS(int, long long); else LMC_SLOTS(int, int);
+  } else {
+    if (long_slots) LMC_SLOTS(long long, long long); else LMC_SLOTS(long long, int);
+  }
+#undef LMC_SLOTS
+  return cudaGetLastError();
+}
+
+}  // namespace lmc

@@ -7,12 +7,16 @@ CPU test tier).  They implement the same formats as the CUDA kernels:
 * CacheGen (``cachegen_kernels.cu``): aligned power-of-two CDF with the code
   length in the low 4 bits of each entry, MSB-first prefix codes, decode
   from an inclusive prefix sum of stream lengths;
-* RoPE delta re-rotation (``pos_kernels.cu``).
+* RoPE delta re-rotation (``pos_kernels.cu``);
+* slot maps from request lengths, rotary positions with cache writes, and the
+  attention operators (``slot_kernels.cu``, ``rope_cache_kernels.cu``,
+  ``attention_kernels.cu``).
 """
 
 from __future__ import annotations
 
-from typing import List, Tuple
+import math
+from typing import Any, Dict, List, Optional, Tuple
 
 import numpy as np
 import torch
@@ -213,3 +217,206 @@ def make_cos_sin_cache(max_pos: int, rot_dim: int, base: float = 10000.0,
     t = torch.arange(max_pos, dtype=torch.float64)
     f = torch.outer(t, inv)
     return torch.cat([f.cos(), f.sin()], dim=-1).to(dtype)
+
+
+def make_scaled_cos_sin_cache(max_pos: int, rot_dim: int, base: float = 10000.0,
+                              scaling: Optional[Dict[str, Any]] = None,
+                              dtype=torch.float32) -> torch.Tensor:
+    """``make_cos_sin_cache`` with the frequencies scaled for long contexts;
+    angles in 64 bits.  ``scaling`` is a ``rope_scaling`` dict:
+
+    * ``linear``: every frequency divided by ``factor``;
+    * ``dynamic``: the base grown so that ``max_pos`` positions keep the slowest
+      turn of ``original_max_position_embeddings`` (``factor`` times as many);
+    * ``llama3``: frequencies of more than ``high_freq_factor`` turns over the
+      original context kept, of fewer than ``low_freq_factor`` divided by
+      ``factor``, a ramp between;
+    * ``yarn``: a ramp over the dimensions between ``beta_fast`` and ``beta_slow``
+      turns, and a gain of ``attention_factor`` (default 0.1 ln(factor) + 1) on
+      the cosines and sines.
+    """
+    scaling = dict(scaling or {})
+    kind = scaling.get("rope_type", scaling.get("type", "default"))
+    dims = torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim
+    gain = 1.0
+    if kind == "default":
+        inv = 1.0 / base ** dims
+    elif kind == "linear":
+        inv = base ** -dims / float(scaling["factor"])
+    elif kind == "dynamic":
+        f, orig = float(scaling["factor"]), int(scaling["original_max_position_embeddings"])
+        if rot_dim <= 2:
+            raise ValueError("dynamic rope scaling needs a rotated part of more than one pair")
+        grown = base * max(1.0, f * max_pos / orig - (f - 1)) ** (rot_dim / (rot_dim - 2))
+        inv = grown ** -dims
+    elif kind == "llama3":
+        f, orig = float(scaling["factor"]), int(scaling["original_max_position_embeddings"])
+        lo, hi = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        inv = base ** -dims
+        turns = orig * inv / (2 * math.pi)
+        ramp = ((turns - lo) / (hi - lo)).clamp(0, 1) if hi > lo else (turns >= hi).double()
+        inv = inv / f * (1 - ramp) + inv * ramp
+    elif kind == "yarn":
+        f, orig = float(scaling["factor"]), int(scaling["original_max_position_embeddings"])
+
+        def dim_of(turns: float) -> float:
+            return rot_dim * math.log(orig / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+        lo = max(math.floor(dim_of(float(scaling.get("beta_fast", 32.0)))), 0)
+        hi = min(math.ceil(dim_of(float(scaling.get("beta_slow", 1.0)))), rot_dim - 1)
+        ramp = ((torch.arange(rot_dim // 2, dtype=torch.float64) - lo)
+                / max(hi - lo, 0.001)).clamp(0, 1)
+        inv = base ** -dims
+        inv = inv / f * ramp + inv * (1 - ramp)
+        given = scaling.get("attention_factor")
+        gain = float(given) if given is not None else (0.1 * math.log(f) + 1.0 if f > 1 else 1.0)
+    else:
+        raise ValueError(f"unknown rope scaling {kind!r}")
+    a = torch.outer(torch.arange(max_pos, dtype=torch.float64), inv)
+    return (torch.cat([a.cos(), a.sin()], dim=-1) * gain).to(dtype)
+
+
+# ---------------------------------------------------------------------------
+# Serving operators next to the cache
+# ---------------------------------------------------------------------------
+def build_slot_mapping_ref(context_lens, new_lens, block_tables, block_size, num_tokens,
+                           free_blocks=None, num_blocks=None, dtype=torch.int64):
+    """One request after the other; grows ``block_tables`` in place.  Returns
+    (slots, positions, request ids, query_start_loc, seq_lens, taken)."""
+    ctx = [max(0, int(c)) for c in context_lens]
+    new = [max(0, int(n)) for n in new_lens]
+    free = None if free_blocks is None else [int(x) for x in free_blocks]
+    limit = (1 << 31) - 1 if num_blocks is None else num_blocks
+    width = block_tables.shape[1]
+    slots = torch.full((num_tokens,), -1, dtype=dtype)
+    positions = torch.zeros(num_tokens, dtype=dtype)
+    ids = torch.full((num_tokens,), -1, dtype=torch.int32)
+    start, taken = [0], [0]
+    for b, (c, n) in enumerate(zip(ctx, new)):
+        have, need = -(-c // block_size), -(-(c + n) // block_size)
+        got = 0
+        if free is not None:
+            for j in range(need - have):
+                at = taken[-1] + j
+                if have + j < width:
+                    block_tables[b, have + j] = free[at] if at < len(free) else -1
+            got = need - have
+        for i in range(n):
+            t = start[-1] + i
+            if t >= num_tokens:
+                break
+            p = c + i
+            col = p // block_size
+            page = int(block_tables[b, col]) if col < width else -1
+            if 0 <= page < limit:
+                slots[t] = page * block_size + p % block_size
+            positions[t] = p
+            ids[t] = b
+        start.append(start[-1] + n)
+        taken.append(taken[-1] + got)
+    i32 = torch.int32
+    return (slots, positions, ids, torch.tensor(start, dtype=i32),
+            torch.tensor([c + n for c, n in zip(ctx, new)], dtype=i32),
+            torch.tensor(taken, dtype=i32))
+
+
+def rotary_embedding_ref(positions, x, head_size, cos_sin_cache, is_neox, compute=torch.float32):
+    """Rows x [T, heads * D] or [T, heads, D] rotated by the table rows of
+    ``positions``; rows whose position is outside the table are zero.  In
+    ``compute``, not rounded."""
+    T, rot = positions.numel(), cos_sin_cache.shape[1]
+    half = rot // 2
+    ok = (positions >= 0) & (positions < cos_sin_cache.shape[0])
+    cs = cos_sin_cache.to(compute)[positions.long() * ok]
+    c, s = cs[:, None, :half], cs[:, None, half:]
+    y = x.reshape(T, -1, head_size).to(compute).clone()
+    first = slice(0, half) if is_neox else slice(0, rot, 2)
+    second = slice(half, rot) if is_neox else slice(1, rot, 2)
+    a, b = y[..., first].clone(), y[..., second].clone()
+    y[..., first], y[..., second] = a * c - b * s, b * c + a * s
+    y[~ok] = 0
+    return y.reshape(x.shape)
+
+
+def write_cache_ref(positions, rows, cache, slot_mapping, max_pos):
+    """Rows [T, KH, D] to their slots of a [NB, BS, KH, D] cache; rows of slot
+    -1 or of a position outside the table stay out."""
+    bs = cache.shape[1]
+    sm = slot_mapping.long()
+    keep = (sm >= 0) & (sm < cache.shape[0] * bs) & (positions >= 0) & (positions < max_pos)
+    cache[sm[keep] // bs, sm[keep] % bs] = rows.reshape(
+        rows.shape[0], cache.shape[2], cache.shape[3])[keep].to(cache.dtype)
+
+
+def attend_ref(q, k, v, visible, distance, scale, softcap, slopes):
+    """q [H, R, D] over k, v [KH, N, D] (already in the type to compute in);
+    ``visible`` and ``distance`` [R, N].  Keys that a row does not see take no
+    part.  Returns (o [H, R, D], lse [H, R]); a row without keys is 0, -inf."""
+    H, R, D = q.shape
+    rep = H // k.shape[0]
+    o = torch.zeros_like(q)
+    lse = torch.full((H, R), -math.inf, dtype=q.dtype)
+    for h in range(H):
+        x = (q[h] @ k[h // rep].T) * scale
+        if softcap:
+            x = softcap * torch.tanh(x / softcap)
+        if slopes is not None:
+            x = x - slopes[h].to(q.dtype) * distance.to(q.dtype)
+        x = torch.where(visible, x, torch.full_like(x, -math.inf))
+        some = visible.any(dim=1)
+        m = x.amax(dim=1, keepdim=True) if x.shape[1] else x.new_full((R, 1), -math.inf)
+        w = torch.exp(x - torch.where(some[:, None], m, torch.zeros_like(m)))
+        total = w.sum(dim=1)
+        y = w @ v[h // rep]
+        for r in torch.nonzero(~torch.isfinite(y).all(dim=1)).flatten().tolist():
+            sel = visible[r]  # a key it does not see holds an inf or NaN
+            y[r] = w[r, sel] @ v[h // rep][sel]
+        o[h] = torch.where(some[:, None], y / total[:, None], torch.zeros_like(y))
+        lse[h] = torch.where(some, m[:, 0] + torch.log(total), lse[h])
+    return o, lse
+
+
+def shared_prefix_attention_ref(query, key_cache, value_cache, prefix_blocks, prefix_len,
+                                block_tables, seq_lens, scale, softcap=0.0, alibi_slopes=None,
+                                compute=torch.float32):
+    """Oracle of ``api.shared_prefix_attention`` in ``compute``, not rounded."""
+    q4 = query.unsqueeze(1) if query.dim() == 3 else query
+    B, Tq, H, D = q4.shape
+    NB, bs = key_cache.shape[0], key_cache.shape[1]
+    out = torch.zeros(B, Tq, H, D, dtype=compute)
+    lse = torch.full((B, Tq, H), -math.inf, dtype=compute)
+    for b in range(B):
+        n = max(0, int(seq_lens[b]))
+        cols = min(-(-n // bs), block_tables.shape[1])
+        page = torch.cat([prefix_blocks[:-(-prefix_len // bs)].long().repeat_interleave(bs)[
+            :prefix_len], block_tables[b, :cols].long().repeat_interleave(bs)[:n]])
+        off = torch.cat([torch.arange(prefix_len) % bs, torch.arange(min(n, cols * bs)) % bs])
+        ok = (page >= 0) & (page < NB)
+        k = key_cache[page * ok, off].to(compute).transpose(0, 1)
+        v = value_cache[page * ok, off].to(compute).transpose(0, 1)
+        at = torch.arange(page.numel())
+        i = torch.arange(Tq)[:, None]
+        visible = ok[None] & ((at < prefix_len) | (at - prefix_len <= n - Tq + i))
+        distance = (prefix_len + n - Tq + i - at).abs()
+        o, e = attend_ref(q4[b].to(compute).transpose(0, 1), k, v, visible, distance, scale,
+                          softcap, alibi_slopes)
+        out[b], lse[b] = o.transpose(0, 1), e.T
+    return out.reshape(query.shape), lse.reshape(query.shape[:-1])
+
+
+def position_attention_ref(query, key, value, q_positions, k_positions, scale, softcap=0.0,
+                           alibi_slopes=None, q_documents=None, k_documents=None,
+                           q_prefix_lens=None, causal=True, compute=torch.float32):
+    """Oracle of ``api.position_attention`` in ``compute``, not rounded."""
+    qp = q_positions.long()
+    kp = torch.arange(key.shape[0]) if k_positions is None else k_positions.long()
+    limit = qp + 1 if causal else torch.full_like(qp, 1 << 40)  # no row is that far
+    if q_prefix_lens is not None:
+        limit = torch.maximum(limit, q_prefix_lens.long())
+    visible = kp[None] < limit[:, None]
+    if q_documents is not None:
+        visible &= (q_documents[:, None] == k_documents[None]) & (q_documents[:, None] >= 0)
+    o, e = attend_ref(query.to(compute).transpose(0, 1), key.to(compute).transpose(0, 1),
+                      value.to(compute).transpose(0, 1), visible,
+                      (qp[:, None] - kp[None]).abs(), scale, softcap, alibi_slopes)
+    return o.transpose(0, 1), e.T
