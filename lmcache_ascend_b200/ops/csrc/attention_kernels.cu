@@ -1,5 +1,5 @@
-// Attention next to the cache: a batch over a shared prefix in pages, and rows
-// at given positions over dense keys.  One warp per row, by the definition.
+// Attention of a batch over a shared prefix in pages: one warp per row, by the
+// definition.
 #include <algorithm>
 
 #include "attention.cuh"
@@ -46,32 +46,6 @@ __global__ void __launch_bounds__(128) paged_rows_kernel(PagedArgs a) {
   }
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(128) position_rows_kernel(PositionArgs a) {
-  const long long rows = static_cast<long long>(a.q_tokens) * a.heads;
-  const int group = a.heads / a.kv_heads;
-  for (long long r = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5); r < rows;
-       r += static_cast<long long>(gridDim.x) * 4) {
-    const int h = static_cast<int>(r % a.heads);
-    const int t = static_cast<int>(r / a.heads);
-    const long long pos = position_at(a.q_pos, a.long_q_pos, t);
-    long long limit = a.causal ? pos + 1 : (1ll << 40);
-    if (a.q_prefix) limit = max(limit, static_cast<long long>(a.q_prefix[t]));
-    const int doc = a.q_doc ? a.q_doc[t] : 0;
-    const float slope = a.slopes ? a.slopes[h] : 0.f;
-    WarpRow<T, D> row;
-    row.start(static_cast<const T *>(a.q) + t * a.q_token + h * a.q_head);
-    for (int j = 0; j < a.k_tokens; ++j) {
-      const long long kp = a.k_pos ? position_at(a.k_pos, a.long_k_pos, j) : j;
-      if (doc < 0 || kp >= limit || (a.k_doc && a.k_doc[j] != doc)) continue;
-      row.add(static_cast<const T *>(a.k) + j * a.k_token + h / group * a.k_head,
-              static_cast<const T *>(a.v) + j * a.v_token + h / group * a.v_head, a.scale,
-              a.softcap, slope * fabsf(static_cast<float>(pos - kp)));
-    }
-    row.finish(static_cast<T *>(a.out) + r * D, a.lse ? a.lse + r : nullptr);
-  }
-}
-
 }  // namespace
 
 cudaError_t launch_shared_prefix_attention(const PagedArgs &a, RowType type, int dim,
@@ -79,20 +53,6 @@ cudaError_t launch_shared_prefix_attention(const PagedArgs &a, RowType type, int
   const long long rows = static_cast<long long>(a.batch) * a.q_len * a.heads;
   const unsigned grid = static_cast<unsigned>(std::min((rows + 3) / 4, 1ll << 20));
 #define LMC_ROWS(T, D) paged_rows_kernel<T, D><<<grid, 128, 0, stream>>>(a)
-  if (type == RowType::kBFloat16) {
-    if (dim == 64) LMC_ROWS(__nv_bfloat16, 64); else LMC_ROWS(__nv_bfloat16, 128);
-  } else {
-    if (dim == 64) LMC_ROWS(__half, 64); else LMC_ROWS(__half, 128);
-  }
-#undef LMC_ROWS
-  return cudaGetLastError();
-}
-
-cudaError_t launch_position_attention(const PositionArgs &a, RowType type, int dim,
-                                      cudaStream_t stream) {
-  const long long rows = static_cast<long long>(a.q_tokens) * a.heads;
-  const unsigned grid = static_cast<unsigned>(std::min((rows + 3) / 4, 1ll << 20));
-#define LMC_ROWS(T, D) position_rows_kernel<T, D><<<grid, 128, 0, stream>>>(a)
   if (type == RowType::kBFloat16) {
     if (dim == 64) LMC_ROWS(__nv_bfloat16, 64); else LMC_ROWS(__nv_bfloat16, 128);
   } else {

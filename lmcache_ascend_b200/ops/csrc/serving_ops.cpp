@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <limits>
 
 #include "serving_ops.h"
 
@@ -77,7 +78,8 @@ bool cache_aligned(const at::Tensor &x) {
 bool vector_rows(const at::Tensor &x) {
   const int64_t es = x.element_size(), last = x.dim() - 1;
   bool ok = reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && x.stride(last) == 1;
-  for (int64_t d = 0; d < last; ++d) ok = ok && (x.size(d) <= 1 || x.stride(d) * es % 16 == 0);
+  for (int64_t d = 0; d < last; ++d)
+    ok = ok && (x.size(d) <= 1 || (x.stride(d) > 0 && x.stride(d) * es % 16 == 0));
   return ok;
 }
 
@@ -90,7 +92,7 @@ at::Tensor with_vector_rows(const at::Tensor &x) {
 void check_scores(const char *op, double scale, double softcap,
                   const c10::optional<at::Tensor> &slopes, int64_t heads,
                   const c10::Device &dev) {
-  TORCH_CHECK(std::isfinite(scale), op, ": scale must be finite");
+  TORCH_CHECK(std::isfinite(scale) && scale > 0, op, ": scale must be positive and finite");
   TORCH_CHECK(std::isfinite(softcap) && softcap >= 0, op, ": softcap must be >= 0 (0: none)");
   if (slopes.has_value()) {
     check_dense(*slopes, op, "alibi_slopes", dev, at::kFloat);
@@ -396,6 +398,11 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> position_attention(
   c10::optional<at::Tensor> lse;
   if (return_lse) lse = at::empty({Tq, H}, query.options().dtype(at::kFloat));
   if (Tq == 0) return {out, lse};
+  if (Tk == 0) {
+    out.zero_();
+    if (return_lse) lse->fill_(-std::numeric_limits<float>::infinity());
+    return {out, lse};
+  }
   PositionArgs a = {};
   a.q = q.data_ptr(), a.k = k.data_ptr(), a.v = v.data_ptr();
   a.out = out.data_ptr();
@@ -415,7 +422,10 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> position_attention(
   a.heads = static_cast<int>(H), a.kv_heads = static_cast<int>(KH);
   a.causal = causal;
   a.scale = static_cast<float>(scale), a.softcap = static_cast<float>(softcap);
+  const auto workspace = at::empty({position_attention_workspace(a, static_cast<int>(D))},
+                                   query.options().dtype(at::kByte));
   C10_CUDA_CHECK(launch_position_attention(a, row_type(dt), static_cast<int>(D),
+                                           workspace.data_ptr(),
                                            at::cuda::getCurrentCUDAStream().stream()));
   return {out, lse};
 }

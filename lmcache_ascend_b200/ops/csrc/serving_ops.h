@@ -82,7 +82,9 @@ cudaError_t launch_rope_cache(const RopeArgs &a, RowType rows, RowType table, bo
                               cudaStream_t stream);
 cudaError_t launch_shared_prefix_attention(const PagedArgs &a, RowType type, int dim,
                                            cudaStream_t stream);
+// Bytes of device workspace (16-byte aligned) that the launch takes.
+long long position_attention_workspace(const PositionArgs &a, int dim);
 cudaError_t launch_position_attention(const PositionArgs &a, RowType type, int dim,
-                                      cudaStream_t stream);
+                                      void *workspace, cudaStream_t stream);
 
 }  // namespace lmc

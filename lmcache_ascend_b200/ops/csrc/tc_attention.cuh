@@ -1,0 +1,572 @@
+// Attention of many rows over a stream of keys on the tensor cores.
+//
+// A block owns 256 rows of one KV head, as two tiles of 128: rows are (token,
+// query head of the group) pairs, token-major, so heads that share keys share
+// their loads whatever the group's size.  Keys come in tiles of 128.  Per key
+// tile and row tile
+//   S = Q K^T            tcgen05, both operands in shared memory, S in TMEM
+//   P = exp2(S c - m)    a thread per row: S from TMEM to registers, its running
+//                        maximum m and sum l, P as 16-bit back over S in TMEM
+//   O = O + P V          tcgen05, P from TMEM, V as it lies (MN-major)
+// While one tile's scores are in the registers the tensor cores work on the
+// other's.  m only moves when the maximum grows by more than 2^8, so O in TMEM
+// is seldom rescaled (by the thread that owns the row; P stays below 2^8 and
+// sums are fp32, so nothing is lost).
+//
+// Roles: warps 0-3 and 4-7 one row tile each, warp 8 issues the mma, warp 9 the
+// TMA loads through a ring of four 128-key stages (K and V alternate); they give
+// registers to the row tiles, whose threads hold a row of 128 scores each
+// (384 threads x 168 at launch = 256 x 216 + 128 x 72).
+// 256 rows a block because a K/V tile then feeds 256 flop a byte from L2.
+#pragma once
+#include "attention.cuh"
+#include "tcgen05.cuh"
+
+namespace lmc {
+
+constexpr int kTileM = 128, kTileN = 128, kBlockRows = 256;
+constexpr int kStages = 4;
+constexpr int kTcThreads = 384;
+constexpr float kLazy = 8.f;  // log2 of how far P may pass 1 before O is rescaled
+
+// Dense keys: positions and documents of a key tile.
+struct TileStats {
+  int pos_min, pos_max, doc_min, doc_max;
+};
+
+struct TcArgs {
+  const void *q;
+  void *out;      // [tokens, H, D] in the rows' type, when slices == 0
+  float *lse;     // [tokens, H] or null
+  float *part_o;  // [slices, tokens * H, D] normalised, when slices > 0
+  float *part_lse;  // [slices, tokens * H], log2
+  const float *slopes;
+  long long q_batch, q_token, q_head;
+  int tokens, q_len, heads, group;
+  int k_tiles, tiles_per_slice, slices;
+  float scale_log2, cap_in, cap_out;  // x = s scale_log2, or cap_out tanh(s cap_in)
+  // dense keys (prepared arrays, padded to whole tiles)
+  PositionArgs pos;
+  const int *k_pos32, *k_doc32;
+  const float *k_rel;  // position minus the tile's smallest, for the distance bias
+  const TileStats *stats;
+  // paged prefix
+  const int *pages, *own_lens;
+  int block_size, num_blocks;
+  long long prefix_len;
+  DeviceStatus *status;
+};
+
+template <int D>
+struct TcSmem {
+  static constexpr int kTile = kTileN * D * 2;
+  static constexpr int kQ = 0;                       // two row tiles
+  static constexpr int kKV = 2 * kTile;              // kStages key tiles
+  static constexpr int kBars = kKV + kStages * kTile;
+  static constexpr int kBytes = kBars + 256 + 1024;  // + alignment to the swizzle's 1 KB
+};
+
+struct RowRef {
+  int token, head;
+  bool valid;
+};
+
+// (tokens * heads < 2^31, so a row index fits 32 bits)
+__device__ __forceinline__ RowRef row_ref(const TcArgs &a, int kv_head, unsigned rho) {
+  RowRef r;
+  const unsigned t = rho / static_cast<unsigned>(a.group);
+  r.valid = t < static_cast<unsigned>(a.tokens);
+  r.token = r.valid ? static_cast<int>(t) : 0;
+  r.head = kv_head * a.group + static_cast<int>(rho - t * a.group);
+  return r;
+}
+
+// What a dense row may see: key positions below `limit` in document `doc`.
+struct RowMask {
+  int limit, doc, pos;
+};
+
+__device__ __forceinline__ int clamp_pos(long long p) {
+  return static_cast<int>(min(max(p, -2147483646ll), 2147483645ll));
+}
+
+__device__ __forceinline__ RowMask row_mask(const PositionArgs &p, int token) {
+  RowMask m;
+  m.pos = clamp_pos(position_at(p.q_pos, p.long_q_pos, token));
+  m.limit = p.causal ? m.pos + 1 : 2147483647;
+  if (p.q_prefix) m.limit = max(m.limit, p.q_prefix[token]);
+  m.doc = p.q_doc ? p.q_doc[token] : 0;
+  if (m.doc < 0) m.limit = -2147483647 - 1;  // a padding row sees nothing
+  return m;
+}
+
+// A row whose tensor-core result holds an infinity or NaN is computed again by
+// the definition, by one warp: a masked key's weight is 0, and 0 times an
+// infinity in its value is not, so only keys that the row sees may take part.
+template <typename T, int D>
+__device__ __forceinline__ void strict_position_row(const PositionArgs &a, int token, int h) {
+  const RowMask m = row_mask(a, token);
+  const int kv = h / (a.heads / a.kv_heads);
+  WarpRow<T, D> row;
+  row.start(static_cast<const T *>(a.q) + token * a.q_token + h * a.q_head);
+  const float slope = a.slopes ? a.slopes[h] : 0.f;
+#pragma unroll 1
+  for (int j = 0; j < a.k_tokens; ++j) {
+    const int kp = a.k_pos ? clamp_pos(position_at(a.k_pos, a.long_k_pos, j)) : j;
+    if (kp >= m.limit || (a.k_doc && a.k_doc[j] != m.doc)) continue;
+    row.add(static_cast<const T *>(a.k) + j * a.k_token + kv * a.k_head,
+            static_cast<const T *>(a.v) + j * a.v_token + kv * a.v_head, a.scale, a.softcap,
+            slope * fabsf(static_cast<float>(static_cast<long long>(m.pos) - kp)));
+  }
+  const long long r = static_cast<long long>(token) * a.heads + h;
+  row.finish(static_cast<T *>(a.out) + r * D, a.lse ? a.lse + r : nullptr);
+}
+
+// The key tiles of a block, in order; every role walks them alike.
+template <bool kDense>
+struct TileScan {
+  const TcArgs &a;
+  int end, base;
+  uint32_t live, full;
+  int lim_min, lim_max, doc_min, doc_max;
+
+  __device__ TileScan(const TcArgs &args, int begin, int stop, const int *group)
+      : a(args), end(stop), base(begin - 32), live(0), full(0) {
+    if (kDense) lim_min = group[0], lim_max = group[1], doc_min = group[2], doc_max = group[3];
+    else base = begin - 1;
+  }
+
+  __device__ __forceinline__ bool next(int &tile, bool &whole) {
+    if (!kDense) {
+      tile = ++base;
+      whole = true;
+      return base < end;
+    }
+    while (live == 0) {
+      base += 32;
+      if (base >= end) return false;
+      const int t = base + (threadIdx.x & 31);
+      bool some = false, all = false;
+      if (t < end) {
+        const TileStats s = a.stats[t];
+        some = s.pos_min < lim_max && s.doc_min <= doc_max && s.doc_max >= doc_min;
+        all = s.pos_max < lim_min && s.doc_min == s.doc_max && doc_min == doc_max &&
+              s.doc_min == doc_min;
+      }
+      live = __ballot_sync(0xffffffffu, some);
+      full = __ballot_sync(0xffffffffu, some && all);
+    }
+    const int bit = __ffs(live) - 1;
+    live &= live - 1;
+    tile = base + bit;
+    whole = (full >> bit) & 1;
+    return true;
+  }
+};
+
+template <typename T, int D, bool kDense, bool kCap, bool kBias>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    tc_attention_kernel(const __grid_constant__ CUtensorMap k_map,
+                        const __grid_constant__ CUtensorMap v_map,
+                        const __grid_constant__ TcArgs a) {
+  using L = TcSmem<D>;
+  constexpr int kHalves = D / 64;            // 128-byte column blocks of a row
+  constexpr int kHalfBytes = kTileN * 128;   // of one tile
+  constexpr bool kBf16 = sizeof(T) == 2 && __is_same(T, __nv_bfloat16);
+  extern __shared__ uint8_t raw_smem[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>(
+      (reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBars);
+  uint64_t *kv_full = bars, *kv_empty = bars + kStages, *s_full = bars + 2 * kStages,
+           *p_full = s_full + 2, *o_done = p_full + 2, *q_full = o_done + 2, *drain = q_full + 1;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+  int *stopped = reinterpret_cast<int *>(tmem_slot + 1);
+  int *seen = stopped + 1;  // limits and documents of the block's rows
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int kv_heads = a.heads / a.group;
+  // the last rows see the most keys: they start first
+  const int per_row_group = kv_heads * max(1, a.slices);
+  const long long rows = static_cast<long long>(a.tokens) * a.group;
+  const int n_groups = static_cast<int>((rows + kBlockRows - 1) / kBlockRows);
+  const int row_group = n_groups - 1 - static_cast<int>(blockIdx.x / per_row_group);
+  const int rest = static_cast<int>(blockIdx.x % per_row_group);
+  const int kv_head = rest % kv_heads, slice = rest / kv_heads;
+  const unsigned rho0 = static_cast<unsigned>(row_group) * kBlockRows;
+  const int tiles = rho0 + kTileM < rows ? 2 : 1;
+  const int t_begin = slice * a.tiles_per_slice;
+  const int t_end = min(a.k_tiles, t_begin + a.tiles_per_slice);
+
+  if (warp == 8) tmem_alloc(tmem_slot, 512);
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(&kv_full[i], 1), mbar_init(&kv_empty[i], 1);
+    for (int i = 0; i < 2; ++i)
+      mbar_init(&s_full[i], 1), mbar_init(&p_full[i], kTileM), mbar_init(&o_done[i], 1);
+    mbar_init(q_full, kTileM * tiles);
+    mbar_init(drain, 1);
+    *stopped = 0;
+    seen[0] = 2147483647, seen[1] = -2147483647 - 1;
+    seen[2] = 2147483647, seen[3] = -2147483647 - 1;
+    fence_mbar_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // Rows: masks, and Q into shared memory (128-byte swizzled rows).
+  RowRef ref = {0, 0, false};
+  RowMask mask = {0, 0, 0};
+  const int x = warp >> 2;  // row tile of this thread (warps 0-7)
+  if (warp < 8 && x < tiles) {
+    ref = row_ref(a, kv_head, rho0 + x * kTileM + (tid & 127));
+    if (kDense) {
+      constexpr int kLow = -2147483647 - 1, kHigh = 2147483647;
+      mask.limit = kLow;
+      if (ref.valid) mask = row_mask(a.pos, ref.token);
+      const bool in_doc = ref.valid && mask.doc >= 0;
+      const int lo = __reduce_min_sync(0xffffffffu, ref.valid ? mask.limit : kHigh);
+      const int hi = __reduce_max_sync(0xffffffffu, in_doc ? mask.limit : kLow);
+      const int d_lo = __reduce_min_sync(0xffffffffu, in_doc ? mask.doc : kHigh);
+      const int d_hi = __reduce_max_sync(0xffffffffu, in_doc ? mask.doc : kLow);
+      if (lane == 0) {
+        atomicMin(&seen[0], lo), atomicMax(&seen[1], hi);
+        atomicMin(&seen[2], d_lo), atomicMax(&seen[3], d_hi);
+      }
+    }
+    constexpr int kVecs = D / 8;
+    uint8_t *dst = smem + L::kQ + x * L::kTile;
+#pragma unroll 4
+    for (int i = tid & 127; i < kTileM * kVecs; i += kTileM) {
+      const int r = i / kVecs, c = i % kVecs;
+      const RowRef o = row_ref(a, kv_head, rho0 + x * kTileM + r);
+      int4 v = make_int4(0, 0, 0, 0);
+      if (o.valid) {
+        const int b = o.token / a.q_len;
+        v = ld_nc_v4(static_cast<const T *>(a.q) + b * a.q_batch +
+                     (o.token - b * a.q_len) * a.q_token + o.head * a.q_head + c * 8);
+      }
+      *reinterpret_cast<int4 *>(dst + (c >> 3) * kHalfBytes + r * 128 +
+                                (((c & 7) ^ (r & 7)) << 4)) = v;
+    }
+    fence_proxy_async_smem();
+    mbar_arrive(q_full);
+  }
+  __syncthreads();  // `seen` is whole
+  TileScan<kDense> scan(a, t_begin, t_end, seen);
+
+  // (each role sets its registers in its own branch: the compiler then allots
+  // them per branch)
+  if (warp == 9) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    // ------------------------------------------------------------- loader
+    if (lane == 0) prefetch_map(&k_map), prefetch_map(&v_map);
+    int tile, it = 0;
+    bool whole, ok = true;
+    const int boxes = kDense ? 1 : max(1, kTileN / a.block_size);
+    while (ok && scan.next(tile, whole)) {
+#pragma unroll 1
+      for (int kv = 0; kv < 2; ++kv, ++it) {
+        const int st = it % kStages;
+        if (it >= kStages) ok = wait_or_stop(&kv_empty[st], (it / kStages - 1) & 1, stopped);
+        if (!ok) break;
+        uint8_t *dst = smem + L::kKV + st * L::kTile;
+        const CUtensorMap *map = kv ? &v_map : &k_map;
+        if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], L::kTile);
+        __syncwarp();
+        if (kDense) {
+          if (lane < kHalves)
+            tma_load_3d(dst + lane * kHalfBytes, map, lane * 64, kv_head, tile * kTileN,
+                        &kv_full[st]);
+        } else if (lane < boxes) {
+          // a page, or 128 slots of a larger one; an id outside the cache reads zeros
+          const int box_rows = min(kTileN, a.block_size);
+          const int j = tile * kTileN + lane * box_rows;
+          const int col = j / a.block_size;
+          int page = a.pages[col];
+          if (page < 0 || page >= a.num_blocks) page = a.num_blocks;
+#pragma unroll
+          for (int h = 0; h < kHalves; ++h)
+            tma_load_4d(dst + h * kHalfBytes + lane * box_rows * 128, map, h * 64, kv_head,
+                        j - col * a.block_size, page, &kv_full[st]);
+        }
+      }
+    }
+    // loads in flight land before the block's memory is given back
+    for (int i = max(0, it - kStages); i < it; ++i)
+      mbar_wait_bounded(&kv_full[i % kStages], (i / kStages) & 1, 2000000000ull);
+  } else if (warp == 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    // ------------------------------------------------------------- mma
+    constexpr uint32_t kQK = mma_desc(kBf16, false, kTileM, kTileN);
+    constexpr uint32_t kPV = mma_desc(kBf16, true, kTileM, D);
+    const uint32_t q_addr = smem_u32(smem + L::kQ), kv_addr = smem_u32(smem + L::kKV);
+    auto score = [&](int t, int st) {
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const uint32_t off = (k >> 2) * kHalfBytes + (k & 3) * 32;
+        mma_ss(tmem + t * kTileN, smem_desc(q_addr + t * L::kTile + off, 16, 1024),
+               smem_desc(kv_addr + st * L::kTile + off, 16, 1024), kQK, k > 0);
+      }
+      mma_commit(&s_full[t]);
+    };
+    auto weigh = [&](int t, int st, bool accumulate) {
+#pragma unroll
+      for (int k = 0; k < kTileN / 16; ++k)
+        mma_ts(tmem + 2 * kTileN + t * D, tmem + t * kTileN + k * 8,
+               smem_desc(kv_addr + st * L::kTile + k * 2048, kHalfBytes, 1024), kPV,
+               accumulate || k > 0);
+    };
+    int tile, it = 0;
+    bool whole;
+    bool ok = wait_or_stop(q_full, 0, stopped);
+    bool more = ok && scan.next(tile, whole);
+    if (more) {
+      ok = wait_or_stop(&kv_full[0], 0, stopped);
+      tc_fence_after();
+      if (ok && lane == 0) {
+        for (int t = 0; t < tiles; ++t) score(t, 0);
+        mma_commit(&kv_empty[0]);
+      }
+      it = 1;
+    }
+    for (int j = 0; ok && more; ++j) {
+      more = scan.next(tile, whole);
+      const int v_st = it % kStages, k_st = (it + 1) % kStages;
+      ok = wait_or_stop(&kv_full[v_st], (it / kStages) & 1, stopped);
+      if (ok && more)
+        ok = wait_or_stop(&kv_full[k_st], ((it + 1) / kStages) & 1, stopped);
+      for (int t = 0; ok && t < tiles; ++t) {
+        ok = wait_or_stop(&p_full[t], j & 1, stopped);
+        tc_fence_after();
+        if (ok && lane == 0) {
+          weigh(t, v_st, j > 0);
+          if (!more) mma_commit(&o_done[t]);
+          if (t == tiles - 1) mma_commit(&kv_empty[v_st]);
+          if (more) {
+            score(t, k_st);
+            if (t == tiles - 1) mma_commit(&kv_empty[k_st]);
+          }
+        }
+        __syncwarp();
+      }
+      it += 2;
+    }
+    if (!ok) {  // only after a wait that ran out: let the mma in flight end
+      if (lane == 0) mma_commit(drain);
+      mbar_wait_bounded(drain, 0, 2000000000ull);
+    }
+  } else if (warp > 9) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    if (x < tiles) {
+    // ------------------------------------------------------------- softmax
+    const uint32_t lane_base = static_cast<uint32_t>(warp & 3) << 21;
+    const uint32_t s_addr = tmem + lane_base + x * kTileN;
+    const uint32_t o_addr = tmem + lane_base + 2 * kTileN + x * D;
+    float m = -INFINITY, l = 0.f;
+    const float slope = kBias && ref.valid ? a.slopes[ref.head] * kLog2e : 0.f;
+    float q_at = 0.f;  // position in the prefix, for the distance bias
+    int own = 0;
+    if (!kDense && ref.valid) {
+      const int b = ref.token / a.q_len;
+      own = max(0, a.own_lens[b]) - a.q_len + (ref.token - b * a.q_len);
+      q_at = static_cast<float>(a.prefix_len + own);
+    }
+    int tile, j = 0;
+    bool whole, ok = true;
+    while (scan.next(tile, whole)) {
+      uint32_t bad = 0;  // pages of this tile that lie outside the cache
+      if (!kDense) {
+        const int boxes = max(1, kTileN / a.block_size);
+        bool out_of_cache = false;
+        if (lane < boxes) {
+          const int page =
+              a.pages[(tile * kTileN + lane * min(kTileN, a.block_size)) / a.block_size];
+          out_of_cache = page < 0 || page >= a.num_blocks;
+          if (out_of_cache) report_status(a.status, kStatusBadSlot, -1, tile, page);
+        }
+        bad = __ballot_sync(0xffffffffu, out_of_cache);
+      }
+      ok = wait_or_stop(&s_full[x], j & 1, stopped);
+      if (!ok) break;
+      tc_fence_after();
+      float s[kTileN];
+#pragma unroll
+      for (int c = 0; c < kTileN / 32; ++c)
+        tmem_ld32(s_addr + c * 32, reinterpret_cast<uint32_t(&)[32]>(s[c * 32]));
+      tmem_wait_ld();
+      // x = s c in log2 units, unless it is only scaled (then c goes into exp2)
+      if (kCap || kBias) {
+#pragma unroll
+        for (int i = 0; i < kTileN; ++i) {
+          if (kCap) {
+            // tanh(u) = 1 - 2 / (1 + e^2u): absolute error of a few 2^-22
+            const float e = ex2(s[i] * a.cap_in);
+            s[i] = fmaf(rcp(1.f + e), -2.f * a.cap_out, a.cap_out);
+          } else {
+            s[i] *= a.scale_log2;
+          }
+        }
+        if (kBias) {
+          if (kDense) {
+            const float at = static_cast<float>(static_cast<long long>(mask.pos) -
+                                                a.stats[tile].pos_min);
+            const float4 *rel = reinterpret_cast<const float4 *>(a.k_rel + tile * kTileN);
+#pragma unroll
+            for (int i = 0; i < kTileN / 4; ++i) {
+              const float4 p = rel[i];
+              s[4 * i] = fmaf(-slope, fabsf(at - p.x), s[4 * i]);
+              s[4 * i + 1] = fmaf(-slope, fabsf(at - p.y), s[4 * i + 1]);
+              s[4 * i + 2] = fmaf(-slope, fabsf(at - p.z), s[4 * i + 2]);
+              s[4 * i + 3] = fmaf(-slope, fabsf(at - p.w), s[4 * i + 3]);
+            }
+          } else {
+            const float at = q_at - static_cast<float>(tile * kTileN);
+#pragma unroll
+            for (int i = 0; i < kTileN; ++i)
+              s[i] = fmaf(-slope, fabsf(at - static_cast<float>(i)), s[i]);
+          }
+        }
+      }
+      if (kDense && !whole) {
+        const int4 *kp = reinterpret_cast<const int4 *>(a.k_pos32 + tile * kTileN);
+#pragma unroll
+        for (int i = 0; i < kTileN / 4; ++i) {
+          const int4 p = kp[i];
+          if (p.x >= mask.limit) s[4 * i] = -INFINITY;
+          if (p.y >= mask.limit) s[4 * i + 1] = -INFINITY;
+          if (p.z >= mask.limit) s[4 * i + 2] = -INFINITY;
+          if (p.w >= mask.limit) s[4 * i + 3] = -INFINITY;
+        }
+        if (a.k_doc32) {
+          const int4 *kd = reinterpret_cast<const int4 *>(a.k_doc32 + tile * kTileN);
+#pragma unroll
+          for (int i = 0; i < kTileN / 4; ++i) {
+            const int4 p = kd[i];
+            if (p.x != mask.doc) s[4 * i] = -INFINITY;
+            if (p.y != mask.doc) s[4 * i + 1] = -INFINITY;
+            if (p.z != mask.doc) s[4 * i + 2] = -INFINITY;
+            if (p.w != mask.doc) s[4 * i + 3] = -INFINITY;
+          }
+        }
+      }
+      if (!kDense && bad) {
+        const int rows_of = min(kTileN, a.block_size);
+#pragma unroll
+        for (int i = 0; i < kTileN; ++i)
+          if ((bad >> (i / rows_of)) & 1) s[i] = -INFINITY;
+      }
+      const float c = kCap || kBias ? 1.f : a.scale_log2;
+      float t0 = s[0], t1 = s[1], t2 = s[2], t3 = s[3];
+#pragma unroll
+      for (int i = 4; i < kTileN; i += 4) {
+        t0 = fmaxf(t0, s[i]), t1 = fmaxf(t1, s[i + 1]);
+        t2 = fmaxf(t2, s[i + 2]), t3 = fmaxf(t3, s[i + 3]);
+      }
+      const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * c;
+      const bool grow = top > m + kLazy;  // also the first finite score
+      if (__any_sync(0xffffffffu, grow)) {
+        const float to = grow ? top : m;
+        const float keep = grow ? ex2(m - to) : 1.f;
+        m = to;
+        l *= keep;
+        if (j > 0) {  // the score barrier also covers the last product into O
+#pragma unroll 1
+          for (int k = 0; k < D / 32; ++k) {
+            uint32_t o[32];
+            tmem_ld32(o_addr + k * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+            tmem_st32(o_addr + k * 32, o);
+          }
+        }
+      }
+      const float off = m == -INFINITY ? 0.f : m;
+      float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t p[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float u = ex2(fmaf(s[h * 64 + 2 * i], c, -off));
+          const float v = ex2(fmaf(s[h * 64 + 2 * i + 1], c, -off));
+          l0 += u, l1 += v;
+          p[i] = pair_from_float<T>(u, v);
+        }
+        tmem_st32(s_addr + h * 32, p);
+      }
+      l += l0 + l1;
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&p_full[x]);
+      ++j;
+    }
+    // ------------------------------------------------------------- result
+    if (ok && j > 0) ok = wait_or_stop(&o_done[x], 0, stopped);
+    tc_fence_after();
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : NAN);
+    const long long row = static_cast<long long>(ref.token) * a.heads + ref.head;
+    bool finite = true;
+#pragma unroll 1
+    for (int k = 0; k < D / 32; ++k) {
+      float o[32];
+      if (ok && j > 0) {
+        tmem_ld32(o_addr + k * 32, reinterpret_cast<uint32_t(&)[32]>(o));
+        tmem_wait_ld();
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        o[i] = ok ? (j > 0 ? o[i] * inv : 0.f) : NAN;
+        finite = finite && fabsf(o[i]) <= 3.4028235e38f;
+      }
+      if (!ref.valid) continue;
+      if (a.slices == 0) {
+        T *dst = static_cast<T *>(a.out) + row * D + k * 32;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          int4 w;
+          w.x = pair_from_float<T>(o[8 * i], o[8 * i + 1]);
+          w.y = pair_from_float<T>(o[8 * i + 2], o[8 * i + 3]);
+          w.z = pair_from_float<T>(o[8 * i + 4], o[8 * i + 5]);
+          w.w = pair_from_float<T>(o[8 * i + 6], o[8 * i + 7]);
+          st_v4(dst + 8 * i, w);
+        }
+      } else {
+        float *dst = a.part_o + (static_cast<long long>(slice) * a.tokens * a.heads + row) * D +
+                     k * 32;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          *reinterpret_cast<float4 *>(dst + 4 * i) =
+              make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+      }
+    }
+    if (ref.valid) {
+      if (a.slices == 0) {
+        if (a.lse) a.lse[row] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+      } else {
+        a.part_lse[static_cast<long long>(slice) * a.tokens * a.heads + row] =
+            l == 0.f ? -INFINITY : m + log2f(l);
+      }
+    }
+    if (kDense && a.slices == 0 && ok) {
+      __syncwarp();  // a row written above is written again below
+      uint32_t again = __ballot_sync(0xffffffffu, ref.valid && !finite);
+      while (again) {
+        const int src = __ffs(again) - 1;
+        again &= again - 1;
+        strict_position_row<T, D>(a.pos, __shfl_sync(0xffffffffu, ref.token, src),
+                                  __shfl_sync(0xffffffffu, ref.head, src));
+      }
+    }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 8) tmem_free(tmem, 512);
+}
+
+}  // namespace lmc
