@@ -1,0 +1,403 @@
+// Attention of few rows over paged keys, split over the keys.
+//
+// A block owns 16 rows of one KV head (a request's query tokens and heads; a
+// decode step's group of heads fits) and a slice of their keys.  Each of its
+// four warps streams 16 keys at a time through its own ring of cp.async stages
+// and keeps its own maximum, sum and output, so no barrier is met until the
+// warps' results are joined at the end.  Products are 16x8x16 tensor
+// instructions: the block reads every key and value once and multiplies it with
+// 16 rows, 16 flop a byte, so it is bound by the reads and the small
+// instruction loses nothing.  Any block size, page order and stride.
+#pragma once
+#include "attention_join.cuh"
+
+namespace lmc {
+
+constexpr int kSplitWarps = 4, kSplitKeys = 16, kSplitRows = 16, kSplitStages = 3;
+
+// Which keys and rows a pass covers: prefix keys [pre_begin, pre_end), then the
+// own keys of the unit's request when `own`; a unit is a request, or all of
+// them (own == false).
+struct SplitPass {
+  int pre_begin, pre_end;
+  bool own;
+  int unit_tokens, row_tiles, slices;
+  float *part_o, *part_lse;  // first slice of this pass
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(valid ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                          uint32_t b1) {
+  if constexpr (__is_same(T, __nv_bfloat16))
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <int D>
+struct SplitSmem {
+  static constexpr int kKeys = kSplitKeys * D * 2;        // 16 rows of K or V
+  static constexpr int kStage = 2 * kKeys;
+  static constexpr int kWarp = kSplitStages * kStage;
+  static constexpr int kBytes = kSplitWarps * kWarp;
+  // the join at the end: each warp's output and statistics
+  static_assert(kBytes >= kSplitWarps * kSplitRows * (D + 2) * 4, "join fits in the rings");
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kSplitWarps * 32, 2)
+    paged_split_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ SplitPass s) {
+  using L = SplitSmem<D>;
+  constexpr int kChunks = D / 8;  // 16-byte chunks of a row
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int group = a.heads / a.kv_heads;
+  const int slice = blockIdx.y;
+  int u = blockIdx.x;
+  const int kv = u % a.kv_heads;
+  u /= a.kv_heads;
+  const int row_tile = u % s.row_tiles, unit = u / s.row_tiles;
+  const int n = s.own ? max(0, a.own_lens[unit]) : 0;
+  const int pre = s.pre_end - s.pre_begin;
+  // keys: the pass's prefix part, then own keys within the request's table row
+  const long long room = static_cast<long long>(a.width) * a.block_size;
+  const int own_keys = static_cast<int>(min(static_cast<long long>(n), room));
+  if (n > room && slice == 0 && row_tile == 0 && threadIdx.x == 0)
+    report_status(a.status, kStatusBadIndex, unit, n, room);
+  const int total = pre + own_keys;
+  const int chunk = kSplitWarps * kSplitKeys;
+  const int per = ((total + s.slices - 1) / s.slices + chunk - 1) / chunk * chunk;
+  const int k0 = min(total, slice * per), k1 = min(total, k0 + per);
+  const long long all_rows = static_cast<long long>(a.batch) * a.q_len * a.heads;
+
+  // row r of this tile: token and head (rows past the unit's are not stored)
+  const int rows = s.unit_tokens * group - row_tile * kSplitRows;
+  auto token_of = [&](int r) { return unit * s.unit_tokens + (row_tile * kSplitRows + r) / group; };
+  auto head_of = [&](int r) { return kv * group + (row_tile * kSplitRows + r) % group; };
+  float *part_o = s.part_o + static_cast<long long>(slice) * all_rows * D;
+  float *part_lse = s.part_lse + static_cast<long long>(slice) * all_rows;
+  if (k0 >= k1) {  // no keys: an empty part
+    if (threadIdx.x < kSplitRows && static_cast<int>(threadIdx.x) < rows)
+      part_lse[static_cast<long long>(token_of(threadIdx.x)) * a.heads + head_of(threadIdx.x)] =
+          -INFINITY;
+    return;
+  }
+
+  uint8_t *ring = smem + warp * L::kWarp;
+  const uint32_t ring_addr = smem_u32(ring);
+  const int steps = (k1 - k0 + chunk - 1) / chunk;
+
+  // Pages of the 16 keys of step `it` of this warp: lane i (and i + 16) key i.
+  auto key_page = [&](int it, int &off, bool &bad) -> int {
+    const int j = k0 + it * chunk + warp * kSplitKeys + (lane & 15);
+    bad = false;
+    off = 0;
+    if (j >= k1) return -1;
+    const bool shared = j < pre;
+    const unsigned at = shared ? s.pre_begin + j : j - pre;
+    const unsigned col = at / static_cast<unsigned>(a.block_size);
+    off = static_cast<int>(at - col * a.block_size);
+    const int page = shared ? a.prefix_blocks[col] : a.tables[unit * a.table_stride + col];
+    if (page >= 0 && page < a.num_blocks) return page;
+    bad = true;
+    if (lane < 16) report_status(a.status, kStatusBadSlot, shared ? -1 : unit, col, page);
+    return -1;
+  };
+  auto load = [&](int it, int page, int off) {
+    const uint32_t dst = ring_addr + (it % kSplitStages) * L::kStage;
+    const int c = lane % kChunks;
+    constexpr int kRowsAtOnce = 32 / kChunks;
+#pragma unroll
+    for (int i = 0; i < kSplitKeys / kRowsAtOnce; ++i) {
+      const int r = i * kRowsAtOnce + lane / kChunks;
+      const int pg = __shfl_sync(0xffffffffu, page, r), of = __shfl_sync(0xffffffffu, off, r);
+      const bool valid = pg >= 0;  // else zeros: nothing of the page is read
+      const long long p = valid ? pg : 0;
+      const uint32_t at = r * (D * 2) + ((c & ~7) << 4) + (((c & 7) ^ (r & 7)) << 4);
+      cp_async16(dst + at, static_cast<const T *>(a.k) + p * a.k_block + of * a.k_slot +
+                               kv * a.k_head + c * 8, valid);
+      cp_async16(dst + L::kKeys + at, static_cast<const T *>(a.v) + p * a.v_block +
+                                          of * a.v_slot + kv * a.v_head + c * 8, valid);
+    }
+  };
+
+  // keys of each stage in flight that lie outside the cache
+  uint32_t bad_ring[kSplitStages];
+#pragma unroll
+  for (int i = 0; i < kSplitStages; ++i) bad_ring[i] = 0;
+  int page, off;
+  bool bad;
+#pragma unroll
+  for (int i = 0; i < kSplitStages - 1; ++i) {
+    if (i < steps) {
+      page = key_page(i, off, bad);
+      bad_ring[i] = __ballot_sync(0xffffffffu, bad) & 0xffff;
+      load(i, page, off);
+    }
+    cp_async_commit();
+  }
+  page = -1;
+  bad = false;
+  if (kSplitStages - 1 < steps) page = key_page(kSplitStages - 1, off, bad);
+
+  // Q as the A operand: row lane/4 (and + 8), columns 2 (lane % 4) of each 8.
+  const int r0 = lane >> 2, r1 = r0 + 8, c0 = (lane & 3) * 2;
+  uint32_t q[D / 16][4];
+  auto q_row = [&](int r) -> const T * {
+    const int t = token_of(r), b = t / a.q_len;
+    return static_cast<const T *>(a.q) + b * a.q_batch + (t - b * a.q_len) * a.q_token +
+           head_of(r) * a.q_head;
+  };
+  {
+    const T *p0 = r0 < rows ? q_row(r0) : nullptr, *p1 = r1 < rows ? q_row(r1) : nullptr;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      const int c = k * 16 + c0;
+      q[k][0] = p0 ? *reinterpret_cast<const uint32_t *>(p0 + c) : 0;
+      q[k][1] = p1 ? *reinterpret_cast<const uint32_t *>(p1 + c) : 0;
+      q[k][2] = p0 ? *reinterpret_cast<const uint32_t *>(p0 + c + 8) : 0;
+      q[k][3] = p1 ? *reinterpret_cast<const uint32_t *>(p1 + c + 8) : 0;
+    }
+  }
+  // Row i of a request sees its own keys up to n - q_len + i: as an index into
+  // this pass's keys, j < last.
+  auto last_of = [&](int r) {
+    if (!s.own) return total;
+    const int i = r < rows ? token_of(r) - unit * a.q_len : 0;
+    return pre + max(0, min(own_keys, n - a.q_len + i + 1));
+  };
+  const int last0 = last_of(r0), last1 = last_of(r1);
+  float slope0 = 0.f, slope1 = 0.f, at0 = 0.f, at1 = 0.f;
+  if (a.slopes) {
+    auto place = [&](int r, float &slope, float &at) {
+      if (r >= rows) return;
+      const int t = token_of(r), b = t / a.q_len;
+      slope = a.slopes[head_of(r)] * kLog2e;
+      at = static_cast<float>(a.prefix_len + max(0, a.own_lens[b]) - a.q_len + (t - b * a.q_len));
+    };
+    place(r0, slope0, at0);
+    place(r1, slope1, at1);
+  }
+  // position of pass key j: in the prefix, or behind it
+  auto place_of = [&](int j) {
+    return static_cast<float>(j < pre ? s.pre_begin + j : a.prefix_len + (j - pre));
+  };
+  const float scale = a.scale * kLog2e;
+  const float cap_in = a.softcap > 0.f ? 2.f * kLog2e * a.scale / a.softcap : 0.f;
+  const float cap_out = a.softcap * kLog2e;
+
+  float o[D / 8][4];
+#pragma unroll
+  for (int d = 0; d < D / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+
+  for (int it = 0; it < steps; ++it) {
+    // one more step's loads, and the pages of the step after it
+    {
+      const int nx = it + kSplitStages - 1;
+      __syncwarp();  // every lane is done with the stage that is filled next
+      if (nx < steps) {
+        const uint32_t b = __ballot_sync(0xffffffffu, bad) & 0xffff;
+#pragma unroll
+        for (int i = 0; i < kSplitStages; ++i)
+          if (nx % kSplitStages == i) bad_ring[i] = b;
+        load(nx, page, off);
+      }
+      cp_async_commit();
+      if (nx + 1 < steps) page = key_page(nx + 1, off, bad);
+    }
+    cp_async_wait<kSplitStages - 1>();
+    __syncwarp();
+    const uint32_t kb = ring_addr + (it % kSplitStages) * L::kStage, vb = kb + L::kKeys;
+    float sc[2][4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      const int r = (lane & 7) + ((lane >> 4) << 3), c = k * 2 + ((lane >> 3) & 1);
+      uint32_t b[4];
+      ldmatrix4(b, kb + r * (D * 2) + ((c & ~7) << 4) + (((c & 7) ^ (r & 7)) << 4));
+      mma_16816<T>(sc[0], q[k], b[0], b[1]);
+      mma_16816<T>(sc[1], q[k], b[2], b[3]);
+    }
+    const int j0 = k0 + it * chunk + warp * kSplitKeys;
+    uint32_t bad_keys = 0;
+#pragma unroll
+    for (int i = 0; i < kSplitStages; ++i)
+      if (it % kSplitStages == i) bad_keys = bad_ring[i];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int col = t * 8 + c0 + (e & 1), j = j0 + col;
+        float x = sc[t][e];
+        if (cap_out > 0.f)
+          x = fmaf(rcp(1.f + ex2(x * cap_in)), -2.f * cap_out, cap_out);
+        else
+          x *= scale;
+        if (a.slopes)
+          x = fmaf(-(e < 2 ? slope0 : slope1), fabsf((e < 2 ? at0 : at1) - place_of(j)), x);
+        if (j >= (e < 2 ? last0 : last1) || j >= k1 || ((bad_keys >> col) & 1)) x = -INFINITY;
+        sc[t][e] = x;
+      }
+    }
+    float top0 = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1]));
+    float top1 = fmaxf(fmaxf(sc[0][2], sc[0][3]), fmaxf(sc[1][2], sc[1][3]));
+#pragma unroll
+    for (int x = 1; x < 4; x <<= 1) {
+      top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, x));
+      top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, x));
+    }
+    const bool grow0 = top0 > m0 + kLazy, grow1 = top1 > m1 + kLazy;
+    if (__any_sync(0xffffffffu, grow0 || grow1)) {
+      const float to0 = grow0 ? top0 : m0, to1 = grow1 ? top1 : m1;
+      const float f0 = grow0 ? ex2(m0 - to0) : 1.f, f1 = grow1 ? ex2(m1 - to1) : 1.f;
+      m0 = to0, m1 = to1;
+      l0 *= f0, l1 *= f1;
+#pragma unroll
+      for (int d = 0; d < D / 8; ++d) o[d][0] *= f0, o[d][1] *= f0, o[d][2] *= f1, o[d][3] *= f1;
+    }
+    const float off0 = m0 == -INFINITY ? 0.f : m0, off1 = m1 == -INFINITY ? 0.f : m1;
+    uint32_t p[4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const float w0 = ex2(sc[t][0] - off0), w1 = ex2(sc[t][1] - off0);
+      const float w2 = ex2(sc[t][2] - off1), w3 = ex2(sc[t][3] - off1);
+      l0 += w0 + w1, l1 += w2 + w3;
+      p[2 * t] = pair_from_float<T>(w0, w1);
+      p[2 * t + 1] = pair_from_float<T>(w2, w3);
+    }
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) {
+      const int r = (lane & 7) + (((lane >> 3) & 1) << 3), c = d * 2 + (lane >> 4);
+      uint32_t b[4];
+      ldmatrix4_trans(b, vb + r * (D * 2) + ((c & ~7) << 4) + (((c & 7) ^ (r & 7)) << 4));
+      mma_16816<T>(o[2 * d], p, b[0], b[1]);
+      mma_16816<T>(o[2 * d + 1], p, b[2], b[3]);
+    }
+  }
+  // --- the four warps' results in one
+#pragma unroll
+  for (int x = 1; x < 4; x <<= 1) {
+    l0 += __shfl_xor_sync(0xffffffffu, l0, x);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, x);
+  }
+  cp_async_wait<0>();
+  __syncthreads();
+  float *wo = reinterpret_cast<float *>(smem);                 // [warp][16][D]
+  float *wm = wo + kSplitWarps * kSplitRows * D;               // [warp][16]
+  float *wl = wm + kSplitWarps * kSplitRows;
+  if ((lane & 3) == 0) {
+    wm[warp * kSplitRows + r0] = m0, wm[warp * kSplitRows + r1] = m1;
+    wl[warp * kSplitRows + r0] = l0, wl[warp * kSplitRows + r1] = l1;
+  }
+#pragma unroll
+  for (int d = 0; d < D / 8; ++d) {
+    float *w0 = wo + (warp * kSplitRows + r0) * D + d * 8 + c0;
+    *reinterpret_cast<float2 *>(w0) = make_float2(o[d][0], o[d][1]);
+    *reinterpret_cast<float2 *>(w0 + 8 * D) = make_float2(o[d][2], o[d][3]);
+  }
+  __syncthreads();
+  for (int r = warp; r < min(rows, kSplitRows); r += kSplitWarps) {
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kSplitWarps; ++w) m = fmaxf(m, wm[w * kSplitRows + r]);
+    const float base = m == -INFINITY ? 0.f : m;
+    float f[kSplitWarps];
+#pragma unroll
+    for (int w = 0; w < kSplitWarps; ++w) {
+      f[w] = ex2(wm[w * kSplitRows + r] - base);
+      l = fmaf(f[w], wl[w * kSplitRows + r], l);
+    }
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : NAN);
+    const long long row = static_cast<long long>(token_of(r)) * a.heads + head_of(r);
+    for (int d = lane * 4; d < D; d += 128) {
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kSplitWarps; ++w) {
+        const float4 v = *reinterpret_cast<const float4 *>(wo + (w * kSplitRows + r) * D + d);
+        acc.x = fmaf(f[w], v.x, acc.x), acc.y = fmaf(f[w], v.y, acc.y);
+        acc.z = fmaf(f[w], v.z, acc.z), acc.w = fmaf(f[w], v.w, acc.w);
+      }
+      *reinterpret_cast<float4 *>(part_o + row * D + d) =
+          make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    }
+    if (lane == 0) part_lse[row] = l == 0.f ? -INFINITY : m + log2f(l);
+  }
+}
+
+// A row of the batch by the definition, on one warp: when a joined result holds
+// an infinity or NaN (a draft token's value that earlier rows must not see).
+template <typename T, int D>
+__device__ __noinline__ void strict_paged_row(const PagedArgs &a, long long r) {
+  const int h = static_cast<int>(r % a.heads), kv = h / (a.heads / a.kv_heads);
+  const int t = static_cast<int>(r / a.heads), b = t / a.q_len, i = t - b * a.q_len;
+  const int n = max(0, a.own_lens[b]);
+  const long long pos = a.prefix_len + n - a.q_len + i;
+  const long long room = static_cast<long long>(a.width) * a.block_size;
+  const long long own = min(room, max(0ll, static_cast<long long>(n) - a.q_len + i + 1));
+  const float slope = a.slopes ? a.slopes[h] : 0.f;
+  WarpRow<T, D> row;
+  row.start(static_cast<const T *>(a.q) + b * a.q_batch + i * a.q_token + h * a.q_head);
+  for (long long j = 0; j < a.prefix_len + own; ++j) {
+    const bool shared = j < a.prefix_len;
+    const unsigned at = static_cast<unsigned>(shared ? j : j - a.prefix_len);
+    const unsigned col = at / static_cast<unsigned>(a.block_size);
+    const int off = static_cast<int>(at - col * a.block_size);
+    const int page = shared ? a.prefix_blocks[col] : a.tables[b * a.table_stride + col];
+    if (page < 0 || page >= a.num_blocks) continue;
+    row.add(static_cast<const T *>(a.k) + page * a.k_block + off * a.k_slot + kv * a.k_head,
+            static_cast<const T *>(a.v) + page * a.v_block + off * a.v_slot + kv * a.v_head,
+            a.scale, a.softcap, slope * fabsf(static_cast<float>(pos - j)));
+  }
+  row.finish(static_cast<T *>(a.out) + r * D, a.lse ? a.lse + r : nullptr);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(128)
+    join_paged_kernel(const __grid_constant__ PagedArgs a, const float *part_o,
+                      const float *part_lse, int slices) {
+  const long long rows = static_cast<long long>(a.batch) * a.q_len * a.heads;
+  const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  JoinedRow<T, D> r;
+  r.join(part_o, part_lse, slices, rows, row);
+  if (r.finite())
+    r.store(static_cast<T *>(a.out), a.lse, row);
+  else
+    strict_paged_row<T, D>(a, row);
+}
+
+}  // namespace lmc

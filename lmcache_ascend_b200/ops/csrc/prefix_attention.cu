@@ -1,0 +1,133 @@
+// Attention of a batch over a prefix that its requests share: the prefix in
+// whole 128-key tiles once for all rows on the tensor cores, the rest of the
+// prefix and each request's own keys in a pass that is split over the keys, and
+// a join of the parts.
+#include <algorithm>
+
+#include "paged_split.cuh"
+#include "tensor_maps.h"
+
+namespace lmc {
+namespace {
+
+struct PrefixPlan {
+  int tiles, per_slice, tc_slices, groups;  // tensor-core pass over tiles * 128 keys
+  int pre_slices, pre_tiles;                // split pass of all rows over the prefix
+  int own_begin, own_slices, own_tiles;     // split pass per request, from this prefix key on
+};
+
+int split_slices(long long blocks, long long keys) {
+  // towards four blocks per SM (two are resident), with 256 keys or more each
+  const long long want = std::min(148 * 4 / std::max(1ll, blocks), (keys + 255) / 256);
+  return static_cast<int>(std::max(1ll, std::min(want, 64ll)));
+}
+
+PrefixPlan plan_of(const PagedArgs &a) {
+  PrefixPlan p = {};
+  const int group = a.heads / a.kv_heads, bs = a.block_size;
+  const long long tokens = static_cast<long long>(a.batch) * a.q_len;
+  const int prefix = static_cast<int>(a.prefix_len);
+  // whole pages or whole 128-slot parts of them must make up a tile, in 8-row
+  // groups of the swizzle
+  const bool boxes = bs % 8 == 0 && (kTileN % bs == 0 || bs % kTileN == 0);
+  if (boxes && prefix >= kTileN) {
+    p.tiles = prefix / kTileN;
+    p.groups = static_cast<int>((tokens * group + kBlockRows - 1) / kBlockRows);
+    const long long blocks = static_cast<long long>(p.groups) * a.kv_heads;
+    const long long want =
+        std::max(1ll, std::min({148 / blocks, p.tiles / 2ll, 64ll}));
+    p.per_slice = static_cast<int>((p.tiles + want - 1) / want);
+    p.tc_slices = (p.tiles + p.per_slice - 1) / p.per_slice;
+    p.own_begin = p.tiles * kTileN;
+  } else if (a.batch > 1 && prefix >= kTileN) {
+    p.pre_tiles = static_cast<int>((tokens * group + kSplitRows - 1) / kSplitRows);
+    p.pre_slices = split_slices(static_cast<long long>(p.pre_tiles) * a.kv_heads, prefix);
+    p.own_begin = prefix;
+  }
+  p.own_tiles = (a.q_len * group + kSplitRows - 1) / kSplitRows;
+  p.own_slices =
+      split_slices(static_cast<long long>(a.batch) * p.own_tiles * a.kv_heads,
+                   prefix - p.own_begin + static_cast<long long>(a.width) * a.block_size);
+  return p;
+}
+
+template <typename T, int D>
+cudaError_t split_pass(const PagedArgs &a, const SplitPass &s, long long units,
+                       cudaStream_t stream) {
+  constexpr int kBytes = SplitSmem<D>::kBytes;
+  cudaError_t e = cudaFuncSetAttribute(paged_split_kernel<T, D>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+  if (e != cudaSuccess) return e;
+  const dim3 grid(static_cast<unsigned>(units * s.row_tiles * a.kv_heads), s.slices);
+  paged_split_kernel<T, D><<<grid, kSplitWarps * 32, kBytes, stream>>>(a, s);
+  return cudaGetLastError();
+}
+
+template <typename T, int D>
+cudaError_t launch(const PagedArgs &a, void *workspace, cudaStream_t stream) {
+  const PrefixPlan p = plan_of(a);
+  const long long rows = static_cast<long long>(a.batch) * a.q_len * a.heads;
+  const int slices = p.tc_slices + p.pre_slices + p.own_slices;
+  float *part_o = static_cast<float *>(workspace);
+  float *part_lse = part_o + slices * rows * D;
+  cudaError_t e = cudaSuccess;
+  if (p.tc_slices) {
+    TcArgs t = {};
+    t.q = a.q, t.slopes = a.slopes;
+    t.q_batch = a.q_batch, t.q_token = a.q_token, t.q_head = a.q_head;
+    t.tokens = a.batch * a.q_len, t.q_len = a.q_len;
+    t.heads = a.heads, t.group = a.heads / a.kv_heads;
+    t.k_tiles = p.tiles, t.tiles_per_slice = p.per_slice, t.slices = p.tc_slices;
+    t.part_o = part_o, t.part_lse = part_lse;
+    set_scores(t, a.scale, a.softcap);
+    t.pages = a.prefix_blocks, t.own_lens = a.own_lens;
+    t.block_size = a.block_size, t.num_blocks = a.num_blocks, t.prefix_len = a.prefix_len;
+    t.status = a.status;
+    CUtensorMap k_map, v_map;
+    const long long dims[4] = {D, a.kv_heads, a.block_size, a.num_blocks};
+    const long long ks[3] = {a.k_head, a.k_slot, a.k_block};
+    const long long vs[3] = {a.v_head, a.v_slot, a.v_block};
+    const int box[4] = {64, 1, std::min(kTileN, a.block_size), 1};
+    constexpr bool kBf16 = __is_same(T, __nv_bfloat16);
+    if (!encode_rows(&k_map, kBf16, a.k, 4, dims, ks, box) ||
+        !encode_rows(&v_map, kBf16, a.v, 4, dims, vs, box))
+      return cudaErrorInvalidValue;
+    const unsigned grid = static_cast<unsigned>(p.groups) * a.kv_heads * p.tc_slices;
+    e = launch_tc<T, D, false>(k_map, v_map, t, grid, stream);
+    if (e != cudaSuccess) return e;
+  }
+  int first = p.tc_slices;
+  if (p.pre_slices) {
+    const SplitPass s = {0, static_cast<int>(a.prefix_len), false, a.batch * a.q_len, p.pre_tiles,
+                         p.pre_slices, part_o + first * rows * D, part_lse + first * rows};
+    e = split_pass<T, D>(a, s, 1, stream);
+    if (e != cudaSuccess) return e;
+    first += p.pre_slices;
+  }
+  const SplitPass s = {p.own_begin, static_cast<int>(a.prefix_len), true, a.q_len, p.own_tiles,
+                       p.own_slices, part_o + first * rows * D, part_lse + first * rows};
+  e = split_pass<T, D>(a, s, a.batch, stream);
+  if (e != cudaSuccess) return e;
+  join_paged_kernel<T, D><<<static_cast<unsigned>((rows + 3) / 4), 128, 0, stream>>>(
+      a, part_o, part_lse, slices);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+long long shared_prefix_attention_workspace(const PagedArgs &a, int dim) {
+  const PrefixPlan p = plan_of(a);
+  return static_cast<long long>(p.tc_slices + p.pre_slices + p.own_slices) * a.batch * a.q_len *
+         a.heads * (dim + 1) * 4;
+}
+
+cudaError_t launch_shared_prefix_attention(const PagedArgs &a, RowType type, int dim,
+                                           void *workspace, cudaStream_t stream) {
+  if (type == RowType::kBFloat16)
+    return dim == 64 ? launch<__nv_bfloat16, 64>(a, workspace, stream)
+                     : launch<__nv_bfloat16, 128>(a, workspace, stream);
+  return dim == 64 ? launch<__half, 64>(a, workspace, stream)
+                   : launch<__half, 128>(a, workspace, stream);
+}
+
+}  // namespace lmc

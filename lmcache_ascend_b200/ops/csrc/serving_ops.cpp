@@ -306,7 +306,8 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> shared_prefix_attention(
   TORCH_CHECK(vector_rows(key_cache) && vector_rows(value_cache), op,
               ": cache rows must be contiguous and 16-byte aligned");
   TORCH_CHECK(Tq >= 1 && Tq <= 1024, op, ": q_len must be 1 to 1024, got ", Tq);
-  TORCH_CHECK(BS >= 1 && BS <= (1 << 20) && NB <= 0x7fffffff, op, ": bad cache size");
+  TORCH_CHECK(BS >= 1 && BS <= (1 << 20) && NB >= 1 && NB < 0x7fffffff, op,
+              ": bad cache size");
   check_dense(prefix_blocks, op, "prefix_blocks", dev, at::kInt);
   check_dense(own_lens, op, "seq_lens", dev, at::kInt);
   TORCH_CHECK(block_tables.device() == dev && block_tables.scalar_type() == at::kInt &&
@@ -314,11 +315,11 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> shared_prefix_attention(
                   (block_tables.size(1) <= 1 || block_tables.stride(1) == 1),
               op, ": block_tables must be int32 [>= batch, width] with contiguous rows");
   TORCH_CHECK(own_lens.dim() == 1 && own_lens.numel() == B, op, ": seq_lens must be [batch]");
-  TORCH_CHECK(prefix_len >= 0 && prefix_len <= (1ll << 30) &&
+  TORCH_CHECK(prefix_len >= 0 && prefix_len <= (1ll << 29) &&
                   prefix_blocks.numel() * BS >= prefix_len,
               op, ": prefix of ", prefix_len, " tokens needs more than ", prefix_blocks.numel(),
               " blocks of ", BS);
-  TORCH_CHECK(block_tables.size(1) * BS <= (1ll << 30), op, ": block_tables too wide");
+  TORCH_CHECK(block_tables.size(1) <= (1ll << 29) / BS, op, ": block_tables too wide");
   TORCH_CHECK(B * Tq * H <= 0x7fffffff, op, ": too many rows");
   const c10::cuda::CUDAGuard guard(dev);
   const at::Tensor q = with_vector_rows(q4);
@@ -347,7 +348,10 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> shared_prefix_attention(
   a.width = static_cast<int>(block_tables.size(1));
   a.scale = static_cast<float>(scale), a.softcap = static_cast<float>(softcap);
   a.status = checked_status(status, op, dev);
+  const auto workspace = at::empty({shared_prefix_attention_workspace(a, static_cast<int>(D))},
+                                   query.options().dtype(at::kByte));
   C10_CUDA_CHECK(launch_shared_prefix_attention(a, row_type(dt), static_cast<int>(D),
+                                                workspace.data_ptr(),
                                                 at::cuda::getCurrentCUDAStream().stream()));
   return {out, lse};
 }

@@ -80,9 +80,10 @@ cudaError_t launch_slot_mapping(const SlotArgs &a, bool long_lens, bool long_slo
                                 cudaStream_t stream);
 cudaError_t launch_rope_cache(const RopeArgs &a, RowType rows, RowType table, bool vec,
                               cudaStream_t stream);
+// Bytes of device workspace (16-byte aligned) that a launch takes.
+long long shared_prefix_attention_workspace(const PagedArgs &a, int dim);
 cudaError_t launch_shared_prefix_attention(const PagedArgs &a, RowType type, int dim,
-                                           cudaStream_t stream);
-// Bytes of device workspace (16-byte aligned) that the launch takes.
+                                           void *workspace, cudaStream_t stream);
 long long position_attention_workspace(const PositionArgs &a, int dim);
 cudaError_t launch_position_attention(const PositionArgs &a, RowType type, int dim,
                                       void *workspace, cudaStream_t stream);

@@ -137,11 +137,16 @@ struct TileScan {
   }
 
   __device__ __forceinline__ bool next(int &tile, bool &whole) {
-    if (!kDense) {
+    if constexpr (!kDense) {
       tile = ++base;
       whole = true;
       return base < end;
+    } else {
+      return next_dense(tile, whole);
     }
+  }
+
+  __device__ __forceinline__ bool next_dense(int &tile, bool &whole) {
     while (live == 0) {
       base += 32;
       if (base >= end) return false;
