@@ -76,7 +76,8 @@ __global__ void __launch_bounds__(128)
 inline void set_scores(TcArgs &t, float scale, float softcap) {
   t.scale_log2 = scale * kLog2e;
   t.cap_out = softcap * kLog2e;
-  t.cap_in = softcap > 0.f ? 2.f * kLog2e * scale / softcap : 0.f;
+  t.cap_u = softcap > 0.f ? scale / softcap : 0.f;
+  t.cap_in = 2.f * kLog2e * t.cap_u;
 }
 
 template <typename T, int D, bool kDense>

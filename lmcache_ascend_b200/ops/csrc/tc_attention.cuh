@@ -5,18 +5,21 @@
 // their loads whatever the group's size.  Keys come in tiles of 128.  Per key
 // tile and row tile
 //   S = Q K^T            tcgen05, both operands in shared memory, S in TMEM
-//   P = exp2(S c - m)    a thread per row: S from TMEM to registers, its running
-//                        maximum m and sum l, P as 16-bit back over S in TMEM
+//   P = exp2(S c - m)    two threads per row, 64 keys each: S from TMEM to
+//                        registers, running maximum m (common) and sum l (of
+//                        each), P as 16-bit back over S in TMEM
 //   O = O + P V          tcgen05, P from TMEM, V as it lies (MN-major)
 // While one tile's scores are in the registers the tensor cores work on the
 // other's.  m only moves when the maximum grows by more than 2^8, so O in TMEM
 // is seldom rescaled (by the thread that owns the row; P stays below 2^8 and
 // sums are fp32, so nothing is lost).
 //
-// Roles: warps 0-3 and 4-7 one row tile each, warp 8 issues the mma, warp 9 the
-// TMA loads through a ring of four 128-key stages (K and V alternate); they give
-// registers to the row tiles, whose threads hold a row of 128 scores each
-// (384 threads x 168 at launch = 256 x 216 + 128 x 72).
+// Roles: warps 0-7 and 8-15 one row tile each, warp 16 issues the mma, warp 17
+// the TMA loads through a ring of four 128-key stages (K and V alternate); they
+// give registers to the others (640 threads x 96 at launch = 512 x 112 + 128 x
+// 32).  Eight warps a tile, because a tile's chain (scores, weights, product,
+// next scores) is bound by the latency of the weights: with a thread per row
+// (four warps) the tensor cores idled half the time.
 // 256 rows a block because a K/V tile then feeds 256 flop a byte from L2.
 #pragma once
 #include "attention.cuh"
@@ -26,7 +29,10 @@ namespace lmc {
 
 constexpr int kTileM = 128, kTileN = 128, kBlockRows = 256;
 constexpr int kStages = 4;
-constexpr int kTcThreads = 384;
+constexpr int kTcThreads = 640, kMmaWarp = 16, kLoadWarp = 17;
+constexpr int kTileThreads = 256;  // of one row tile: two per row
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
 constexpr float kLazy = 8.f;  // log2 of how far P may pass 1 before O is rescaled
 
 // Dense keys: positions and documents of a key tile.
@@ -44,7 +50,8 @@ struct TcArgs {
   long long q_batch, q_token, q_head;
   int tokens, q_len, heads, group;
   int k_tiles, tiles_per_slice, slices;
-  float scale_log2, cap_in, cap_out;  // x = s scale_log2, or cap_out tanh(s cap_in)
+  // x = s scale_log2, or cap_out tanh(s cap_u) with cap_in = 2 cap_u log2 e
+  float scale_log2, cap_u, cap_in, cap_out;
   // dense keys (prepared arrays, padded to whole tiles)
   PositionArgs pos;
   const int *k_pos32, *k_doc32;
@@ -63,8 +70,21 @@ struct TcSmem {
   static constexpr int kQ = 0;                       // two row tiles
   static constexpr int kKV = 2 * kTile;              // kStages key tiles
   static constexpr int kBars = kKV + kStages * kTile;
-  static constexpr int kBytes = kBars + 256 + 1024;  // + alignment to the swizzle's 1 KB
+  static constexpr int kXch = kBars + 256;           // two floats per row
+  static constexpr int kBytes = kXch + 2048 + 1024;  // + alignment to the swizzle's 1 KB
 };
+
+// True in all threads of a row tile if it is in any of them.
+__device__ __forceinline__ bool tile_any(int tile, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\n"
+      "barrier.cta.red.or.pred q, %2, %3, p;\nselp.u32 %0, 1, 0, q;\n}"
+      : "=r"(r)
+      : "r"(v ? 1u : 0u), "r"(1 + tile), "n"(kTileThreads)
+      : "memory");
+  return r != 0;
+}
 
 struct RowRef {
   int token, head;
@@ -136,6 +156,18 @@ struct TileScan {
     else base = begin - 1;
   }
 
+  // How many tiles there are; the scan is used up.
+  __device__ __forceinline__ int count() {
+    if constexpr (!kDense) return max(0, end - base - 1);
+    int n = 0, tile;
+    bool whole;
+    while (next(tile, whole)) {
+      n += 1 + __popc(live);
+      live = 0;
+    }
+    return n;
+  }
+
   __device__ __forceinline__ bool next(int &tile, bool &whole) {
     if constexpr (!kDense) {
       tile = ++base;
@@ -177,7 +209,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   using L = TcSmem<D>;
   constexpr int kHalves = D / 64;            // 128-byte column blocks of a row
   constexpr int kHalfBytes = kTileN * 128;   // of one tile
-  constexpr bool kBf16 = sizeof(T) == 2 && __is_same(T, __nv_bfloat16);
+  constexpr bool kBf16 = __is_same(T, __nv_bfloat16);
+  // of 8 pairs of weights, how many the FMA pipe computes: ex2 and the mma are
+  // equally long at D = 128, ex2 is the longer at D = 64
+  constexpr int kFmaOf8 = D == 128 ? 2 : 3;
   extern __shared__ uint8_t raw_smem[];
   uint8_t *smem = reinterpret_cast<uint8_t *>(
       (reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -188,7 +223,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   int *stopped = reinterpret_cast<int *>(tmem_slot + 1);
   int *seen = stopped + 1;  // limits and documents of the block's rows
 
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform, for the compiler too
   const int kv_heads = a.heads / a.group;
   // the last rows see the most keys: they start first
   const int per_row_group = kv_heads * max(1, a.slices);
@@ -202,12 +238,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int t_begin = slice * a.tiles_per_slice;
   const int t_end = min(a.k_tiles, t_begin + a.tiles_per_slice);
 
-  if (warp == 8) tmem_alloc(tmem_slot, 512);
+  if (warp == kMmaWarp) tmem_alloc(tmem_slot, 512);
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) mbar_init(&kv_full[i], 1), mbar_init(&kv_empty[i], 1);
     for (int i = 0; i < 2; ++i)
-      mbar_init(&s_full[i], 1), mbar_init(&p_full[i], kTileM), mbar_init(&o_done[i], 1);
-    mbar_init(q_full, kTileM * tiles);
+      mbar_init(&s_full[i], 1), mbar_init(&p_full[i], kTileThreads), mbar_init(&o_done[i], 1);
+    mbar_init(q_full, kTileThreads * tiles);
     mbar_init(drain, 1);
     *stopped = 0;
     seen[0] = 2147483647, seen[1] = -2147483647 - 1;
@@ -217,14 +253,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  // the whole of tensor memory starts at column 0: a constant address
+  constexpr uint32_t tmem = 0;
 
   // Rows: masks, and Q into shared memory (128-byte swizzled rows).
   RowRef ref = {0, 0, false};
   RowMask mask = {0, 0, 0};
-  const int x = warp >> 2;  // row tile of this thread (warps 0-7)
-  if (warp < 8 && x < tiles) {
-    ref = row_ref(a, kv_head, rho0 + x * kTileM + (tid & 127));
+  const int x = warp >> 3, half = (warp >> 2) & 1;  // row tile, and which 64 keys
+  const int row_in_tile = tid & 127;
+  if (warp < kMmaWarp && x < tiles) {
+    ref = row_ref(a, kv_head, rho0 + x * kTileM + row_in_tile);
     if (kDense) {
       constexpr int kLow = -2147483647 - 1, kHigh = 2147483647;
       mask.limit = kLow;
@@ -234,7 +272,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int hi = __reduce_max_sync(0xffffffffu, in_doc ? mask.limit : kLow);
       const int d_lo = __reduce_min_sync(0xffffffffu, in_doc ? mask.doc : kHigh);
       const int d_hi = __reduce_max_sync(0xffffffffu, in_doc ? mask.doc : kLow);
-      if (lane == 0) {
+      if (lane == 0 && half == 0) {
         atomicMin(&seen[0], lo), atomicMax(&seen[1], hi);
         atomicMin(&seen[2], d_lo), atomicMax(&seen[3], d_hi);
       }
@@ -242,7 +280,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     constexpr int kVecs = D / 8;
     uint8_t *dst = smem + L::kQ + x * L::kTile;
 #pragma unroll 4
-    for (int i = tid & 127; i < kTileM * kVecs; i += kTileM) {
+    for (int i = tid & (kTileThreads - 1); i < kTileM * kVecs; i += kTileThreads) {
       const int r = i / kVecs, c = i % kVecs;
       const RowRef o = row_ref(a, kv_head, rho0 + x * kTileM + r);
       int4 v = make_int4(0, 0, 0, 0);
@@ -262,8 +300,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   // (each role sets its registers in its own branch: the compiler then allots
   // them per branch)
-  if (warp == 9) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  if (warp == kLoadWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
     // ------------------------------------------------------------- loader
     if (lane == 0) prefetch_map(&k_map), prefetch_map(&v_map);
     int tile, it = 0;
@@ -300,8 +338,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // loads in flight land before the block's memory is given back
     for (int i = max(0, it - kStages); i < it; ++i)
       mbar_wait_bounded(&kv_full[i % kStages], (i / kStages) & 1, 2000000000ull);
-  } else if (warp == 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  } else if (warp == kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
     // ------------------------------------------------------------- mma
     constexpr uint32_t kQK = mma_desc(kBf16, false, kTileM, kTileN);
     constexpr uint32_t kPV = mma_desc(kBf16, true, kTileM, D);
@@ -322,54 +360,63 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                smem_desc(kv_addr + st * L::kTile + k * 2048, kHalfBytes, 1024), kPV,
                accumulate || k > 0);
     };
-    int tile, it = 0;
-    bool whole;
-    bool ok = wait_or_stop(q_full, 0, stopped);
-    bool more = ok && scan.next(tile, whole);
-    if (more) {
-      ok = wait_or_stop(&kv_full[0], 0, stopped);
-      tc_fence_after();
-      if (ok && lane == 0) {
-        for (int t = 0; t < tiles; ++t) score(t, 0);
-        mma_commit(&kv_empty[0]);
-      }
-      it = 1;
-    }
-    for (int j = 0; ok && more; ++j) {
-      more = scan.next(tile, whole);
-      const int v_st = it % kStages, k_st = (it + 1) % kStages;
-      ok = wait_or_stop(&kv_full[v_st], (it / kStages) & 1, stopped);
-      if (ok && more)
-        ok = wait_or_stop(&kv_full[k_st], ((it + 1) / kStages) & 1, stopped);
-      for (int t = 0; ok && t < tiles; ++t) {
-        ok = wait_or_stop(&p_full[t], j & 1, stopped);
+    // One thread waits and issues: a vote per wait would cost as much as an mma.
+    const int n = scan.count();
+    if (elect_one()) {
+      bool ok = lane_wait(q_full, 0, stopped);
+      if (n > 0) {
+        ok = ok && lane_wait(&kv_full[0], 0, stopped);
         tc_fence_after();
-        if (ok && lane == 0) {
-          weigh(t, v_st, j > 0);
-          if (!more) mma_commit(&o_done[t]);
-          if (t == tiles - 1) mma_commit(&kv_empty[v_st]);
-          if (more) {
-            score(t, k_st);
-            if (t == tiles - 1) mma_commit(&kv_empty[k_st]);
-          }
+        if (ok) {
+          score(0, 0);
+          if (tiles > 1) score(1, 0);
+          mma_commit(&kv_empty[0]);
         }
-        __syncwarp();
       }
-      it += 2;
+      int v_st = 1, v_phase = 0;
+#pragma unroll 1
+      for (int j = 0; ok && j < n; ++j) {
+        const bool more = j + 1 < n;
+        int k_st = v_st + 1, k_phase = v_phase;
+        if (k_st == kStages) k_st = 0, k_phase ^= 1;
+        ok = lane_wait(&kv_full[v_st], v_phase, stopped);
+        if (ok && more) ok = lane_wait(&kv_full[k_st], k_phase, stopped);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (t >= tiles) break;
+          ok = ok && lane_wait(&p_full[t], j & 1, stopped);
+          if (!ok) break;
+          tc_fence_after();
+          weigh(t, v_st, j > 0);
+          if (more) score(t, k_st);
+          if (t == tiles - 1) {
+            mma_commit(&kv_empty[v_st]);
+            if (more) mma_commit(&kv_empty[k_st]);
+          }
+          if (!more) mma_commit(&o_done[t]);
+        }
+        v_st = k_st + 1, v_phase = k_phase;
+        if (v_st == kStages) v_st = 0, v_phase ^= 1;
+      }
+      if (!ok) {  // only after a wait that ran out: let the mma in flight end
+        mma_commit(drain);
+        mbar_wait_bounded(drain, 0, 2000000000ull);
+      }
     }
-    if (!ok) {  // only after a wait that ran out: let the mma in flight end
-      if (lane == 0) mma_commit(drain);
-      mbar_wait_bounded(drain, 0, 2000000000ull);
-    }
-  } else if (warp > 9) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    __syncwarp();
+  } else if (warp > kLoadWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
     if (x < tiles) {
     // ------------------------------------------------------------- softmax
     const uint32_t lane_base = static_cast<uint32_t>(warp & 3) << 21;
+    constexpr int kKeys = kTileN / 2;  // of this thread
     const uint32_t s_addr = tmem + lane_base + x * kTileN;
-    const uint32_t o_addr = tmem + lane_base + 2 * kTileN + x * D;
+    const uint32_t o_addr = tmem + lane_base + 2 * kTileN + x * D + half * (D / 2);
+    float *xch = reinterpret_cast<float *>(smem + L::kXch) + x * 2 * kTileM;
+    float *mine = xch + half * kTileM + row_in_tile;
+    const float *other = xch + (1 - half) * kTileM + row_in_tile;
     float m = -INFINITY, l = 0.f;
     const float slope = kBias && ref.valid ? a.slopes[ref.head] * kLog2e : 0.f;
     float q_at = 0.f;  // position in the prefix, for the distance bias
@@ -395,32 +442,49 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         bad = __ballot_sync(0xffffffffu, out_of_cache);
       }
       ok = wait_or_stop(&s_full[x], j & 1, stopped);
-      if (!ok) break;
       tc_fence_after();
-      float s[kTileN];
+      float s[kKeys];
 #pragma unroll
-      for (int c = 0; c < kTileN / 32; ++c)
-        tmem_ld32(s_addr + c * 32, reinterpret_cast<uint32_t(&)[32]>(s[c * 32]));
+      for (int c = 0; c < kKeys / 32; ++c)
+        tmem_ld32(s_addr + half * kKeys + c * 32, reinterpret_cast<uint32_t(&)[32]>(s[c * 32]));
       tmem_wait_ld();
+      const int key0 = tile * kTileN + half * kKeys;
       // x = s c in log2 units, unless it is only scaled (then c goes into exp2)
       if (kCap || kBias) {
+        if (kCap) {
+          // tanh by a polynomial while every score of the warp's rows is small
+          // against the cap, as they mostly are: on the FMA pipe it costs a
+          // quarter of the exponential and reciprocal of the general form
+          // tanh(u) = 1 - 2 / (1 + e^2u)
+          float big = 0.f;
 #pragma unroll
-        for (int i = 0; i < kTileN; ++i) {
-          if (kCap) {
-            // tanh(u) = 1 - 2 / (1 + e^2u): absolute error of a few 2^-22
-            const float e = ex2(s[i] * a.cap_in);
-            s[i] = fmaf(rcp(1.f + e), -2.f * a.cap_out, a.cap_out);
+          for (int i = 0; i < kKeys; i += 2)
+            big = fmaxf(fmaxf(big, fabsf(s[i])), fabsf(s[i + 1]));
+          if (__all_sync(0xffffffffu, big * a.cap_u <= kSmallTanh)) {
+            const f32x2 cu = pack2(a.cap_u, a.cap_u), c2 = pack2(a.scale_log2, a.scale_log2);
+#pragma unroll
+            for (int i = 0; i < kKeys; i += 2) {
+              const f32x2 x = pack2(s[i], s[i + 1]), u = mul2(x, cu);
+              unpack2(mul2(mul2(x, c2), tanh_ratio(mul2(u, u))), s[i], s[i + 1]);
+            }
           } else {
-            s[i] *= a.scale_log2;
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i) {
+              const float e = ex2(s[i] * a.cap_in);
+              s[i] = fmaf(rcp(1.f + e), -2.f * a.cap_out, a.cap_out);
+            }
           }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kKeys; ++i) s[i] *= a.scale_log2;
         }
         if (kBias) {
           if (kDense) {
             const float at = static_cast<float>(static_cast<long long>(mask.pos) -
                                                 a.stats[tile].pos_min);
-            const float4 *rel = reinterpret_cast<const float4 *>(a.k_rel + tile * kTileN);
+            const float4 *rel = reinterpret_cast<const float4 *>(a.k_rel + key0);
 #pragma unroll
-            for (int i = 0; i < kTileN / 4; ++i) {
+            for (int i = 0; i < kKeys / 4; ++i) {
               const float4 p = rel[i];
               s[4 * i] = fmaf(-slope, fabsf(at - p.x), s[4 * i]);
               s[4 * i + 1] = fmaf(-slope, fabsf(at - p.y), s[4 * i + 1]);
@@ -428,17 +492,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               s[4 * i + 3] = fmaf(-slope, fabsf(at - p.w), s[4 * i + 3]);
             }
           } else {
-            const float at = q_at - static_cast<float>(tile * kTileN);
+            const float at = q_at - static_cast<float>(key0);
 #pragma unroll
-            for (int i = 0; i < kTileN; ++i)
+            for (int i = 0; i < kKeys; ++i)
               s[i] = fmaf(-slope, fabsf(at - static_cast<float>(i)), s[i]);
           }
         }
       }
       if (kDense && !whole) {
-        const int4 *kp = reinterpret_cast<const int4 *>(a.k_pos32 + tile * kTileN);
+        const int4 *kp = reinterpret_cast<const int4 *>(a.k_pos32 + key0);
 #pragma unroll
-        for (int i = 0; i < kTileN / 4; ++i) {
+        for (int i = 0; i < kKeys / 4; ++i) {
           const int4 p = kp[i];
           if (p.x >= mask.limit) s[4 * i] = -INFINITY;
           if (p.y >= mask.limit) s[4 * i + 1] = -INFINITY;
@@ -446,9 +510,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (p.w >= mask.limit) s[4 * i + 3] = -INFINITY;
         }
         if (a.k_doc32) {
-          const int4 *kd = reinterpret_cast<const int4 *>(a.k_doc32 + tile * kTileN);
+          const int4 *kd = reinterpret_cast<const int4 *>(a.k_doc32 + key0);
 #pragma unroll
-          for (int i = 0; i < kTileN / 4; ++i) {
+          for (int i = 0; i < kKeys / 4; ++i) {
             const int4 p = kd[i];
             if (p.x != mask.doc) s[4 * i] = -INFINITY;
             if (p.y != mask.doc) s[4 * i + 1] = -INFINITY;
@@ -460,26 +524,38 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (!kDense && bad) {
         const int rows_of = min(kTileN, a.block_size);
 #pragma unroll
-        for (int i = 0; i < kTileN; ++i)
-          if ((bad >> (i / rows_of)) & 1) s[i] = -INFINITY;
+        for (int i = 0; i < kKeys; ++i)
+          if ((bad >> ((half * kKeys + i) / rows_of)) & 1) s[i] = -INFINITY;
       }
       const float c = kCap || kBias ? 1.f : a.scale_log2;
       float t0 = s[0], t1 = s[1], t2 = s[2], t3 = s[3];
 #pragma unroll
-      for (int i = 4; i < kTileN; i += 4) {
-        t0 = fmaxf(t0, s[i]), t1 = fmaxf(t1, s[i + 1]);
-        t2 = fmaxf(t2, s[i + 2]), t3 = fmaxf(t3, s[i + 3]);
+      for (int i = 4; i + 7 < kKeys; i += 8) {
+        t0 = fmaxf(fmaxf(t0, s[i]), s[i + 1]);
+        t1 = fmaxf(fmaxf(t1, s[i + 2]), s[i + 3]);
+        t2 = fmaxf(fmaxf(t2, s[i + 4]), s[i + 5]);
+        t3 = fmaxf(fmaxf(t3, s[i + 6]), s[i + 7]);
       }
+      t0 = fmaxf(fmaxf(t0, s[kKeys - 4]), s[kKeys - 3]);
+      t1 = fmaxf(fmaxf(t1, s[kKeys - 2]), s[kKeys - 1]);
       const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * c;
-      const bool grow = top > m + kLazy;  // also the first finite score
-      if (__any_sync(0xffffffffu, grow)) {
-        const float to = grow ? top : m;
+      // O is rescaled when a row's maximum has grown (also at its first finite
+      // score), by both of its threads alike
+      if (tile_any(x, top > m + kLazy || !ok)) {
+        *mine = top;
+        if (tile_any(x, !ok)) {
+          ok = false;
+          break;
+        }
+        const float both = fmaxf(top, *other);
+        const bool grow = both > m + kLazy;
+        const float to = grow ? both : m;
         const float keep = grow ? ex2(m - to) : 1.f;
         m = to;
         l *= keep;
         if (j > 0) {  // the score barrier also covers the last product into O
 #pragma unroll 1
-          for (int k = 0; k < D / 32; ++k) {
+          for (int k = 0; k < D / 64; ++k) {
             uint32_t o[32];
             tmem_ld32(o_addr + k * 32, o);
             tmem_wait_ld();
@@ -490,20 +566,36 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       }
       const float off = m == -INFINITY ? 0.f : m;
-      float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      const f32x2 c2 = pack2(c, c), off2 = pack2(-off, -off);
+      f32x2 l0 = pack2(0.f, 0.f), l1 = l0;
+      // the weights, some of them by the polynomial
+      auto weights = [&](auto some_fma) {
         uint32_t p[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-          const float u = ex2(fmaf(s[h * 64 + 2 * i], c, -off));
-          const float v = ex2(fmaf(s[h * 64 + 2 * i + 1], c, -off));
-          l0 += u, l1 += v;
-          p[i] = pair_from_float<T>(u, v);
+          const f32x2 v = fma2(pack2(s[2 * i], s[2 * i + 1]), c2, off2);
+          float e, f;
+          if (decltype(some_fma)::value && i % 8 >= 8 - kFmaOf8) {
+            exp2_fma(v, e, f);
+          } else {
+            unpack2(v, e, f);
+            e = ex2(e), f = ex2(f);
+          }
+          if (i & 1)
+            l1 = add2(l1, pack2(e, f));
+          else
+            l0 = add2(l0, pack2(e, f));
+          p[i] = pair_from_float<T>(e, f);
         }
-        tmem_st32(s_addr + h * 32, p);
-      }
-      l += l0 + l1;
+        tmem_st32(s_addr + half * (kKeys / 2), p);
+      };
+      if (whole)
+        weights(Yes{});
+      else
+        weights(No{});
+      float u0, u1;
+      unpack2(add2(l0, l1), u0, u1);
+      l += u0 + u1;
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&p_full[x]);
@@ -512,11 +604,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // ------------------------------------------------------------- result
     if (ok && j > 0) ok = wait_or_stop(&o_done[x], 0, stopped);
     tc_fence_after();
+    if (ok || j == 0) *mine = l;  // (after a break nobody reads it)
+    ok = !tile_any(x, !ok);
+    if (ok) l += *other;
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : NAN);
     const long long row = static_cast<long long>(ref.token) * a.heads + ref.head;
     bool finite = true;
 #pragma unroll 1
-    for (int k = 0; k < D / 32; ++k) {
+    for (int k = 0; k < D / 64; ++k) {
       float o[32];
       if (ok && j > 0) {
         tmem_ld32(o_addr + k * 32, reinterpret_cast<uint32_t(&)[32]>(o));
@@ -528,8 +623,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         finite = finite && fabsf(o[i]) <= 3.4028235e38f;
       }
       if (!ref.valid) continue;
+      const int d = half * (D / 2) + k * 32;
       if (a.slices == 0) {
-        T *dst = static_cast<T *>(a.out) + row * D + k * 32;
+        T *dst = static_cast<T *>(a.out) + row * D + d;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           int4 w;
@@ -540,15 +636,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           st_v4(dst + 8 * i, w);
         }
       } else {
-        float *dst = a.part_o + (static_cast<long long>(slice) * a.tokens * a.heads + row) * D +
-                     k * 32;
+        float *dst =
+            a.part_o + (static_cast<long long>(slice) * a.tokens * a.heads + row) * D + d;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           *reinterpret_cast<float4 *>(dst + 4 * i) =
               make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
       }
     }
-    if (ref.valid) {
+    if (ref.valid && half == 0) {
       if (a.slices == 0) {
         if (a.lse) a.lse[row] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
       } else {
@@ -557,13 +653,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
     }
     if (kDense && a.slices == 0 && ok) {
-      __syncwarp();  // a row written above is written again below
-      uint32_t again = __ballot_sync(0xffffffffu, ref.valid && !finite);
-      while (again) {
-        const int src = __ffs(again) - 1;
-        again &= again - 1;
-        strict_position_row<T, D>(a.pos, __shfl_sync(0xffffffffu, ref.token, src),
-                                  __shfl_sync(0xffffffffu, ref.head, src));
+      const bool wrong = ref.valid && !finite;
+      if (tile_any(x, wrong)) {  // what was written above is written again below
+        *mine = wrong ? 1.f : 0.f;
+        tile_any(x, false);
+        uint32_t again =
+            half == 0 ? __ballot_sync(0xffffffffu, *mine + *other > 0.f) : 0u;
+        while (again) {
+          const int src = __ffs(again) - 1;
+          again &= again - 1;
+          strict_position_row<T, D>(a.pos, __shfl_sync(0xffffffffu, ref.token, src),
+                                    __shfl_sync(0xffffffffu, ref.head, src));
+        }
       }
     }
     }
@@ -571,7 +672,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) tmem_free(tmem, 512);
+  if (warp == kMmaWarp) tmem_free(tmem, 512);
 }
 
 }  // namespace lmc

@@ -46,6 +46,18 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
       : "memory");
 }
 
+// One lane of a converged warp.  Descriptors of tcgen05.mma live in uniform
+// registers: under this predicate, with operands that are the same in the whole
+// warp, the compiler keeps them there (under `lane == 0` it moves each one over,
+// and the mma waited on those moves half the time).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}"
+      : "=r"(r));
+  return r != 0;
+}
+
 // --- tcgen05.mma, kind::f16, fp32 accumulators, one CTA
 // Instruction descriptor: D fp32, A and B of one 16-bit type (bf16 or f16), A
 // K-major, B K-major or (b_mn) MN-major, M x N.
@@ -113,26 +125,39 @@ __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
                : "memory");
 }
 
-// One lane's wait; see wait_or_stop.
+// Up to 2^16 tries for a phase, of at most about a microsecond each.  The loop is
+// in one asm block: written around the try in C++ the way out of it cost 300
+// cycles per wait, also when the phase was long complete.
+__device__ __forceinline__ bool tries(uint64_t *bar, unsigned parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n.reg .pred p, q;\n.reg .u32 n;\nmov.u32 n, 0;\n"
+      "again_%=:\n"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n"
+      "@p bra done_%=;\n"
+      "add.u32 n, n, 1;\nsetp.lt.u32 q, n, 65536;\n@q bra again_%=;\n"
+      "done_%=:\nselp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+
+// One lane's wait; see wait_or_stop.  At most 32 x 2^16 tries.
 __device__ __forceinline__ bool lane_wait(uint64_t *bar, unsigned parity, int *stopped) {
-  if (mbar_try_wait_parity(bar, parity)) return true;
-  unsigned long long t0, t1;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
-  for (;;) {
+  if (__builtin_expect(tries(bar, parity), 1)) return true;
 #pragma unroll 1
-    for (int i = 0; i < 64; ++i)
-      if (mbar_try_wait_parity(bar, parity)) return true;
+  for (int i = 0; i < 31; ++i) {
     if (*reinterpret_cast<volatile int *>(stopped)) return false;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t1));
-    if (t1 - t0 > 2000000000ull) break;
+    if (tries(bar, parity)) return true;
   }
   *reinterpret_cast<volatile int *>(stopped) = 1;
   return false;
 }
 
-// A whole warp's wait for a phase, with an end: after two seconds, or as soon as
-// another warp of the block gave up, the block's flag is set and every lane of
-// the caller gets false.
+// A whole warp's wait for a phase, with an end: after some two million tries (0.1
+// to 2 seconds), or soon after another warp of the block gave up, the block's
+// flag is set and every lane of the caller gets false.
 __device__ __forceinline__ bool wait_or_stop(uint64_t *bar, unsigned parity, int *stopped) {
   return __all_sync(0xffffffffu, lane_wait(bar, parity, stopped));
 }
@@ -146,6 +171,73 @@ __device__ __forceinline__ float rcp(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// --- pairs of fp32 in one instruction
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pack2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float &a, float &b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 2^x for x below 128 on the FMA pipe: x = j + f with f in [-1/2, 1/2], a
+// degree-5 polynomial for 2^f (relative minimax over the interval by the Remez
+// exchange: 7.5e-8, 2.3e-7 in fp32 Horner form, as exact as ex2) and j added to
+// the exponent.  Below 2^-126 it stays there (weights of that size vanish next
+// to the row's largest); NaN and what it leads to stay outside the finite range.
+__device__ __forceinline__ void exp2_fma(f32x2 x, float &a, float &b) {
+  constexpr float kShift = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer
+  unpack2(x, a, b);
+  x = pack2(max_nan(a, -126.f), max_nan(b, -126.f));
+  const f32x2 t = add2(x, pack2(kShift, kShift));
+  const f32x2 f = fma2(add2(t, pack2(-kShift, -kShift)), pack2(-1.f, -1.f), x);
+  f32x2 p = pack2(0.0013276472454890609f, 0.0013276472454890609f);
+  p = fma2(p, f, pack2(0.009675540961325169f, 0.009675540961325169f));
+  p = fma2(p, f, pack2(0.05550713092088699f, 0.05550713092088699f));
+  p = fma2(p, f, pack2(0.24022120237350464f, 0.24022120237350464f));
+  p = fma2(p, f, pack2(0.6931469440460205f, 0.6931469440460205f));
+  p = fma2(p, f, pack2(1.0000001192092896f, 1.0000001192092896f));
+  float ta, tb;
+  unpack2(t, ta, tb);
+  unpack2(p, a, b);
+  a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(ta) << 23));
+  b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23));
+}
+
+// tanh(u) / u as a polynomial in u^2 for |u| <= 3/4 (relative minimax by the
+// Remez exchange, degree 5: 2.9e-8).
+constexpr float kSmallTanh = 0.75f;
+__device__ __forceinline__ f32x2 tanh_ratio(f32x2 u2) {
+  f32x2 p = pack2(-0.004716257099062204f, -0.004716257099062204f);
+  p = fma2(p, u2, pack2(0.01958290860056877f, 0.01958290860056877f));
+  p = fma2(p, u2, pack2(-0.05334442853927612f, -0.05334442853927612f));
+  p = fma2(p, u2, pack2(0.1332540661096573f, 0.1332540661096573f));
+  p = fma2(p, u2, pack2(-0.33332958817481995f, -0.33332958817481995f));
+  return fma2(p, u2, pack2(1.f, 1.f));
 }
 
 }  // namespace lmc
