@@ -47,6 +47,19 @@ __device__ __forceinline__ uint32_t pair_from_float<__half>(float a, float b) {
   return *reinterpret_cast<uint32_t *>(&w);
 }
 
+// --- 16-byte asynchronous copies; with `valid` false zeros, nothing is read
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(valid ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 // One query row on one warp; lane l holds elements [l D/32, (l + 1) D/32).
 template <typename T, int D>
 struct WarpRow {

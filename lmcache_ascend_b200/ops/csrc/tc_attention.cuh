@@ -67,12 +67,22 @@ struct TcArgs {
 template <int D>
 struct TcSmem {
   static constexpr int kTile = kTileN * D * 2;
-  static constexpr int kQ = 0;                       // two row tiles
-  static constexpr int kKV = 2 * kTile;              // kStages key tiles
+  static constexpr int kQ = 0;  // two row tiles; at the end their results pass through
+  static constexpr int kQTile = kTileM * 256;
+  static constexpr int kKV = 2 * kQTile;             // kStages key tiles
   static constexpr int kBars = kKV + kStages * kTile;
-  static constexpr int kXch = kBars + 256;           // two floats per row
-  static constexpr int kBytes = kXch + 2048 + 1024;  // + alignment to the swizzle's 1 KB
+  static constexpr int kXch = kBars + 256;    // two floats per row
+  static constexpr int kQAt = kXch + 2048;    // where each row's query lies
+  static constexpr int kRowAt = kQAt + 2048;  // and its result, -1 behind the last row
+  static constexpr int kBytes = kRowAt + 1024 + 1024;  // + alignment to the swizzle's 1 KB
 };
+
+// A load whose value nobody waits for.
+__device__ __forceinline__ void touch(const void *p) {
+  uint32_t v;
+  asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p));
+  static_cast<void>(v);
+}
 
 // True in all threads of a row tile if it is in any of them.
 __device__ __forceinline__ bool tile_any(int tile, bool v) {
@@ -239,7 +249,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int t_end = min(a.k_tiles, t_begin + a.tiles_per_slice);
 
   if (warp == kMmaWarp) tmem_alloc(tmem_slot, 512);
-  if (tid == 0) {
+  if (warp == kLoadWarp && lane == 0) {
+    prefetch_map(&k_map), prefetch_map(&v_map);
     for (int i = 0; i < kStages; ++i) mbar_init(&kv_full[i], 1), mbar_init(&kv_empty[i], 1);
     for (int i = 0; i < 2; ++i)
       mbar_init(&s_full[i], 1), mbar_init(&p_full[i], kTileThreads), mbar_init(&o_done[i], 1);
@@ -250,52 +261,55 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     seen[2] = 2147483647, seen[3] = -2147483647 - 1;
     fence_mbar_init();
   }
+  // Rows, while that happens: Q on its way to shared memory (128-byte swizzled
+  // rows), then the masks.
+  RowRef ref = {0, 0, false};
+  RowMask mask = {0, 0, 0};
+  const int x = warp >> 3, half = (warp >> 2) & 1;  // row tile, and which 64 keys
+  const int row_in_tile = tid & 127;
+  int lim_lo = 2147483647, lim_hi = -2147483647 - 1, doc_lo = lim_lo, doc_hi = lim_hi;
+  long long *q_at = reinterpret_cast<long long *>(smem + L::kQAt) + x * kTileM;
+  int *row_at = reinterpret_cast<int *>(smem + L::kRowAt) + x * kTileM;
+  if (warp < kMmaWarp && x < tiles) {
+    ref = row_ref(a, kv_head, rho0 + x * kTileM + row_in_tile);
+    if (half == 0) {
+      const int b = ref.token / a.q_len;
+      q_at[row_in_tile] = b * a.q_batch + (ref.token - b * a.q_len) * a.q_token +
+                          (ref.valid ? ref.head : 0) * a.q_head;
+      row_at[row_in_tile] = ref.valid ? ref.token * a.heads + ref.head : -1;
+    }
+    tile_any(x, false);
+    constexpr int kVecs = D / 8, kAtOnce = kTileThreads / kVecs;
+    const int c = tid % kVecs, r0 = (tid & (kTileThreads - 1)) / kVecs;
+    const uint32_t dst = smem_u32(smem + L::kQ + x * L::kQTile) + (c >> 3) * kHalfBytes;
+    const T *q = static_cast<const T *>(a.q) + c * 8;
+#pragma unroll
+    for (int i = 0; i < kTileM / kAtOnce; ++i) {
+      const int r = r0 + i * kAtOnce;
+      cp_async16(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4), q + q_at[r], row_at[r] >= 0);
+    }
+    if (kDense) {
+      mask.limit = lim_hi;
+      if (ref.valid) mask = row_mask(a.pos, ref.token);
+      const bool in_doc = ref.valid && mask.doc >= 0;
+      lim_lo = __reduce_min_sync(0xffffffffu, ref.valid ? mask.limit : lim_lo);
+      lim_hi = __reduce_max_sync(0xffffffffu, in_doc ? mask.limit : lim_hi);
+      doc_lo = __reduce_min_sync(0xffffffffu, in_doc ? mask.doc : doc_lo);
+      doc_hi = __reduce_max_sync(0xffffffffu, in_doc ? mask.doc : doc_hi);
+    }
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   // the whole of tensor memory starts at column 0: a constant address
   constexpr uint32_t tmem = 0;
-
-  // Rows: masks, and Q into shared memory (128-byte swizzled rows).
-  RowRef ref = {0, 0, false};
-  RowMask mask = {0, 0, 0};
-  const int x = warp >> 3, half = (warp >> 2) & 1;  // row tile, and which 64 keys
-  const int row_in_tile = tid & 127;
-  if (warp < kMmaWarp && x < tiles) {
-    ref = row_ref(a, kv_head, rho0 + x * kTileM + row_in_tile);
-    if (kDense) {
-      constexpr int kLow = -2147483647 - 1, kHigh = 2147483647;
-      mask.limit = kLow;
-      if (ref.valid) mask = row_mask(a.pos, ref.token);
-      const bool in_doc = ref.valid && mask.doc >= 0;
-      const int lo = __reduce_min_sync(0xffffffffu, ref.valid ? mask.limit : kHigh);
-      const int hi = __reduce_max_sync(0xffffffffu, in_doc ? mask.limit : kLow);
-      const int d_lo = __reduce_min_sync(0xffffffffu, in_doc ? mask.doc : kHigh);
-      const int d_hi = __reduce_max_sync(0xffffffffu, in_doc ? mask.doc : kLow);
-      if (lane == 0 && half == 0) {
-        atomicMin(&seen[0], lo), atomicMax(&seen[1], hi);
-        atomicMin(&seen[2], d_lo), atomicMax(&seen[3], d_hi);
-      }
+  if (kDense) {
+    if (warp < kMmaWarp && x < tiles && lane == 0 && half == 0) {
+      atomicMin(&seen[0], lim_lo), atomicMax(&seen[1], lim_hi);
+      atomicMin(&seen[2], doc_lo), atomicMax(&seen[3], doc_hi);
     }
-    constexpr int kVecs = D / 8;
-    uint8_t *dst = smem + L::kQ + x * L::kTile;
-#pragma unroll 4
-    for (int i = tid & (kTileThreads - 1); i < kTileM * kVecs; i += kTileThreads) {
-      const int r = i / kVecs, c = i % kVecs;
-      const RowRef o = row_ref(a, kv_head, rho0 + x * kTileM + r);
-      int4 v = make_int4(0, 0, 0, 0);
-      if (o.valid) {
-        const int b = o.token / a.q_len;
-        v = ld_nc_v4(static_cast<const T *>(a.q) + b * a.q_batch +
-                     (o.token - b * a.q_len) * a.q_token + o.head * a.q_head + c * 8);
-      }
-      *reinterpret_cast<int4 *>(dst + (c >> 3) * kHalfBytes + r * 128 +
-                                (((c & 7) ^ (r & 7)) << 4)) = v;
-    }
-    fence_proxy_async_smem();
-    mbar_arrive(q_full);
+    __syncthreads();  // `seen` is whole
   }
-  __syncthreads();  // `seen` is whole
   TileScan<kDense> scan(a, t_begin, t_end, seen);
 
   // (each role sets its registers in its own branch: the compiler then allots
@@ -303,7 +317,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp == kLoadWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
     // ------------------------------------------------------------- loader
-    if (lane == 0) prefetch_map(&k_map), prefetch_map(&v_map);
     int tile, it = 0;
     bool whole, ok = true;
     const int boxes = kDense ? 1 : max(1, kTileN / a.block_size);
@@ -348,7 +361,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
         const uint32_t off = (k >> 2) * kHalfBytes + (k & 3) * 32;
-        mma_ss(tmem + t * kTileN, smem_desc(q_addr + t * L::kTile + off, 16, 1024),
+        mma_ss(tmem + t * kTileN, smem_desc(q_addr + t * L::kQTile + off, 16, 1024),
                smem_desc(kv_addr + st * L::kTile + off, 16, 1024), kQK, k > 0);
       }
       mma_commit(&s_full[t]);
@@ -419,16 +432,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const float *other = xch + (1 - half) * kTileM + row_in_tile;
     float m = -INFINITY, l = 0.f;
     const float slope = kBias && ref.valid ? a.slopes[ref.head] * kLog2e : 0.f;
-    float q_at = 0.f;  // position in the prefix, for the distance bias
+    float q_place = 0.f;  // position in the prefix, for the distance bias
     int own = 0;
     if (!kDense && ref.valid) {
       const int b = ref.token / a.q_len;
       own = max(0, a.own_lens[b]) - a.q_len + (ref.token - b * a.q_len);
-      q_at = static_cast<float>(a.prefix_len + own);
+      q_place = static_cast<float>(a.prefix_len + own);
     }
+    cp_async_commit();
+    cp_async_wait<0>();
+    fence_proxy_async_smem();
+    mbar_arrive(q_full);
     int tile, j = 0;
     bool whole, ok = true;
     while (scan.next(tile, whole)) {
+      const int key0 = tile * kTileN + half * kKeys;
+      // positions and documents to L1 while the scores are computed
+      if (kDense && lane < 2) {
+        if (!whole) touch(a.k_pos32 + key0 + lane * 32);
+        if (!whole && a.k_doc32) touch(a.k_doc32 + key0 + lane * 32);
+        if (kBias) touch(a.k_rel + key0 + lane * 32);
+      }
       uint32_t bad = 0;  // pages of this tile that lie outside the cache
       if (!kDense) {
         const int boxes = max(1, kTileN / a.block_size);
@@ -448,7 +472,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int c = 0; c < kKeys / 32; ++c)
         tmem_ld32(s_addr + half * kKeys + c * 32, reinterpret_cast<uint32_t(&)[32]>(s[c * 32]));
       tmem_wait_ld();
-      const int key0 = tile * kTileN + half * kKeys;
       // x = s c in log2 units, unless it is only scaled (then c goes into exp2)
       if (kCap || kBias) {
         if (kCap) {
@@ -492,7 +515,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               s[4 * i + 3] = fmaf(-slope, fabsf(at - p.w), s[4 * i + 3]);
             }
           } else {
-            const float at = q_at - static_cast<float>(key0);
+            const float at = q_place - static_cast<float>(key0);
 #pragma unroll
             for (int i = 0; i < kKeys; ++i)
               s[i] = fmaf(-slope, fabsf(at - static_cast<float>(i)), s[i]);
@@ -608,8 +631,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     ok = !tile_any(x, !ok);
     if (ok) l += *other;
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : NAN);
-    const long long row = static_cast<long long>(ref.token) * a.heads + ref.head;
+    const long long row = row_at[row_in_tile];
     bool finite = true;
+    // 64 columns at a time (32 of each half) through the tile's share of Q's
+    // memory, so that stores to the rows run along them
+    uint8_t *stage = smem + L::kQ + x * L::kQTile;
 #pragma unroll 1
     for (int k = 0; k < D / 64; ++k) {
       float o[32];
@@ -622,27 +648,49 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         o[i] = ok ? (j > 0 ? o[i] * inv : 0.f) : NAN;
         finite = finite && fabsf(o[i]) <= 3.4028235e38f;
       }
-      if (!ref.valid) continue;
-      const int d = half * (D / 2) + k * 32;
+      const int swz = row_in_tile & 7;
       if (a.slices == 0) {
-        T *dst = static_cast<T *>(a.out) + row * D + d;
+        uint8_t *w = stage + row_in_tile * 128;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          int4 w;
-          w.x = pair_from_float<T>(o[8 * i], o[8 * i + 1]);
-          w.y = pair_from_float<T>(o[8 * i + 2], o[8 * i + 3]);
-          w.z = pair_from_float<T>(o[8 * i + 4], o[8 * i + 5]);
-          w.w = pair_from_float<T>(o[8 * i + 6], o[8 * i + 7]);
-          st_v4(dst + 8 * i, w);
+          int4 v;
+          v.x = pair_from_float<T>(o[8 * i], o[8 * i + 1]);
+          v.y = pair_from_float<T>(o[8 * i + 2], o[8 * i + 3]);
+          v.z = pair_from_float<T>(o[8 * i + 4], o[8 * i + 5]);
+          v.w = pair_from_float<T>(o[8 * i + 6], o[8 * i + 7]);
+          *reinterpret_cast<int4 *>(w + (((half * 4 + i) ^ swz) << 4)) = v;
         }
       } else {
-        float *dst =
-            a.part_o + (static_cast<long long>(slice) * a.tokens * a.heads + row) * D + d;
+        uint8_t *w = stage + half * kHalfBytes + row_in_tile * 128;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          *reinterpret_cast<float4 *>(dst + 4 * i) =
+          *reinterpret_cast<float4 *>(w + ((i ^ swz) << 4)) =
               make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
       }
+      tile_any(x, false);
+      const int in_tile = tid & (kTileThreads - 1);
+      if (a.slices == 0) {
+#pragma unroll
+        for (int i = 0; i < kTileM * 8 / kTileThreads; ++i) {
+          const int r = (in_tile >> 3) + i * (kTileThreads / 8), v = in_tile & 7;
+          if (row_at[r] < 0) continue;
+          st_v4(static_cast<T *>(a.out) + static_cast<long long>(row_at[r]) * D +
+                    (v >> 2) * (D / 2) + k * 32 + (v & 3) * 8,
+                *reinterpret_cast<const int4 *>(stage + r * 128 + ((v ^ (r & 7)) << 4)));
+        }
+      } else {
+        float *part = a.part_o + static_cast<long long>(slice) * a.tokens * a.heads * D;
+#pragma unroll
+        for (int i = 0; i < kTileM * 16 / kTileThreads; ++i) {
+          const int r = (in_tile >> 4) + i * (kTileThreads / 16), v = in_tile & 15;
+          if (row_at[r] < 0) continue;
+          st_v4(part + static_cast<long long>(row_at[r]) * D + (v >> 3) * (D / 2) + k * 32 +
+                    (v & 7) * 4,
+                *reinterpret_cast<const int4 *>(stage + (v >> 3) * kHalfBytes + r * 128 +
+                                                (((v & 7) ^ (r & 7)) << 4)));
+        }
+      }
+      if (k + 1 < D / 64) tile_any(x, false);
     }
     if (ref.valid && half == 0) {
       if (a.slices == 0) {

@@ -58,6 +58,13 @@ __device__ __forceinline__ bool elect_one() {
   return r != 0;
 }
 
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
 // --- tcgen05.mma, kind::f16, fp32 accumulators, one CTA
 // Instruction descriptor: D fp32, A and B of one 16-bit type (bf16 or f16), A
 // K-major, B K-major or (b_mn) MN-major, M x N.
