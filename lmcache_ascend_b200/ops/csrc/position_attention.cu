@@ -13,8 +13,9 @@ namespace {
 // Positions as 32-bit integers padded to whole tiles with one that no row sees,
 // and each tile's range, so that a block can skip tiles or leave out the masks.
 __global__ void __launch_bounds__(kTileN)
-    key_tiles_kernel(PositionArgs a, int *pos32, int *doc32, float *rel, TileStats *stats) {
-  __shared__ int edge[4][4];
+    key_tiles_kernel(PositionArgs a, int *pos32, int *doc32, float *rel, TileStats *stats,
+                     int *run) {
+  __shared__ int edge[4][4], first;
   const int tile = blockIdx.x, i = tile * kTileN + threadIdx.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int kLow = -2147483647 - 1, kHigh = 2147483647;
@@ -25,7 +26,10 @@ __global__ void __launch_bounds__(kTileN)
   int d_lo = __reduce_min_sync(0xffffffffu, in ? d : kHigh);
   int d_hi = __reduce_max_sync(0xffffffffu, in ? d : kLow);
   if (lane == 0) edge[0][warp] = lo, edge[1][warp] = hi, edge[2][warp] = d_lo, edge[3][warp] = d_hi;
+  if (threadIdx.x == 0) first = p;
   __syncthreads();
+  const bool one_apart =
+      __syncthreads_and(!in || static_cast<long long>(p) == static_cast<long long>(first) + threadIdx.x);
   lo = min(min(edge[0][0], edge[0][1]), min(edge[0][2], edge[0][3]));
   pos32[i] = p;
   doc32[i] = d;
@@ -35,6 +39,7 @@ __global__ void __launch_bounds__(kTileN)
     d_lo = min(min(edge[2][0], edge[2][1]), min(edge[2][2], edge[2][3]));
     d_hi = max(max(edge[3][0], edge[3][1]), max(edge[3][2], edge[3][3]));
     stats[tile] = {lo, hi, d_lo, d_hi};
+    run[tile] = one_apart;
   }
 }
 
@@ -70,11 +75,12 @@ cudaError_t launch(const PositionArgs &a, void *workspace, cudaStream_t stream) 
   int *pos32 = reinterpret_cast<int *>(w);
   int *doc32 = pos32 + p.keys;
   float *rel = reinterpret_cast<float *>(doc32 + p.keys);
-  w = reinterpret_cast<char *>(rel + p.keys);
+  int *run = reinterpret_cast<int *>(rel + p.keys);
+  w = reinterpret_cast<char *>(run + (p.tiles + 3) / 4 * 4);
   TcArgs t = {};
   t.part_o = reinterpret_cast<float *>(w);
   t.part_lse = t.part_o + p.slices * rows * D;
-  key_tiles_kernel<<<p.tiles, kTileN, 0, stream>>>(a, pos32, doc32, rel, stats);
+  key_tiles_kernel<<<p.tiles, kTileN, 0, stream>>>(a, pos32, doc32, rel, stats, run);
   t.q = a.q, t.out = a.out, t.lse = a.lse, t.slopes = a.slopes;
   t.q_batch = 0, t.q_token = a.q_token, t.q_head = a.q_head;
   t.tokens = t.q_len = a.q_tokens;
@@ -83,6 +89,7 @@ cudaError_t launch(const PositionArgs &a, void *workspace, cudaStream_t stream) 
   set_scores(t, a.scale, a.softcap);
   t.pos = a;
   t.k_pos32 = pos32, t.k_doc32 = a.k_doc ? doc32 : nullptr, t.k_rel = rel, t.stats = stats;
+  t.k_run = run;
   CUtensorMap k_map, v_map;
   const long long dims[3] = {D, a.kv_heads, a.k_tokens};
   const long long ks[2] = {a.k_head, a.k_token}, vs[2] = {a.v_head, a.v_token};
@@ -103,7 +110,7 @@ cudaError_t launch(const PositionArgs &a, void *workspace, cudaStream_t stream) 
 
 long long position_attention_workspace(const PositionArgs &a, int dim) {
   const Plan p = plan_of(a);
-  return p.tiles * static_cast<long long>(sizeof(TileStats)) + p.keys * 12 +
+  return p.tiles * static_cast<long long>(sizeof(TileStats)) + p.keys * 12 + (p.tiles + 3) / 4 * 16 +
          p.slices * static_cast<long long>(a.q_tokens) * a.heads * (dim + 1) * 4;
 }
 

@@ -50,12 +50,15 @@ struct TcArgs {
   long long q_batch, q_token, q_head;
   int tokens, q_len, heads, group;
   int k_tiles, tiles_per_slice, slices;
-  // x = s scale_log2, or cap_out tanh(s cap_u) with cap_in = 2 cap_u log2 e
-  float scale_log2, cap_u, cap_in, cap_out;
+  // x = s scale_log2, or cap_out tanh(s cap_u) with cap_in = 2 cap_u log2 e; for
+  // |s| up to cap_small x = s P(s^2)
+  float scale_log2, cap_in, cap_out, cap_small;
+  float2 cap_poly[5];
   // dense keys (prepared arrays, padded to whole tiles)
   PositionArgs pos;
   const int *k_pos32, *k_doc32;
   const float *k_rel;  // position minus the tile's smallest, for the distance bias
+  const int *k_run;    // the tile's positions go up by one
   const TileStats *stats;
   // paged prefix
   const int *pages, *own_lens;
@@ -76,13 +79,6 @@ struct TcSmem {
   static constexpr int kRowAt = kQAt + 2048;  // and its result, -1 behind the last row
   static constexpr int kBytes = kRowAt + 1024 + 1024;  // + alignment to the swizzle's 1 KB
 };
-
-// A load whose value nobody waits for.
-__device__ __forceinline__ void touch(const void *p) {
-  uint32_t v;
-  asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p));
-  static_cast<void>(v);
-}
 
 // True in all threads of a row tile if it is in any of them.
 __device__ __forceinline__ bool tile_any(int tile, bool v) {
@@ -111,6 +107,8 @@ __device__ __forceinline__ RowRef row_ref(const TcArgs &a, int kv_head, unsigned
   return r;
 }
 
+constexpr int kSeesNothing = -2147483647 - 1;
+
 // What a dense row may see: key positions below `limit` in document `doc`.
 struct RowMask {
   int limit, doc, pos;
@@ -121,13 +119,49 @@ __device__ __forceinline__ int clamp_pos(long long p) {
 }
 
 __device__ __forceinline__ RowMask row_mask(const PositionArgs &p, int token) {
+  const long long at = position_at(p.q_pos, p.long_q_pos, token);
+  const int prefix = p.q_prefix ? p.q_prefix[token] : 0;
+  const int doc = p.q_doc ? p.q_doc[token] : 0;
   RowMask m;
-  m.pos = clamp_pos(position_at(p.q_pos, p.long_q_pos, token));
+  m.pos = clamp_pos(at);
   m.limit = p.causal ? m.pos + 1 : 2147483647;
-  if (p.q_prefix) m.limit = max(m.limit, p.q_prefix[token]);
-  m.doc = p.q_doc ? p.q_doc[token] : 0;
-  if (m.doc < 0) m.limit = -2147483647 - 1;  // a padding row sees nothing
+  if (p.q_prefix) m.limit = max(m.limit, prefix);
+  m.doc = doc;
+  if (m.doc < 0) m.limit = kSeesNothing;  // a padding row
   return m;
+}
+
+// Which of 64 keys each row of the warp sees, as bits: lane i holds positions and
+// documents of keys i and 32 + i.  Rows of one document (mostly all 32) share
+// the keys below their least limit and above their greatest; only keys between
+// are compared row by row.
+__device__ __forceinline__ void visible_keys(const RowMask &row, int kp0, int kp1, int kd0, int kd1,
+                                             bool docs, uint32_t &vis0, uint32_t &vis1) {
+  constexpr uint32_t kAll = 0xffffffffu;
+  vis0 = vis1 = 0;
+  uint32_t todo = __ballot_sync(kAll, row.limit != kSeesNothing);
+  while (todo) {
+    const int doc = __shfl_sync(kAll, row.doc, __ffs(todo) - 1);
+    const bool mine = row.limit != kSeesNothing && row.doc == doc;
+    todo &= ~__ballot_sync(kAll, mine);
+    const int lo = __reduce_min_sync(kAll, mine ? row.limit : 2147483647);
+    const int hi = __reduce_max_sync(kAll, mine ? row.limit : kSeesNothing);
+    const bool in0 = !docs || kd0 == doc, in1 = !docs || kd1 == doc;
+    uint32_t v0 = __ballot_sync(kAll, in0 && kp0 < lo), v1 = __ballot_sync(kAll, in1 && kp1 < lo);
+    uint32_t s0 = __ballot_sync(kAll, in0 && kp0 >= lo && kp0 < hi);
+    uint32_t s1 = __ballot_sync(kAll, in1 && kp1 >= lo && kp1 < hi);
+    while (s0) {
+      const int b = __ffs(s0) - 1;
+      s0 &= s0 - 1;
+      v0 |= static_cast<uint32_t>(__shfl_sync(kAll, kp0, b) < row.limit) << b;
+    }
+    while (s1) {
+      const int b = __ffs(s1) - 1;
+      s1 &= s1 - 1;
+      v1 |= static_cast<uint32_t>(__shfl_sync(kAll, kp1, b) < row.limit) << b;
+    }
+    if (mine) vis0 = v0, vis1 = v1;
+  }
 }
 
 // A row whose tensor-core result holds an infinity or NaN is computed again by
@@ -221,8 +255,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   constexpr int kHalfBytes = kTileN * 128;   // of one tile
   constexpr bool kBf16 = __is_same(T, __nv_bfloat16);
   // of 8 pairs of weights, how many the FMA pipe computes: ex2 and the mma are
-  // equally long at D = 128, ex2 is the longer at D = 64
-  constexpr int kFmaOf8 = D == 128 ? 2 : 3;
+  // equally long at D = 128, ex2 is the longer at D = 64, and a cap or a bias
+  // keeps the FMA pipe busy
+  constexpr int kFmaOf8 = kCap || kBias ? 0 : D == 128 ? 2 : 3;
   extern __shared__ uint8_t raw_smem[];
   uint8_t *smem = reinterpret_cast<uint8_t *>(
       (reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -267,7 +302,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   RowMask mask = {0, 0, 0};
   const int x = warp >> 3, half = (warp >> 2) & 1;  // row tile, and which 64 keys
   const int row_in_tile = tid & 127;
-  int lim_lo = 2147483647, lim_hi = -2147483647 - 1, doc_lo = lim_lo, doc_hi = lim_hi;
+  int lim_lo = 2147483647, lim_hi = kSeesNothing, doc_lo = lim_lo, doc_hi = lim_hi;
   long long *q_at = reinterpret_cast<long long *>(smem + L::kQAt) + x * kTileM;
   int *row_at = reinterpret_cast<int *>(smem + L::kRowAt) + x * kTileM;
   if (warp < kMmaWarp && x < tiles) {
@@ -447,11 +482,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     bool whole, ok = true;
     while (scan.next(tile, whole)) {
       const int key0 = tile * kTileN + half * kKeys;
-      // positions and documents to L1 while the scores are computed
-      if (kDense && lane < 2) {
-        if (!whole) touch(a.k_pos32 + key0 + lane * 32);
-        if (!whole && a.k_doc32) touch(a.k_doc32 + key0 + lane * 32);
-        if (kBias) touch(a.k_rel + key0 + lane * 32);
+      // masks while the scores are computed
+      uint32_t vis0 = 0xffffffffu, vis1 = 0xffffffffu;
+      if (kDense && !whole) {
+        const int kp0 = a.k_pos32[key0 + lane], kp1 = a.k_pos32[key0 + 32 + lane];
+        const bool docs = a.k_doc32 != nullptr;
+        const int kd0 = docs ? a.k_doc32[key0 + lane] : 0;
+        const int kd1 = docs ? a.k_doc32[key0 + 32 + lane] : 0;
+        visible_keys(mask, kp0, kp1, kd0, kd1, docs, vis0, vis1);
       }
       uint32_t bad = 0;  // pages of this tile that lie outside the cache
       if (!kDense) {
@@ -473,75 +511,82 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tmem_ld32(s_addr + half * kKeys + c * 32, reinterpret_cast<uint32_t(&)[32]>(s[c * 32]));
       tmem_wait_ld();
       // x = s c in log2 units, unless it is only scaled (then c goes into exp2)
-      if (kCap || kBias) {
-        if (kCap) {
-          // tanh by a polynomial while every score of the warp's rows is small
-          // against the cap, as they mostly are: on the FMA pipe it costs a
-          // quarter of the exponential and reciprocal of the general form
-          // tanh(u) = 1 - 2 / (1 + e^2u)
-          float big = 0.f;
+      if (kCap) {
+        // tanh by an odd polynomial while every score of the warp's rows is small
+        // against the cap, as they mostly are: three FMA slots a score instead of
+        // the exponential and reciprocal of tanh(u) = 1 - 2 / (1 + e^2u)
+        float big = 0.f;
 #pragma unroll
-          for (int i = 0; i < kKeys; i += 2)
-            big = fmaxf(fmaxf(big, fabsf(s[i])), fabsf(s[i + 1]));
-          if (__all_sync(0xffffffffu, big * a.cap_u <= kSmallTanh)) {
-            const f32x2 cu = pack2(a.cap_u, a.cap_u), c2 = pack2(a.scale_log2, a.scale_log2);
+        for (int i = 0; i < kKeys; i += 2)
+          big = fmaxf(fmaxf(big, fabsf(s[i])), fabsf(s[i + 1]));
+        if (__all_sync(0xffffffffu, big <= a.cap_small)) {
+          f32x2 k[5];
 #pragma unroll
-            for (int i = 0; i < kKeys; i += 2) {
-              const f32x2 x = pack2(s[i], s[i + 1]), u = mul2(x, cu);
-              unpack2(mul2(mul2(x, c2), tanh_ratio(mul2(u, u))), s[i], s[i + 1]);
-            }
-          } else {
+          for (int i = 0; i < 5; ++i) k[i] = pack2(a.cap_poly[i].x, a.cap_poly[i].y);
 #pragma unroll
-            for (int i = 0; i < kKeys; ++i) {
-              const float e = ex2(s[i] * a.cap_in);
-              s[i] = fmaf(rcp(1.f + e), -2.f * a.cap_out, a.cap_out);
-            }
+          for (int i = 0; i < kKeys; i += 2) {
+            const f32x2 v = pack2(s[i], s[i + 1]), w = mul2(v, v);
+            unpack2(mul2(v, fma2(fma2(fma2(fma2(k[4], w, k[3]), w, k[2]), w, k[1]), w, k[0])),
+                    s[i], s[i + 1]);
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < kKeys; ++i) s[i] *= a.scale_log2;
+          for (int i = 0; i < kKeys; ++i)
+            s[i] = fmaf(rcp(1.f + ex2(s[i] * a.cap_in)), -2.f * a.cap_out, a.cap_out);
         }
-        if (kBias) {
-          if (kDense) {
-            const float at = static_cast<float>(static_cast<long long>(mask.pos) -
-                                                a.stats[tile].pos_min);
-            const float4 *rel = reinterpret_cast<const float4 *>(a.k_rel + key0);
+      } else if (kBias) {
 #pragma unroll
-            for (int i = 0; i < kKeys / 4; ++i) {
-              const float4 p = rel[i];
-              s[4 * i] = fmaf(-slope, fabsf(at - p.x), s[4 * i]);
-              s[4 * i + 1] = fmaf(-slope, fabsf(at - p.y), s[4 * i + 1]);
-              s[4 * i + 2] = fmaf(-slope, fabsf(at - p.z), s[4 * i + 2]);
-              s[4 * i + 3] = fmaf(-slope, fabsf(at - p.w), s[4 * i + 3]);
-            }
-          } else {
-            const float at = q_place - static_cast<float>(key0);
+        for (int i = 0; i < kKeys; ++i) s[i] *= a.scale_log2;
+      }
+      float lift = 0.f;  // what all scores of this row and tile still lack
+      if (kBias) {
+        // -slope |p - p_j|; for keys one apart at or before the row, slope j plus
+        // a constant (what else is in the tile is masked)
+        bool run = true;
+        float at;  // the row's place counted from this thread's first key
+        if (kDense) {
+          run = a.k_run[tile] != 0;
+          at = static_cast<float>(static_cast<long long>(mask.pos) - a.stats[tile].pos_min) -
+               (run ? static_cast<float>(half * kKeys) : 0.f);
+        } else {
+          at = q_place - static_cast<float>(key0);
+        }
+        const bool before = kDense ? mask.limit <= mask.pos + 1 || at >= kKeys : at >= kKeys - 1;
+        if (run && __all_sync(0xffffffffu, before || !ref.valid)) {
+          lift = -slope * at;
+          const f32x2 sl = pack2(slope, slope), two = pack2(2.f, 2.f);
+          f32x2 n = pack2(0.f, 1.f);
 #pragma unroll
-            for (int i = 0; i < kKeys; ++i)
-              s[i] = fmaf(-slope, fabsf(at - static_cast<float>(i)), s[i]);
+          for (int i = 0; i < kKeys; i += 2) {
+            unpack2(fma2(sl, n, pack2(s[i], s[i + 1])), s[i], s[i + 1]);
+            n = add2(n, two);
+          }
+        } else if (run) {
+#pragma unroll
+          for (int i = 0; i < kKeys; ++i)
+            s[i] = fmaf(-slope, fabsf(at - static_cast<float>(i)), s[i]);
+        } else {
+          const float4 *rel = reinterpret_cast<const float4 *>(a.k_rel + key0);
+#pragma unroll
+          for (int i = 0; i < kKeys / 4; ++i) {
+            const float4 p = rel[i];
+            s[4 * i] = fmaf(-slope, fabsf(at - p.x), s[4 * i]);
+            s[4 * i + 1] = fmaf(-slope, fabsf(at - p.y), s[4 * i + 1]);
+            s[4 * i + 2] = fmaf(-slope, fabsf(at - p.z), s[4 * i + 2]);
+            s[4 * i + 3] = fmaf(-slope, fabsf(at - p.w), s[4 * i + 3]);
           }
         }
       }
       if (kDense && !whole) {
-        const int4 *kp = reinterpret_cast<const int4 *>(a.k_pos32 + key0);
+        if (__any_sync(0xffffffffu, vis0 != 0xffffffffu)) {
 #pragma unroll
-        for (int i = 0; i < kKeys / 4; ++i) {
-          const int4 p = kp[i];
-          if (p.x >= mask.limit) s[4 * i] = -INFINITY;
-          if (p.y >= mask.limit) s[4 * i + 1] = -INFINITY;
-          if (p.z >= mask.limit) s[4 * i + 2] = -INFINITY;
-          if (p.w >= mask.limit) s[4 * i + 3] = -INFINITY;
+          for (int i = 0; i < 32; ++i)
+            if (!((vis0 >> i) & 1)) s[i] = -INFINITY;
         }
-        if (a.k_doc32) {
-          const int4 *kd = reinterpret_cast<const int4 *>(a.k_doc32 + key0);
+        if (__any_sync(0xffffffffu, vis1 != 0xffffffffu)) {
 #pragma unroll
-          for (int i = 0; i < kKeys / 4; ++i) {
-            const int4 p = kd[i];
-            if (p.x != mask.doc) s[4 * i] = -INFINITY;
-            if (p.y != mask.doc) s[4 * i + 1] = -INFINITY;
-            if (p.z != mask.doc) s[4 * i + 2] = -INFINITY;
-            if (p.w != mask.doc) s[4 * i + 3] = -INFINITY;
-          }
+          for (int i = 0; i < 32; ++i)
+            if (!((vis1 >> i) & 1)) s[32 + i] = -INFINITY;
         }
       }
       if (!kDense && bad) {
@@ -561,7 +606,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       t0 = fmaxf(fmaxf(t0, s[kKeys - 4]), s[kKeys - 3]);
       t1 = fmaxf(fmaxf(t1, s[kKeys - 2]), s[kKeys - 1]);
-      const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * c;
+      const float top = fmaf(fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)), c, lift);
       // O is rescaled when a row's maximum has grown (also at its first finite
       // score), by both of its threads alike
       if (tile_any(x, top > m + kLazy || !ok)) {
@@ -588,7 +633,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
         }
       }
-      const float off = m == -INFINITY ? 0.f : m;
+      const float off = (m == -INFINITY ? 0.f : m) - lift;
       const f32x2 c2 = pack2(c, c), off2 = pack2(-off, -off);
       f32x2 l0 = pack2(0.f, 0.f), l1 = l0;
       // the weights, some of them by the polynomial

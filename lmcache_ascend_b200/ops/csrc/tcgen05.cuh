@@ -235,16 +235,4 @@ __device__ __forceinline__ void exp2_fma(f32x2 x, float &a, float &b) {
   b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23));
 }
 
-// tanh(u) / u as a polynomial in u^2 for |u| <= 3/4 (relative minimax by the
-// Remez exchange, degree 5: 2.9e-8).
-constexpr float kSmallTanh = 0.75f;
-__device__ __forceinline__ f32x2 tanh_ratio(f32x2 u2) {
-  f32x2 p = pack2(-0.004716257099062204f, -0.004716257099062204f);
-  p = fma2(p, u2, pack2(0.01958290860056877f, 0.01958290860056877f));
-  p = fma2(p, u2, pack2(-0.05334442853927612f, -0.05334442853927612f));
-  p = fma2(p, u2, pack2(0.1332540661096573f, 0.1332540661096573f));
-  p = fma2(p, u2, pack2(-0.33332958817481995f, -0.33332958817481995f));
-  return fma2(p, u2, pack2(1.f, 1.f));
-}
-
 }  // namespace lmc
