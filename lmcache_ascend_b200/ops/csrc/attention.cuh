@@ -60,6 +60,14 @@ template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
+// --- overlapped launches of one call (see launch_ordered)
+__device__ __forceinline__ void let_next_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void wait_for_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // One query row on one warp; lane l holds elements [l D/32, (l + 1) D/32).
 template <typename T, int D>
 struct WarpRow {

@@ -3,6 +3,10 @@
 // with o_s normalised in its slice and L_s the base-2 log of its sum.  One warp
 // per row, fp32.
 #pragma once
+#include <mutex>
+#include <set>
+#include <utility>
+
 #include "tc_attention.cuh"
 
 namespace lmc {
@@ -63,6 +67,7 @@ __global__ void __launch_bounds__(128)
     join_position_kernel(PositionArgs a, const float *part_o, const float *part_lse, int slices) {
   const long long rows = static_cast<long long>(a.q_tokens) * a.heads;
   const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  wait_for_previous();
   if (row >= rows) return;
   JoinedRow<T, D> r;
   r.join(part_o, part_lse, slices, rows, row);
@@ -89,19 +94,56 @@ inline void set_scores(TcArgs &t, float scale, float softcap) {
   t.cap_small = u >= 1e-4 ? static_cast<float>(0.6 / u) : -1.f;
 }
 
+// Lets a kernel use `bytes` of shared memory on the current device; asked of the
+// runtime once per device (the call costs as much as a launch).
+template <typename Kernel>
+cudaError_t allow_smem(Kernel kernel, int bytes) {
+  static std::mutex lock;
+  static std::set<std::pair<const void *, int>> done;
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const std::lock_guard<std::mutex> hold(lock);
+  const auto key = std::make_pair(reinterpret_cast<const void *>(kernel), device);
+  if (done.count(key)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.insert(key);
+  return e;
+}
+
+// Launches one of a call's kernels.  The first waits for all that was in the
+// stream before it; the blocks of a later one may start while the kernel before
+// it ends (it hides the launch and fills the SMs that are done).  Every kernel
+// calls wait_for_previous() before it reads what an earlier one of the call
+// wrote, and in any case before its blocks end, so that they complete in order.
+template <typename... Params, typename... Args>
+cudaError_t launch_ordered(void (*kernel)(Params...), dim3 grid, unsigned threads, int smem,
+                           bool first, cudaStream_t stream, const Args &...args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = static_cast<size_t>(smem);
+  config.stream = stream;
+  cudaLaunchAttribute attribute = {};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attribute;
+  config.numAttrs = first ? 0 : 1;
+  return cudaLaunchKernelEx(&config, kernel, Params(args)...);
+}
+
 template <typename T, int D, bool kDense>
 cudaError_t launch_tc(const CUtensorMap &k_map, const CUtensorMap &v_map, const TcArgs &t,
-                      unsigned grid, cudaStream_t stream) {
+                      unsigned grid, bool first, cudaStream_t stream) {
   const bool cap = t.cap_out > 0.f, bias = t.slopes != nullptr;
   auto kernel = cap ? (bias ? tc_attention_kernel<T, D, kDense, true, true>
                             : tc_attention_kernel<T, D, kDense, true, false>)
                     : (bias ? tc_attention_kernel<T, D, kDense, false, true>
                             : tc_attention_kernel<T, D, kDense, false, false>);
   constexpr int kBytes = TcSmem<D>::kBytes;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+  cudaError_t e = allow_smem(kernel, kBytes);
   if (e != cudaSuccess) return e;
-  kernel<<<grid, kTcThreads, kBytes, stream>>>(k_map, v_map, t);
-  return cudaGetLastError();
+  return launch_ordered(kernel, dim3(grid), kTcThreads, kBytes, first, stream, k_map, v_map, t);
 }
 
 }  // namespace lmc

@@ -3,8 +3,7 @@
 // kernel, and a join when the keys are split.
 #include <algorithm>
 
-#include "attention_join.cuh"
-#include "tc_attention.cuh"
+#include "split_attention.cuh"
 #include "tensor_maps.h"
 
 namespace lmc {
@@ -16,6 +15,7 @@ __global__ void __launch_bounds__(kTileN)
     key_tiles_kernel(PositionArgs a, int *pos32, int *doc32, float *rel, TileStats *stats,
                      int *run) {
   __shared__ int edge[4][4], first;
+  let_next_start();
   const int tile = blockIdx.x, i = tile * kTileN + threadIdx.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int kLow = -2147483647 - 1, kHigh = 2147483647;
@@ -44,19 +44,35 @@ __global__ void __launch_bounds__(kTileN)
 }
 
 struct Plan {
+  bool split;  // the kernel for few rows or keys; else the tensor-core kernel
+  int row_tiles;
   int tiles, per_slice, slices, groups;  // slices == 0: not split
   long long keys;                        // padded
 };
+
+// Blocks of 16 rows times steps of 64 keys up to which the split kernel is taken.
+// Measured (B200, 32/8 heads of 128, split / tensor cores, us): 38 rows on 257 keys
+// (400 steps) 11.2 / 14.8, 128 on 512 (2048) 16.1 / 16.5, 1 on 16384 (2048)
+// 20.2 / 24.7, 8 on 16384 (4096) 30.7 / 26.0, 256 on 512 (4096) 29.0 / 16.5.
+constexpr long long kSplitSteps = 2048;
 
 // The keys are split when the blocks would not fill the GPU: towards one block
 // per SM, with at least four tiles each (below that the join costs more than
 // the shorter stream saves).
 Plan plan_of(const PositionArgs &a) {
-  Plan p;
+  Plan p = {};
   p.tiles = (a.k_tokens + kTileN - 1) / kTileN;
   p.keys = static_cast<long long>(p.tiles) * kTileN;
   const long long rows = static_cast<long long>(a.q_tokens) * (a.heads / a.kv_heads);
   p.groups = static_cast<int>((rows + kBlockRows - 1) / kBlockRows);
+  p.row_tiles = static_cast<int>((rows + kSplitRows - 1) / kSplitRows);
+  const long long steps = static_cast<long long>(p.row_tiles) * a.kv_heads *
+                          ((a.k_tokens + kSplitWarps * kSplitKeys - 1) / (kSplitWarps * kSplitKeys));
+  if (steps <= kSplitSteps) {
+    p.split = true;
+    p.slices = split_slices(static_cast<long long>(p.row_tiles) * a.kv_heads, a.k_tokens);
+    return p;
+  }
   const long long blocks = static_cast<long long>(p.groups) * a.kv_heads;
   const long long want = std::min(148 / std::max(1ll, blocks), p.tiles / 4ll);
   p.slices = want >= 2 ? static_cast<int>(want) : 0;
@@ -69,6 +85,15 @@ template <typename T, int D>
 cudaError_t launch(const PositionArgs &a, void *workspace, cudaStream_t stream) {
   const Plan p = plan_of(a);
   const long long rows = static_cast<long long>(a.q_tokens) * a.heads;
+  if (p.split) {
+    float *part_o = p.slices > 1 ? static_cast<float *>(workspace) : nullptr;
+    float *part_lse = part_o + p.slices * rows * D;
+    const SplitPass s = {0, 0, false, a.q_tokens, p.row_tiles, p.slices, part_o, part_lse};
+    cudaError_t e = launch_split<T, D>(a, s, 1, true, stream);
+    if (e != cudaSuccess || p.slices == 1) return e;
+    return launch_ordered(join_position_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)),
+                          128, 0, false, stream, a, part_o, part_lse, p.slices);
+  }
   char *w = static_cast<char *>(workspace);
   TileStats *stats = reinterpret_cast<TileStats *>(w);
   w += p.tiles * sizeof(TileStats);
@@ -99,17 +124,18 @@ cudaError_t launch(const PositionArgs &a, void *workspace, cudaStream_t stream) 
       !encode_rows(&v_map, kBf16, a.v, 3, dims, vs, box))
     return cudaErrorInvalidValue;
   const unsigned grid = static_cast<unsigned>(p.groups) * a.kv_heads * std::max(1, p.slices);
-  cudaError_t e = launch_tc<T, D, true>(k_map, v_map, t, grid, stream);
+  cudaError_t e = launch_tc<T, D, true>(k_map, v_map, t, grid, false, stream);
   if (e != cudaSuccess || !p.slices) return e;
-  join_position_kernel<T, D><<<static_cast<unsigned>((rows + 3) / 4), 128, 0, stream>>>(
-      a, t.part_o, t.part_lse, p.slices);
-  return cudaGetLastError();
+  return launch_ordered(join_position_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128,
+                        0, false, stream, a, t.part_o, t.part_lse, p.slices);
 }
 
 }  // namespace
 
 long long position_attention_workspace(const PositionArgs &a, int dim) {
   const Plan p = plan_of(a);
+  if (p.split)
+    return p.slices == 1 ? 0 : p.slices * static_cast<long long>(a.q_tokens) * a.heads * (dim + 1) * 4;
   return p.tiles * static_cast<long long>(sizeof(TileStats)) + p.keys * 12 + (p.tiles + 3) / 4 * 16 +
          p.slices * static_cast<long long>(a.q_tokens) * a.heads * (dim + 1) * 4;
 }

@@ -4,7 +4,7 @@
 // a join of the parts.
 #include <algorithm>
 
-#include "paged_split.cuh"
+#include "split_attention.cuh"
 #include "tensor_maps.h"
 
 namespace lmc {
@@ -16,11 +16,12 @@ struct PrefixPlan {
   int own_begin, own_slices, own_tiles;     // split pass per request, from this prefix key on
 };
 
-int split_slices(long long blocks, long long keys) {
-  // towards four blocks per SM (two are resident), with 256 keys or more each
-  const long long want = std::min(148 * 4 / std::max(1ll, blocks), (keys + 255) / 256);
-  return static_cast<int>(std::max(1ll, std::min(want, 64ll)));
-}
+// Blocks of 16 rows times steps of 64 keys up to which the split pass reads the
+// prefix.  Measured (B200, 32/8 heads of 128, split / tensor cores, us): 250 steps
+// 11.8 / 15.9, 1024 steps 17.5 / 20.3 and 22.2 / 24.8, 2000 steps 20.1 / 25.0
+// (one request), 4096 steps 36.1 / 26.4.
+constexpr long long kSplitSteps = 2000;
+constexpr long long kFewSteps = 600;
 
 PrefixPlan plan_of(const PagedArgs &a) {
   PrefixPlan p = {};
@@ -30,18 +31,23 @@ PrefixPlan plan_of(const PagedArgs &a) {
   // whole pages or whole 128-slot parts of them must make up a tile, in 8-row
   // groups of the swizzle
   const bool boxes = bs % 8 == 0 && (kTileN % bs == 0 || bs % kTileN == 0);
-  if (boxes && prefix >= kTileN) {
+  const long long row_tiles = (tokens * group + kSplitRows - 1) / kSplitRows;
+  const long long prefix_steps = (prefix + kSplitWarps * kSplitKeys - 1) / (kSplitWarps * kSplitKeys);
+  const long long request_tiles = (a.q_len * group + kSplitRows - 1) / kSplitRows;
+  if (a.batch * request_tiles * a.kv_heads * prefix_steps <= kFewSteps) {
+    // short enough for every request to read the prefix with its own keys (one
+    // pass): 4 requests on 500 tokens, 8 KV heads: 9.6 us in two passes
+  } else if (boxes && prefix >= kTileN && row_tiles * a.kv_heads * prefix_steps > kSplitSteps) {
     p.tiles = prefix / kTileN;
     p.groups = static_cast<int>((tokens * group + kBlockRows - 1) / kBlockRows);
     const long long blocks = static_cast<long long>(p.groups) * a.kv_heads;
-    const long long want =
-        std::max(1ll, std::min({148 / blocks, p.tiles / 2ll, 64ll}));
+    const long long want = std::max(1ll, std::min({148 / blocks, p.tiles / 2ll, 64ll}));
     p.per_slice = static_cast<int>((p.tiles + want - 1) / want);
     p.tc_slices = (p.tiles + p.per_slice - 1) / p.per_slice;
     p.own_begin = p.tiles * kTileN;
-  } else if (a.batch > 1 && prefix >= kTileN) {
-    p.pre_tiles = static_cast<int>((tokens * group + kSplitRows - 1) / kSplitRows);
-    p.pre_slices = split_slices(static_cast<long long>(p.pre_tiles) * a.kv_heads, prefix);
+  } else if (a.batch > 1) {
+    p.pre_tiles = static_cast<int>(row_tiles);
+    p.pre_slices = split_slices(row_tiles * a.kv_heads, prefix);
     p.own_begin = prefix;
   }
   p.own_tiles = (a.q_len * group + kSplitRows - 1) / kSplitRows;
@@ -49,18 +55,6 @@ PrefixPlan plan_of(const PagedArgs &a) {
       split_slices(static_cast<long long>(a.batch) * p.own_tiles * a.kv_heads,
                    prefix - p.own_begin + static_cast<long long>(a.width) * a.block_size);
   return p;
-}
-
-template <typename T, int D>
-cudaError_t split_pass(const PagedArgs &a, const SplitPass &s, long long units,
-                       cudaStream_t stream) {
-  constexpr int kBytes = SplitSmem<D>::kBytes;
-  cudaError_t e = cudaFuncSetAttribute(paged_split_kernel<T, D>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-  if (e != cudaSuccess) return e;
-  const dim3 grid(static_cast<unsigned>(units * s.row_tiles * a.kv_heads), s.slices);
-  paged_split_kernel<T, D><<<grid, kSplitWarps * 32, kBytes, stream>>>(a, s);
-  return cudaGetLastError();
 }
 
 template <typename T, int D>
@@ -93,32 +87,33 @@ cudaError_t launch(const PagedArgs &a, void *workspace, cudaStream_t stream) {
         !encode_rows(&v_map, kBf16, a.v, 4, dims, vs, box))
       return cudaErrorInvalidValue;
     const unsigned grid = static_cast<unsigned>(p.groups) * a.kv_heads * p.tc_slices;
-    e = launch_tc<T, D, false>(k_map, v_map, t, grid, stream);
+    e = launch_tc<T, D, false>(k_map, v_map, t, grid, true, stream);
     if (e != cudaSuccess) return e;
   }
   int first = p.tc_slices;
   if (p.pre_slices) {
     const SplitPass s = {0, static_cast<int>(a.prefix_len), false, a.batch * a.q_len, p.pre_tiles,
                          p.pre_slices, part_o + first * rows * D, part_lse + first * rows};
-    e = split_pass<T, D>(a, s, 1, stream);
+    e = launch_split<T, D>(a, s, 1, true, stream);
     if (e != cudaSuccess) return e;
     first += p.pre_slices;
   }
   const SplitPass s = {p.own_begin, static_cast<int>(a.prefix_len), true, a.q_len, p.own_tiles,
-                       p.own_slices, part_o + first * rows * D, part_lse + first * rows};
-  e = split_pass<T, D>(a, s, a.batch, stream);
-  if (e != cudaSuccess) return e;
-  join_paged_kernel<T, D><<<static_cast<unsigned>((rows + 3) / 4), 128, 0, stream>>>(
-      a, part_o, part_lse, slices);
-  return cudaGetLastError();
+                       p.own_slices, slices > 1 ? part_o + first * rows * D : nullptr,
+                       part_lse + first * rows};
+  e = launch_split<T, D>(a, s, a.batch, first == 0, stream);
+  if (e != cudaSuccess || slices == 1) return e;
+  return launch_ordered(join_paged_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0,
+                        false, stream, a, part_o, part_lse, slices);
 }
 
 }  // namespace
 
 long long shared_prefix_attention_workspace(const PagedArgs &a, int dim) {
   const PrefixPlan p = plan_of(a);
-  return static_cast<long long>(p.tc_slices + p.pre_slices + p.own_slices) * a.batch * a.q_len *
-         a.heads * (dim + 1) * 4;
+  const int slices = p.tc_slices + p.pre_slices + p.own_slices;
+  return slices == 1 ? 0
+                     : static_cast<long long>(slices) * a.batch * a.q_len * a.heads * (dim + 1) * 4;
 }
 
 cudaError_t launch_shared_prefix_attention(const PagedArgs &a, RowType type, int dim,

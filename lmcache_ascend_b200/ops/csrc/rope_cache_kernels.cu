@@ -9,11 +9,13 @@
 // with its gain, is used as it is).
 //
 // Bound by HBM: each row is read once and written once, so K and V go straight
-// to their slots instead of through a second pass.  A thread moves a unit of two
-// 16-byte vectors that holds both halves of its pairs (in the half layout the
+// to their slots instead of through a second pass.  A thread moves units of two
+// 16-byte vectors that hold both halves of its pairs (in the half layout the
 // vectors at i and i + rot/2, otherwise two adjacent ones); a head of D elements
-// has D / (2 * VE) units whatever the layout, so one flat index covers q, k and
-// v, and blocks get equal work for one row or many.
+// has D / (2 * VE) units whatever the layout.  A thread keeps its place in the
+// head and walks over the heads of q, k and v of one row after the other, so that
+// a unit costs no division and a row's cosines and sines are loaded once for
+// several heads; blocks get equal work for one row or many.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -26,7 +28,7 @@ namespace lmc {
 namespace {
 
 constexpr int kRopeThreads = 256;
-constexpr int kUnitsPerThread = 4;  // 8 vector loads in flight per thread
+constexpr int kHeadsPerThread = 8, kAtOnce = 2;  // four vector loads in flight a thread
 
 __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -94,90 +96,140 @@ __device__ __forceinline__ void load_table(const CT *p, float *f) {
   constexpr int V = 16 / sizeof(CT) < N ? 16 / sizeof(CT) : N;
 #pragma unroll
   for (int i = 0; i < N; i += V) {
-    const uint4 w = *reinterpret_cast<const uint4 *>(p + i);
+    const uint4 w = __ldg(reinterpret_cast<const uint4 *>(p + i));  // the table is not written
     const CT *e = reinterpret_cast<const CT *>(&w);
 #pragma unroll
     for (int j = 0; j < V; ++j) f[i + j] = as_float(e[j]);
   }
 }
 
-// 16-byte units.  Needs dim % (2 VE) == 0 and rot % (2 VE) == 0 and aligned rows.
+// 16-byte units.  Needs dim % (2 VE) == 0 and rot % (2 VE) == 0, aligned rows and
+// at most kRopeThreads units per head.  `heads` counts those of q, k and v; a
+// block takes `per_block` of them in a row, up to kHeadsPerThread a thread.  Its rows are looked up first (position, page), so that its data
+// and table loads wait for nothing but their own memory.
 template <typename T, typename CT>
-__global__ void __launch_bounds__(kRopeThreads) rope_cache_vec_kernel(RopeArgs a) {
+__global__ void __launch_bounds__(kRopeThreads) rope_cache_vec_kernel(RopeArgs a, int heads,
+                                                                      int per_block) {
   constexpr int VE = 16 / sizeof(T);
+  struct Row {
+    long long pos, k_at, v_at;  // position, offsets of the slot's first head; -1: none
+  };
+  extern __shared__ __align__(16) unsigned char rope_smem[];
+  Row *rows = reinterpret_cast<Row *>(rope_smem);
   const int per_head = a.dim / (2 * VE);
-  const int rot_units = a.rot / (2 * VE);
-  const int per_row = per_head * (a.heads + (a.k ? a.kv_heads : 0) + (a.v ? a.kv_heads : 0));
-  const long long total = a.num_tokens * per_row;
-  const long long first = static_cast<long long>(blockIdx.x) * (kRopeThreads * kUnitsPerThread);
-  const long long t_first = first / per_row;
-  const int rem = static_cast<int>(first - t_first * per_row);
-  uint4 x[kUnitsPerThread], y[kUnitsPerThread];
-  HeadRef<T> ref[kUnitsPerThread];
-  long long pos[kUnitsPerThread];
-  int at1[kUnitsPerThread], at2[kUnitsPerThread], unit[kUnitsPerThread];
-#pragma unroll
-  for (int i = 0; i < kUnitsPerThread; ++i) {
-    const int local = i * kRopeThreads + static_cast<int>(threadIdx.x);
-    ref[i].src = nullptr;
-    if (first + local >= total) continue;
-    const unsigned u = static_cast<unsigned>(rem + local);
-    const unsigned dt = u / static_cast<unsigned>(per_row);
-    const unsigned v = u - dt * per_row;
-    const int h = static_cast<int>(v / static_cast<unsigned>(per_head));
-    const int j = static_cast<int>(v) - h * per_head;
-    const long long t = t_first + dt;
-    ref[i] = head_ref<T>(a, t, h);
-    pos[i] = int_at(a.positions, a.long_pos, t);
-    unit[i] = j;
-    if (a.neox && j < rot_units)
-      at1[i] = j * VE, at2[i] = j * VE + a.rot / 2;
-    else
-      at1[i] = j * 2 * VE, at2[i] = at1[i] + VE;
-    x[i] = *reinterpret_cast<const uint4 *>(ref[i].src + at1[i]);
-    y[i] = *reinterpret_cast<const uint4 *>(ref[i].src + at2[i]);
-    if (pos[i] < 0 || pos[i] >= a.max_pos) {
+  const int lanes = kRopeThreads / per_head;
+  const long long total = a.num_tokens * heads;
+  const long long first = static_cast<long long>(blockIdx.x) * per_block;
+  const long long t_first = first / heads;
+  const int rem = static_cast<int>(first - t_first * heads);
+  const int count = static_cast<int>(min(total - first, static_cast<long long>(per_block)));
+  const int n_rows = (rem + count - 1) / heads + 1;
+  for (int i = threadIdx.x; i < n_rows; i += kRopeThreads) {
+    const long long t = t_first + i;
+    Row r = {int_at(a.positions, a.long_pos, t), -1, -1};
+    if (r.pos < 0 || r.pos >= a.max_pos) {
       // no angle: nothing reaches the pages, the row's outputs are zero
-      report_status(a.status, kStatusBadIndex, 0, t, pos[i]);
-      x[i] = y[i] = make_uint4(0, 0, 0, 0);
-      ref[i].dst2 = nullptr;
-      ref[i].rotate = false;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < kUnitsPerThread; ++i) {
-    if (ref[i].src == nullptr) continue;
-    if (ref[i].rotate && unit[i] < rot_units) {
-      const CT *row = static_cast<const CT *>(a.table) + pos[i] * a.rot + unit[i] * VE;
-      float c[VE], s[VE];
-      load_table<CT, VE>(row, c);
-      load_table<CT, VE>(row + a.rot / 2, s);
-      T *p = reinterpret_cast<T *>(&x[i]), *r = reinterpret_cast<T *>(&y[i]);
-      if (a.neox) {
-#pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          const float f = as_float(p[e]), g = as_float(r[e]);
-          p[e] = round_to<T>(f * c[e] - g * s[e]);
-          r[e] = round_to<T>(g * c[e] + f * s[e]);
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          T *w = e < VE / 2 ? p + 2 * e : r + 2 * e - VE;
-          const float f = as_float(w[0]), g = as_float(w[1]);
-          w[0] = round_to<T>(f * c[e] - g * s[e]);
-          w[1] = round_to<T>(g * c[e] + f * s[e]);
-        }
+      report_status(a.status, kStatusBadIndex, 0, t, r.pos);
+      r.pos = -1;
+    } else if (a.slots) {
+      const long long slot = int_at(a.slots, a.long_slots, t);
+      if (slot >= 0 && slot < a.num_slots) {
+        const long long page = slot / a.block_size, off = slot - page * a.block_size;
+        r.k_at = page * a.k_block + off * a.k_slot;
+        r.v_at = page * a.v_block + off * a.v_slot;
+      } else if (slot >= a.num_slots) {
+        report_status(a.status, kStatusBadSlot, 0, t, slot);
       }
     }
-    if (ref[i].dst) {
-      *reinterpret_cast<uint4 *>(ref[i].dst + at1[i]) = x[i];
-      *reinterpret_cast<uint4 *>(ref[i].dst + at2[i]) = y[i];
+    rows[i] = r;
+  }
+  __syncthreads();
+  const int lane = static_cast<int>(threadIdx.x) / per_head;
+  const int j = static_cast<int>(threadIdx.x) - lane * per_head;
+  if (lane >= lanes) return;
+  const bool rotated = j < a.rot / (2 * VE);
+  int at1 = j * 2 * VE, at2 = at1 + VE;
+  if (a.neox && rotated) at1 = j * VE, at2 = at1 + a.rot / 2;
+  int done = lane;              // of the block's heads
+  int dt = 0, h = rem + lane;   // row and head
+  int angle_of = -1;            // row whose cosines and sines are in c and s
+  float c[VE], s[VE];
+#pragma unroll 1
+  while (done < count) {
+    // the loads of kAtOnce units before the first store: results may go to the
+    // inputs, so the compiler would not move a load over a store
+    uint4 x[kAtOnce], y[kAtOnce];
+    T *dst[kAtOnce], *dst2[kAtOnce];
+    int row[kAtOnce];  // -1: passes through
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      dst[i] = dst2[i] = nullptr;
+      row[i] = -1;
+      if (done + i * lanes >= count) continue;
+      while (h >= heads) h -= heads, ++dt;
+      const long long t = t_first + dt;
+      const Row &r = rows[dt];
+      const T *src;
+      int of = h;
+      if (of < a.heads) {
+        src = static_cast<const T *>(a.q) + t * a.q_stride + of * a.dim;
+        dst[i] = static_cast<T *>(a.q_out) + t * a.q_out_stride + of * a.dim;
+        row[i] = dt;
+      } else if ((of -= a.heads) < a.kv_heads) {
+        src = static_cast<const T *>(a.k) + t * a.k_stride + of * a.dim;
+        if (a.k_out) dst[i] = static_cast<T *>(a.k_out) + t * a.k_out_stride + of * a.dim;
+        if (r.k_at >= 0) dst2[i] = static_cast<T *>(a.k_cache) + r.k_at + of * a.k_head;
+        row[i] = dt;
+      } else {
+        of -= a.kv_heads;
+        src = static_cast<const T *>(a.v) + t * a.v_stride + of * a.dim;
+        if (r.v_at >= 0) dst2[i] = static_cast<T *>(a.v_cache) + r.v_at + of * a.v_head;
+      }
+      x[i] = *reinterpret_cast<const uint4 *>(src + at1);
+      y[i] = *reinterpret_cast<const uint4 *>(src + at2);
+      if (r.pos < 0) {
+        x[i] = y[i] = make_uint4(0, 0, 0, 0);
+        row[i] = -1;
+      }
+      h += lanes;
     }
-    if (ref[i].dst2) {
-      *reinterpret_cast<uint4 *>(ref[i].dst2 + at1[i]) = x[i];
-      *reinterpret_cast<uint4 *>(ref[i].dst2 + at2[i]) = y[i];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (row[i] >= 0 && rotated) {
+        if (row[i] != angle_of) {
+          const CT *table = static_cast<const CT *>(a.table) + rows[row[i]].pos * a.rot + j * VE;
+          load_table<CT, VE>(table, c);
+          load_table<CT, VE>(table + a.rot / 2, s);
+          angle_of = row[i];
+        }
+        T *p = reinterpret_cast<T *>(&x[i]), *r = reinterpret_cast<T *>(&y[i]);
+        if (a.neox) {
+#pragma unroll
+          for (int e = 0; e < VE; ++e) {
+            const float f = as_float(p[e]), g = as_float(r[e]);
+            p[e] = round_to<T>(f * c[e] - g * s[e]);
+            r[e] = round_to<T>(g * c[e] + f * s[e]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < VE; ++e) {
+            T *w = e < VE / 2 ? p + 2 * e : r + 2 * e - VE;
+            const float f = as_float(w[0]), g = as_float(w[1]);
+            w[0] = round_to<T>(f * c[e] - g * s[e]);
+            w[1] = round_to<T>(g * c[e] + f * s[e]);
+          }
+        }
+      }
+      if (dst[i]) {
+        *reinterpret_cast<uint4 *>(dst[i] + at1) = x[i];
+        *reinterpret_cast<uint4 *>(dst[i] + at2) = y[i];
+      }
+      if (dst2[i]) {
+        *reinterpret_cast<uint4 *>(dst2[i] + at1) = x[i];
+        *reinterpret_cast<uint4 *>(dst2[i] + at2) = y[i];
+      }
     }
+    done += kAtOnce * lanes;
   }
 }
 
@@ -229,11 +281,16 @@ template <typename T, typename CT>
 cudaError_t launch(const RopeArgs &a, bool vec, cudaStream_t stream) {
   const long long heads = a.heads + (a.k ? a.kv_heads : 0) + (a.v ? a.kv_heads : 0);
   if (vec) {
-    const long long units = a.num_tokens * heads * (a.dim / (2 * (16 / sizeof(T))));
-    const long long per_block = kRopeThreads * kUnitsPerThread;
-    const long long blocks = (units + per_block - 1) / per_block;
+    const long long lanes = kRopeThreads / (a.dim / (2 * (16 / static_cast<int>(sizeof(T)))));
+    // fewer heads a thread while that fills the GPU better (two blocks per SM)
+    const long long all = a.num_tokens * heads;
+    const long long deep = std::max(1ll, std::min(all / (lanes * 296), 1ll * kHeadsPerThread));
+    const long long per_block = lanes * deep;
+    const long long blocks = (all + per_block - 1) / per_block;
     if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    rope_cache_vec_kernel<T, CT><<<static_cast<unsigned>(blocks), kRopeThreads, 0, stream>>>(a);
+    const int rows = static_cast<int>((per_block + heads - 2) / heads + 1);  // at most, of a block
+    rope_cache_vec_kernel<T, CT><<<static_cast<unsigned>(blocks), kRopeThreads, rows * 24, stream>>>(
+        a, static_cast<int>(heads), static_cast<int>(per_block));
   } else {
     const long long units = a.num_tokens * heads * ((a.dim + 1) / 2);
     const long long blocks = std::min((units + kRopeThreads - 1) / kRopeThreads, 148ll * 32);

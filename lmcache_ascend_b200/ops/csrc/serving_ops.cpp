@@ -274,7 +274,7 @@ void rotary_embedding_and_cache(
   const int64_t es = query.element_size(), cs = cos_sin_cache.element_size();
   // 16-byte units: whole pairs of vectors in the head and in its rotated part,
   // and table rows whose halves start on 16 bytes
-  vec = vec && D * es % 32 == 0 && rot * es % 32 == 0 && rot / 2 * cs % 16 == 0 &&
+  vec = vec && D * es % 32 == 0 && D * es <= 32 * 256 && rot * es % 32 == 0 && rot / 2 * cs % 16 == 0 &&
         16 / es * cs % 16 == 0 && reinterpret_cast<uintptr_t>(a.table) % 16 == 0;
   const c10::cuda::CUDAGuard guard(dev);
   C10_CUDA_CHECK(launch_rope_cache(a, row_type(dt), row_type(cos_sin_cache.scalar_type()), vec,

@@ -151,31 +151,42 @@ __global__ void __launch_bounds__(kSlotThreads) slot_mapping_kernel(SlotArgs a) 
       report_status(a.status, kStatusBadIndex, kWhereTable, b, col);
   }
 
-  // --- tokens
+  // --- tokens: a warp takes 128 in a row, mostly of one request, which it looks
+  // up once
   OT *slots = static_cast<OT *>(a.slots);
   OT *positions = static_cast<OT *>(a.positions);
-  const long long t0 = static_cast<long long>(blockIdx.x) * kTokensPerBlock;
-  const long long t1 = min(a.num_tokens, t0 + kTokensPerBlock);
-  for (long long t = t0 + tid; t < t1; t += kSlotThreads) {
+  const long long t0 =
+      static_cast<long long>(blockIdx.x) * kTokensPerBlock + warp * (kTokensPerBlock / (kSlotThreads / 32));
+  const long long t1 = min(a.num_tokens, t0 + kTokensPerBlock / (kSlotThreads / 32));
+  if (t0 >= t1) return;
+  int b = 0;
+  long long start = 0, pages = 0, c = 0, have = 0;
+  Need n = {0, 0};
+  auto look_up = [&](int request) {
+    b = request;
+    c = length_of<LT>(a.ctx, b);
+    n = need_of<LT>(a, b);
+    have = pages_of(c, a.block_size);
+  };
+  if (t0 < total_tokens) {
+    const int g = last_leq(s.tokens, kSlotThreads, t0);
+    start = s.tokens[g], pages = s.pages[g];
+    look_up(g * seg);
+  }
+  for (long long t = t0 + lane; t < t1; t += 32) {
     if (t >= total_tokens) {  // rows behind the last request
       slots[t] = -1;
       positions[t] = 0;
       a.request_ids[t] = -1;
       continue;
     }
-    const int g = last_leq(s.tokens, kSlotThreads, t);
-    int b = g * seg;
-    long long start = s.tokens[g], pages = s.pages[g];
-    Need n = need_of<LT>(a, b);
     while (t >= start + n.tokens) {
       start += n.tokens;
       pages += n.pages;
-      n = need_of<LT>(a, ++b);
+      look_up(b + 1);
     }
-    const long long c = length_of<LT>(a.ctx, b);
     const long long pos = c + (t - start);
     const long long col = static_cast<unsigned>(pos) / static_cast<unsigned>(a.block_size);
-    const long long have = pages_of(c, a.block_size);
     long long page = -1;
     if (col >= a.width) {
       report_status(a.status, kStatusBadIndex, kWhereTable, b, col);

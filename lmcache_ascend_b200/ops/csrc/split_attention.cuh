@@ -1,4 +1,4 @@
-// Attention of few rows over paged keys, split over the keys.
+// Attention of few rows, or over few keys, split over the keys.
 //
 // A block owns 16 rows of one KV head (a request's query tokens and heads; a
 // decode step's group of heads fits) and a slice of their keys.  Each of its
@@ -7,7 +7,9 @@
 // warps' results are joined at the end.  Products are 16x8x16 tensor
 // instructions: the block reads every key and value once and multiplies it with
 // 16 rows, 16 flop a byte, so it is bound by the reads and the small
-// instruction loses nothing.  Any block size, page order and stride.
+// instruction loses nothing.  Any block size, page order and stride; dense keys
+// for few rows or short calls, where the tensor-core kernel's 256-row blocks
+// would wait most of the time.  With one slice the block writes the result.
 #pragma once
 #include "attention_join.cuh"
 
@@ -15,14 +17,14 @@ namespace lmc {
 
 constexpr int kSplitWarps = 4, kSplitKeys = 16, kSplitRows = 16, kSplitStages = 3;
 
-// Which keys and rows a pass covers: prefix keys [pre_begin, pre_end), then the
-// own keys of the unit's request when `own`; a unit is a request, or all of
-// them (own == false).
+// Which keys and rows a pass covers.  Paged: prefix keys [pre_begin, pre_end),
+// then the own keys of the unit's request when `own`; a unit is a request, or all
+// of them (own == false).  Dense: one unit of all rows, all keys.
 struct SplitPass {
   int pre_begin, pre_end;
   bool own;
   int unit_tokens, row_tiles, slices;
-  float *part_o, *part_lse;  // first slice of this pass
+  float *part_o, *part_lse;  // first slice of this pass; null: write the result
 };
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
@@ -64,12 +66,41 @@ struct SplitSmem {
   static_assert(kBytes >= kSplitWarps * kSplitRows * (D + 2) * 4, "join fits in the rings");
 };
 
+// A row of the batch by the definition, on one warp: when a joined result holds
+// an infinity or NaN (a draft token's value that earlier rows must not see).
 template <typename T, int D>
+__device__ __noinline__ void strict_paged_row(const PagedArgs &a, long long r) {
+  const int h = static_cast<int>(r % a.heads), kv = h / (a.heads / a.kv_heads);
+  const int t = static_cast<int>(r / a.heads), b = t / a.q_len, i = t - b * a.q_len;
+  const int n = max(0, a.own_lens[b]);
+  const long long pos = a.prefix_len + n - a.q_len + i;
+  const long long room = static_cast<long long>(a.width) * a.block_size;
+  const long long own = min(room, max(0ll, static_cast<long long>(n) - a.q_len + i + 1));
+  const float slope = a.slopes ? a.slopes[h] : 0.f;
+  WarpRow<T, D> row;
+  row.start(static_cast<const T *>(a.q) + b * a.q_batch + i * a.q_token + h * a.q_head);
+  for (long long j = 0; j < a.prefix_len + own; ++j) {
+    const bool shared = j < a.prefix_len;
+    const unsigned at = static_cast<unsigned>(shared ? j : j - a.prefix_len);
+    const unsigned col = at / static_cast<unsigned>(a.block_size);
+    const int off = static_cast<int>(at - col * a.block_size);
+    const int page = shared ? a.prefix_blocks[col] : a.tables[b * a.table_stride + col];
+    if (page < 0 || page >= a.num_blocks) continue;
+    row.add(static_cast<const T *>(a.k) + page * a.k_block + off * a.k_slot + kv * a.k_head,
+            static_cast<const T *>(a.v) + page * a.v_block + off * a.v_slot + kv * a.v_head,
+            a.scale, a.softcap, slope * fabsf(static_cast<float>(pos - j)));
+  }
+  row.finish(static_cast<T *>(a.out) + r * D, a.lse ? a.lse + r : nullptr);
+}
+
+template <typename T, int D, typename Args>
 __global__ void __launch_bounds__(kSplitWarps * 32, 2)
-    paged_split_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ SplitPass s) {
+    split_attention_kernel(const __grid_constant__ Args a, const __grid_constant__ SplitPass s) {
+  constexpr bool kDense = __is_same(Args, PositionArgs);
   using L = SplitSmem<D>;
   constexpr int kChunks = D / 8;  // 16-byte chunks of a row
   extern __shared__ __align__(128) uint8_t smem[];
+  let_next_start();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int group = a.heads / a.kv_heads;
   const int slice = blockIdx.y;
@@ -77,18 +108,25 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 2)
   const int kv = u % a.kv_heads;
   u /= a.kv_heads;
   const int row_tile = u % s.row_tiles, unit = u / s.row_tiles;
-  const int n = s.own ? max(0, a.own_lens[unit]) : 0;
-  const int pre = s.pre_end - s.pre_begin;
-  // keys: the pass's prefix part, then own keys within the request's table row
-  const long long room = static_cast<long long>(a.width) * a.block_size;
-  const int own_keys = static_cast<int>(min(static_cast<long long>(n), room));
-  if (n > room && slice == 0 && row_tile == 0 && threadIdx.x == 0)
-    report_status(a.status, kStatusBadIndex, unit, n, room);
-  const int total = pre + own_keys;
+  int n = 0, pre = 0, own_keys = 0, total;
+  long long all_rows;
+  if constexpr (kDense) {
+    total = a.k_tokens;
+    all_rows = static_cast<long long>(a.q_tokens) * a.heads;
+  } else {
+    // the pass's prefix part, then own keys within the request's table row
+    n = s.own ? max(0, a.own_lens[unit]) : 0;
+    pre = s.pre_end - s.pre_begin;
+    const long long room = static_cast<long long>(a.width) * a.block_size;
+    own_keys = static_cast<int>(min(static_cast<long long>(n), room));
+    if (n > room && slice == 0 && row_tile == 0 && threadIdx.x == 0)
+      report_status(a.status, kStatusBadIndex, unit, n, room);
+    total = pre + own_keys;
+    all_rows = static_cast<long long>(a.batch) * a.q_len * a.heads;
+  }
   const int chunk = kSplitWarps * kSplitKeys;
   const int per = ((total + s.slices - 1) / s.slices + chunk - 1) / chunk * chunk;
   const int k0 = min(total, slice * per), k1 = min(total, k0 + per);
-  const long long all_rows = static_cast<long long>(a.batch) * a.q_len * a.heads;
 
   // row r of this tile: token and head (rows past the unit's are not stored)
   const int rows = s.unit_tokens * group - row_tile * kSplitRows;
@@ -96,10 +134,12 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 2)
   auto head_of = [&](int r) { return kv * group + (row_tile * kSplitRows + r) % group; };
   float *part_o = s.part_o + static_cast<long long>(slice) * all_rows * D;
   float *part_lse = s.part_lse + static_cast<long long>(slice) * all_rows;
-  if (k0 >= k1) {  // no keys: an empty part
+  const bool direct = s.part_o == nullptr;
+  if (k0 >= k1 && !direct) {  // no keys: an empty part
     if (threadIdx.x < kSplitRows && static_cast<int>(threadIdx.x) < rows)
       part_lse[static_cast<long long>(token_of(threadIdx.x)) * a.heads + head_of(threadIdx.x)] =
           -INFINITY;
+    wait_for_previous();
     return;
   }
 
@@ -107,12 +147,15 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 2)
   const uint32_t ring_addr = smem_u32(ring);
   const int steps = (k1 - k0 + chunk - 1) / chunk;
 
-  // Pages of the 16 keys of step `it` of this warp: lane i (and i + 16) key i.
+  // Pages (dense: indices) of the 16 keys of step `it` of this warp: lane i (and
+  // i + 16) key i; -1 where there is none.
   auto key_page = [&](int it, int &off, bool &bad) -> int {
     const int j = k0 + it * chunk + warp * kSplitKeys + (lane & 15);
     bad = false;
     off = 0;
     if (j >= k1) return -1;
+    if constexpr (kDense) return j;
+    else {
     const bool shared = j < pre;
     const unsigned at = shared ? s.pre_begin + j : j - pre;
     const unsigned col = at / static_cast<unsigned>(a.block_size);
@@ -122,6 +165,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 2)
     bad = true;
     if (lane < 16) report_status(a.status, kStatusBadSlot, shared ? -1 : unit, col, page);
     return -1;
+    }
   };
   auto load = [&](int it, int page, int off) {
     const uint32_t dst = ring_addr + (it % kSplitStages) * L::kStage;
@@ -134,10 +178,15 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 2)
       const bool valid = pg >= 0;  // else zeros: nothing of the page is read
       const long long p = valid ? pg : 0;
       const uint32_t at = r * (D * 2) + ((c & ~7) << 4) + (((c & 7) ^ (r & 7)) << 4);
-      cp_async16(dst + at, static_cast<const T *>(a.k) + p * a.k_block + of * a.k_slot +
-                               kv * a.k_head + c * 8, valid);
-      cp_async16(dst + L::kKeys + at, static_cast<const T *>(a.v) + p * a.v_block +
-                                          of * a.v_slot + kv * a.v_head + c * 8, valid);
+      const T *k = static_cast<const T *>(a.k) + kv * a.k_head + c * 8;
+      const T *v = static_cast<const T *>(a.v) + kv * a.v_head + c * 8;
+      if constexpr (kDense) {
+        k += p * a.k_token, v += p * a.v_token;
+      } else {
+        k += p * a.k_block + of * a.k_slot, v += p * a.v_block + of * a.v_slot;
+      }
+      cp_async16(dst + at, k, valid);
+      cp_async16(dst + L::kKeys + at, v, valid);
     }
   };
 
@@ -164,9 +213,10 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 2)
   const int r0 = lane >> 2, r1 = r0 + 8, c0 = (lane & 3) * 2;
   uint32_t q[D / 16][4];
   auto q_row = [&](int r) -> const T * {
-    const int t = token_of(r), b = t / a.q_len;
-    return static_cast<const T *>(a.q) + b * a.q_batch + (t - b * a.q_len) * a.q_token +
-           head_of(r) * a.q_head;
+    const int t = token_of(r);
+    const T *p = static_cast<const T *>(a.q) + head_of(r) * a.q_head;
+    if constexpr (kDense) return p + t * a.q_token;
+    else return p + t / a.q_len * a.q_batch + t % a.q_len * a.q_token;
   };
   {
     const T *p0 = r0 < rows ? q_row(r0) : nullptr, *p1 = r1 < rows ? q_row(r1) : nullptr;
@@ -179,29 +229,50 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 2)
       q[k][3] = p1 ? *reinterpret_cast<const uint32_t *>(p1 + c + 8) : 0;
     }
   }
-  // Row i of a request sees its own keys up to n - q_len + i: as an index into
-  // this pass's keys, j < last.
-  auto last_of = [&](int r) {
-    if (!s.own) return total;
-    const int i = r < rows ? token_of(r) - unit * a.q_len : 0;
-    return pre + max(0, min(own_keys, n - a.q_len + i + 1));
-  };
-  const int last0 = last_of(r0), last1 = last_of(r1);
+  // Paged: row i of a request sees its own keys up to n - q_len + i, as an index
+  // into this pass's keys j < last.  Dense: positions below the row's limit in its
+  // document.
+  RowMask mask0 = {0, 0, 0}, mask1 = {0, 0, 0};
+  int last0 = total, last1 = total;
   float slope0 = 0.f, slope1 = 0.f, at0 = 0.f, at1 = 0.f;
   if (a.slopes) {
-    auto place = [&](int r, float &slope, float &at) {
-      if (r >= rows) return;
-      const int t = token_of(r), b = t / a.q_len;
-      slope = a.slopes[head_of(r)] * kLog2e;
-      at = static_cast<float>(a.prefix_len + max(0, a.own_lens[b]) - a.q_len + (t - b * a.q_len));
-    };
-    place(r0, slope0, at0);
-    place(r1, slope1, at1);
+    slope0 = r0 < rows ? a.slopes[head_of(r0)] * kLog2e : 0.f;
+    slope1 = r1 < rows ? a.slopes[head_of(r1)] * kLog2e : 0.f;
   }
-  // position of pass key j: in the prefix, or behind it
-  auto place_of = [&](int j) {
-    return static_cast<float>(j < pre ? s.pre_begin + j : a.prefix_len + (j - pre));
+  if constexpr (kDense) {
+    if (r0 < rows) mask0 = row_mask(a, token_of(r0));
+    if (r1 < rows) mask1 = row_mask(a, token_of(r1));
+  } else {
+    auto place = [&](int r, int &last, float &at) {
+      if (r >= rows) return;
+      const int t = token_of(r), b = t / a.q_len, i = t - b * a.q_len;
+      if (s.own) last = pre + max(0, min(own_keys, n - a.q_len + i + 1));
+      if (a.slopes)
+        at = static_cast<float>(a.prefix_len + max(0, a.own_lens[b]) - a.q_len + i);
+    };
+    place(r0, last0, at0);
+    place(r1, last1, at1);
+  }
+  // -slope times the distance between the row and pass key j
+  auto bias = [&](bool second, int j, int kp) {
+    if constexpr (kDense) {
+      const long long at = second ? mask1.pos : mask0.pos;
+      return -(second ? slope1 : slope0) * fabsf(static_cast<float>(at - kp));
+    } else {
+      const float at = static_cast<float>(j < pre ? s.pre_begin + j : a.prefix_len + (j - pre));
+      return -(second ? slope1 : slope0) * fabsf((second ? at1 : at0) - at);
+    }
   };
+  // dense: position and document of key lane % 16 of a step
+  int kp_next = 0, kd_next = 0;
+  auto key_marks = [&](int it) {
+    if constexpr (kDense) {
+      const int j = min(k0 + it * chunk + warp * kSplitKeys + (lane & 15), a.k_tokens - 1);
+      kp_next = a.k_pos ? clamp_pos(position_at(a.k_pos, a.long_k_pos, j)) : j;
+      kd_next = a.k_doc ? a.k_doc[j] : 0;
+    }
+  };
+  if (steps > 0) key_marks(0);
   const float scale = a.scale * kLog2e;
   const float cap_in = a.softcap > 0.f ? 2.f * kLog2e * a.scale / a.softcap : 0.f;
   const float cap_out = a.softcap * kLog2e;
@@ -226,6 +297,8 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 2)
       cp_async_commit();
       if (nx + 1 < steps) page = key_page(nx + 1, off, bad);
     }
+    const int kp_all = kp_next, kd_all = kd_next;
+    if (it + 1 < steps) key_marks(it + 1);
     cp_async_wait<kSplitStages - 1>();
     __syncwarp();
     const uint32_t kb = ring_addr + (it % kSplitStages) * L::kStage, vb = kb + L::kKeys;
@@ -248,17 +321,31 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 2)
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int col = t * 8 + c0 + (e & 1), j = j0 + col;
-        float x = sc[t][e];
-        if (cap_out > 0.f)
-          x = fmaf(rcp(1.f + ex2(x * cap_in)), -2.f * cap_out, cap_out);
-        else
-          x *= scale;
-        if (a.slopes)
-          x = fmaf(-(e < 2 ? slope0 : slope1), fabsf((e < 2 ? at0 : at1) - place_of(j)), x);
-        if (j >= (e < 2 ? last0 : last1) || j >= k1 || ((bad_keys >> col) & 1)) x = -INFINITY;
-        sc[t][e] = x;
+      for (int e = 0; e < 2; ++e) {
+        const int col = t * 8 + c0 + e, j = j0 + col;
+        bool out0 = j >= k1, out1 = out0;
+        int kp = 0;
+        if constexpr (kDense) {
+          kp = __shfl_sync(0xffffffffu, kp_all, col);
+          const int kd = __shfl_sync(0xffffffffu, kd_all, col);
+          out0 = out0 || kp >= mask0.limit || (a.k_doc && kd != mask0.doc);
+          out1 = out1 || kp >= mask1.limit || (a.k_doc && kd != mask1.doc);
+        } else {
+          const bool bad_key = (bad_keys >> col) & 1;
+          out0 = out0 || j >= last0 || bad_key;
+          out1 = out1 || j >= last1 || bad_key;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float x = sc[t][2 * h + e];
+          if (cap_out > 0.f)
+            x = fmaf(rcp(1.f + ex2(x * cap_in)), -2.f * cap_out, cap_out);
+          else
+            x *= scale;
+          if (a.slopes) x += bias(h == 1, j, kp);
+          if (h ? out1 : out0) x = -INFINITY;
+          sc[t][2 * h + e] = x;
+        }
       }
     }
     float top0 = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1]));
@@ -331,6 +418,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 2)
     }
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : NAN);
     const long long row = static_cast<long long>(token_of(r)) * a.heads + head_of(r);
+    bool finite = true;
     for (int d = lane * 4; d < D; d += 128) {
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -339,38 +427,50 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 2)
         acc.x = fmaf(f[w], v.x, acc.x), acc.y = fmaf(f[w], v.y, acc.y);
         acc.z = fmaf(f[w], v.z, acc.z), acc.w = fmaf(f[w], v.w, acc.w);
       }
-      *reinterpret_cast<float4 *>(part_o + row * D + d) =
-          make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+      acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
+      if (direct) {
+        const uint2 w = make_uint2(pair_from_float<T>(acc.x, acc.y),
+                                   pair_from_float<T>(acc.z, acc.w));
+        *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + row * D + d) = w;
+        const float big = fmaxf(fmaxf(fabsf(acc.x), fabsf(acc.y)), fmaxf(fabsf(acc.z), fabsf(acc.w)));
+        finite = finite && big <= 3.4028235e38f && acc.x + acc.y + acc.z + acc.w ==
+                                                       acc.x + acc.y + acc.z + acc.w;
+      } else {
+        *reinterpret_cast<float4 *>(part_o + row * D + d) = acc;
+      }
     }
-    if (lane == 0) part_lse[row] = l == 0.f ? -INFINITY : m + log2f(l);
+    if (lane == 0) {
+      const float log2_sum = l == 0.f ? -INFINITY : m + log2f(l);
+      if (!direct) part_lse[row] = log2_sum;
+      else if (a.lse) a.lse[row] = log2_sum * kLn2;
+    }
+    if (direct && !__all_sync(0xffffffffu, finite)) {
+      __syncwarp();  // the row written above is written again
+      if constexpr (kDense)
+        strict_position_row<T, D>(a, token_of(r), head_of(r));
+      else
+        strict_paged_row<T, D>(a, row);
+    }
   }
+  wait_for_previous();
 }
 
-// A row of the batch by the definition, on one warp: when a joined result holds
-// an infinity or NaN (a draft token's value that earlier rows must not see).
-template <typename T, int D>
-__device__ __noinline__ void strict_paged_row(const PagedArgs &a, long long r) {
-  const int h = static_cast<int>(r % a.heads), kv = h / (a.heads / a.kv_heads);
-  const int t = static_cast<int>(r / a.heads), b = t / a.q_len, i = t - b * a.q_len;
-  const int n = max(0, a.own_lens[b]);
-  const long long pos = a.prefix_len + n - a.q_len + i;
-  const long long room = static_cast<long long>(a.width) * a.block_size;
-  const long long own = min(room, max(0ll, static_cast<long long>(n) - a.q_len + i + 1));
-  const float slope = a.slopes ? a.slopes[h] : 0.f;
-  WarpRow<T, D> row;
-  row.start(static_cast<const T *>(a.q) + b * a.q_batch + i * a.q_token + h * a.q_head);
-  for (long long j = 0; j < a.prefix_len + own; ++j) {
-    const bool shared = j < a.prefix_len;
-    const unsigned at = static_cast<unsigned>(shared ? j : j - a.prefix_len);
-    const unsigned col = at / static_cast<unsigned>(a.block_size);
-    const int off = static_cast<int>(at - col * a.block_size);
-    const int page = shared ? a.prefix_blocks[col] : a.tables[b * a.table_stride + col];
-    if (page < 0 || page >= a.num_blocks) continue;
-    row.add(static_cast<const T *>(a.k) + page * a.k_block + off * a.k_slot + kv * a.k_head,
-            static_cast<const T *>(a.v) + page * a.v_block + off * a.v_slot + kv * a.v_head,
-            a.scale, a.softcap, slope * fabsf(static_cast<float>(pos - j)));
-  }
-  row.finish(static_cast<T *>(a.out) + r * D, a.lse ? a.lse + r : nullptr);
+// Towards one wave of two blocks per SM, with 128 keys or more each: a block has
+// a start and an end to pay whatever the length of its slice.
+inline int split_slices(long long blocks, long long keys) {
+  const long long want = std::min(296 / std::max(1ll, blocks), (keys + 127) / 128);
+  return static_cast<int>(std::max(1ll, std::min(want, 64ll)));
+}
+
+template <typename T, int D, typename Args>
+cudaError_t launch_split(const Args &a, const SplitPass &s, long long units, bool first,
+                         cudaStream_t stream) {
+  constexpr int kBytes = SplitSmem<D>::kBytes;
+  cudaError_t e = allow_smem(split_attention_kernel<T, D, Args>, kBytes);
+  if (e != cudaSuccess) return e;
+  const dim3 grid(static_cast<unsigned>(units * s.row_tiles * a.kv_heads), s.slices);
+  return launch_ordered(split_attention_kernel<T, D, Args>, grid, kSplitWarps * 32, kBytes, first,
+                        stream, a, s);
 }
 
 template <typename T, int D>
@@ -379,6 +479,7 @@ __global__ void __launch_bounds__(128)
                       const float *part_lse, int slices) {
   const long long rows = static_cast<long long>(a.batch) * a.q_len * a.heads;
   const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  wait_for_previous();
   if (row >= rows) return;
   JoinedRow<T, D> r;
   r.join(part_o, part_lse, slices, rows, row);

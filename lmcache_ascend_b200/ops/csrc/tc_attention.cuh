@@ -283,6 +283,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int t_begin = slice * a.tiles_per_slice;
   const int t_end = min(a.k_tiles, t_begin + a.tiles_per_slice);
 
+  let_next_start();
   if (warp == kMmaWarp) tmem_alloc(tmem_slot, 512);
   if (warp == kLoadWarp && lane == 0) {
     prefetch_map(&k_map), prefetch_map(&v_map);
@@ -339,6 +340,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   // the whole of tensor memory starts at column 0: a constant address
   constexpr uint32_t tmem = 0;
   if (kDense) {
+    wait_for_previous();  // the key tiles' ranges
     if (warp < kMmaWarp && x < tiles && lane == 0 && half == 0) {
       atomicMin(&seen[0], lim_lo), atomicMax(&seen[1], lim_hi);
       atomicMin(&seen[2], doc_lo), atomicMax(&seen[3], doc_hi);
