@@ -15,7 +15,11 @@
 // has D / (2 * VE) units whatever the layout.  A thread keeps its place in the
 // head and walks over the heads of q, k and v of one row after the other, so that
 // a unit costs no division and a row's cosines and sines are loaded once for
-// several heads; blocks get equal work for one row or many.
+// several heads; blocks get equal work for one row or many.  The loads in flight
+// come from many threads with one unit each (five blocks of 256 per SM), not from
+// several units a thread: 16385 rows of 64/8 heads of 128 (680 MB) take 113 us
+// (6.0 TB/s) so, 150 us with two units a thread in four blocks, 126 us in six
+// blocks (spills).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -28,7 +32,7 @@ namespace lmc {
 namespace {
 
 constexpr int kRopeThreads = 256;
-constexpr int kHeadsPerThread = 8, kAtOnce = 2;  // four vector loads in flight a thread
+constexpr int kHeadsPerThread = 12, kBlockHeads = 2048, kResident = 148 * 5;
 
 __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -108,8 +112,8 @@ __device__ __forceinline__ void load_table(const CT *p, float *f) {
 // block takes `per_block` of them in a row, up to kHeadsPerThread a thread.  Its rows are looked up first (position, page), so that its data
 // and table loads wait for nothing but their own memory.
 template <typename T, typename CT>
-__global__ void __launch_bounds__(kRopeThreads) rope_cache_vec_kernel(RopeArgs a, int heads,
-                                                                      int per_block) {
+__global__ void __launch_bounds__(kRopeThreads, 5)
+    rope_cache_vec_kernel(RopeArgs a, int heads, int per_block) {
   constexpr int VE = 16 / sizeof(T);
   struct Row {
     long long pos, k_at, v_at;  // position, offsets of the slot's first head; -1: none
@@ -150,86 +154,68 @@ __global__ void __launch_bounds__(kRopeThreads) rope_cache_vec_kernel(RopeArgs a
   const bool rotated = j < a.rot / (2 * VE);
   int at1 = j * 2 * VE, at2 = at1 + VE;
   if (a.neox && rotated) at1 = j * VE, at2 = at1 + a.rot / 2;
-  int done = lane;              // of the block's heads
-  int dt = 0, h = rem + lane;   // row and head
-  int angle_of = -1;            // row whose cosines and sines are in c and s
+  int dt = 0, h = rem + lane;  // row and head
+  int angle_of = -1;           // row whose cosines and sines are in c and s
   float c[VE], s[VE];
 #pragma unroll 1
-  while (done < count) {
-    // the loads of kAtOnce units before the first store: results may go to the
-    // inputs, so the compiler would not move a load over a store
-    uint4 x[kAtOnce], y[kAtOnce];
-    T *dst[kAtOnce], *dst2[kAtOnce];
-    int row[kAtOnce];  // -1: passes through
+  for (int done = lane; done < count; done += lanes, h += lanes) {
+    while (h >= heads) h -= heads, ++dt;
+    const long long t = t_first + dt;
+    const Row &r = rows[dt];
+    const T *src;
+    T *dst = nullptr, *dst2 = nullptr;
+    int of = h;
+    bool turn = rotated;
+    if (of < a.heads) {
+      src = static_cast<const T *>(a.q) + t * a.q_stride + of * a.dim;
+      dst = static_cast<T *>(a.q_out) + t * a.q_out_stride + of * a.dim;
+    } else if ((of -= a.heads) < a.kv_heads) {
+      src = static_cast<const T *>(a.k) + t * a.k_stride + of * a.dim;
+      if (a.k_out) dst = static_cast<T *>(a.k_out) + t * a.k_out_stride + of * a.dim;
+      if (r.k_at >= 0) dst2 = static_cast<T *>(a.k_cache) + r.k_at + of * a.k_head;
+    } else {
+      of -= a.kv_heads;
+      turn = false;
+      src = static_cast<const T *>(a.v) + t * a.v_stride + of * a.dim;
+      if (r.v_at >= 0) dst2 = static_cast<T *>(a.v_cache) + r.v_at + of * a.v_head;
+    }
+    uint4 x = *reinterpret_cast<const uint4 *>(src + at1);
+    uint4 y = *reinterpret_cast<const uint4 *>(src + at2);
+    if (r.pos < 0) {
+      x = y = make_uint4(0, 0, 0, 0);
+    } else if (turn) {
+      if (dt != angle_of) {
+        const CT *table = static_cast<const CT *>(a.table) + r.pos * a.rot + j * VE;
+        load_table<CT, VE>(table, c);
+        load_table<CT, VE>(table + a.rot / 2, s);
+        angle_of = dt;
+      }
+      T *p = reinterpret_cast<T *>(&x), *q = reinterpret_cast<T *>(&y);
+      if (a.neox) {
 #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      dst[i] = dst2[i] = nullptr;
-      row[i] = -1;
-      if (done + i * lanes >= count) continue;
-      while (h >= heads) h -= heads, ++dt;
-      const long long t = t_first + dt;
-      const Row &r = rows[dt];
-      const T *src;
-      int of = h;
-      if (of < a.heads) {
-        src = static_cast<const T *>(a.q) + t * a.q_stride + of * a.dim;
-        dst[i] = static_cast<T *>(a.q_out) + t * a.q_out_stride + of * a.dim;
-        row[i] = dt;
-      } else if ((of -= a.heads) < a.kv_heads) {
-        src = static_cast<const T *>(a.k) + t * a.k_stride + of * a.dim;
-        if (a.k_out) dst[i] = static_cast<T *>(a.k_out) + t * a.k_out_stride + of * a.dim;
-        if (r.k_at >= 0) dst2[i] = static_cast<T *>(a.k_cache) + r.k_at + of * a.k_head;
-        row[i] = dt;
+        for (int e = 0; e < VE; ++e) {
+          const float f = as_float(p[e]), g = as_float(q[e]);
+          p[e] = round_to<T>(f * c[e] - g * s[e]);
+          q[e] = round_to<T>(g * c[e] + f * s[e]);
+        }
       } else {
-        of -= a.kv_heads;
-        src = static_cast<const T *>(a.v) + t * a.v_stride + of * a.dim;
-        if (r.v_at >= 0) dst2[i] = static_cast<T *>(a.v_cache) + r.v_at + of * a.v_head;
-      }
-      x[i] = *reinterpret_cast<const uint4 *>(src + at1);
-      y[i] = *reinterpret_cast<const uint4 *>(src + at2);
-      if (r.pos < 0) {
-        x[i] = y[i] = make_uint4(0, 0, 0, 0);
-        row[i] = -1;
-      }
-      h += lanes;
-    }
 #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      if (row[i] >= 0 && rotated) {
-        if (row[i] != angle_of) {
-          const CT *table = static_cast<const CT *>(a.table) + rows[row[i]].pos * a.rot + j * VE;
-          load_table<CT, VE>(table, c);
-          load_table<CT, VE>(table + a.rot / 2, s);
-          angle_of = row[i];
-        }
-        T *p = reinterpret_cast<T *>(&x[i]), *r = reinterpret_cast<T *>(&y[i]);
-        if (a.neox) {
-#pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            const float f = as_float(p[e]), g = as_float(r[e]);
-            p[e] = round_to<T>(f * c[e] - g * s[e]);
-            r[e] = round_to<T>(g * c[e] + f * s[e]);
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            T *w = e < VE / 2 ? p + 2 * e : r + 2 * e - VE;
-            const float f = as_float(w[0]), g = as_float(w[1]);
-            w[0] = round_to<T>(f * c[e] - g * s[e]);
-            w[1] = round_to<T>(g * c[e] + f * s[e]);
-          }
+        for (int e = 0; e < VE; ++e) {
+          T *w = e < VE / 2 ? p + 2 * e : q + 2 * e - VE;
+          const float f = as_float(w[0]), g = as_float(w[1]);
+          w[0] = round_to<T>(f * c[e] - g * s[e]);
+          w[1] = round_to<T>(g * c[e] + f * s[e]);
         }
       }
-      if (dst[i]) {
-        *reinterpret_cast<uint4 *>(dst[i] + at1) = x[i];
-        *reinterpret_cast<uint4 *>(dst[i] + at2) = y[i];
-      }
-      if (dst2[i]) {
-        *reinterpret_cast<uint4 *>(dst2[i] + at1) = x[i];
-        *reinterpret_cast<uint4 *>(dst2[i] + at2) = y[i];
-      }
     }
-    done += kAtOnce * lanes;
+    if (dst) {
+      *reinterpret_cast<uint4 *>(dst + at1) = x;
+      *reinterpret_cast<uint4 *>(dst + at2) = y;
+    }
+    if (dst2) {
+      *reinterpret_cast<uint4 *>(dst2 + at1) = x;
+      *reinterpret_cast<uint4 *>(dst2 + at2) = y;
+    }
   }
 }
 
@@ -282,9 +268,12 @@ cudaError_t launch(const RopeArgs &a, bool vec, cudaStream_t stream) {
   const long long heads = a.heads + (a.k ? a.kv_heads : 0) + (a.v ? a.kv_heads : 0);
   if (vec) {
     const long long lanes = kRopeThreads / (a.dim / (2 * (16 / static_cast<int>(sizeof(T)))));
-    // fewer heads a thread while that fills the GPU better (two blocks per SM)
+    // heads a thread: whole waves of the blocks that fit, none much longer than
+    // kHeadsPerThread (5001 rows of 48 heads: one wave of 11 each 26.8 us, 8 each 31)
     const long long all = a.num_tokens * heads;
-    const long long deep = std::max(1ll, std::min(all / (lanes * 296), 1ll * kHeadsPerThread));
+    const long long most = std::min(1ll * kHeadsPerThread, kBlockHeads / lanes);
+    const long long waves = (all + lanes * kResident * most - 1) / (lanes * kResident * most);
+    const long long deep = (all + lanes * kResident * waves - 1) / (lanes * kResident * waves);
     const long long per_block = lanes * deep;
     const long long blocks = (all + per_block - 1) / per_block;
     if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;

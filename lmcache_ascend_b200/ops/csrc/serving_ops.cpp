@@ -159,6 +159,9 @@ build_slot_mapping(const at::Tensor &context_lens, const at::Tensor &new_lens,
   a.batch = static_cast<int>(B);
   a.width = static_cast<int>(block_tables.size(1));
   a.block_size = static_cast<int>(block_size);
+  a.block_shift = -1;
+  for (int i = 0; i < 21; ++i)
+    if (block_size == (1ll << i)) a.block_shift = i;
   a.num_tokens = num_tokens;
   a.slots = slots.data_ptr();
   a.positions = positions.data_ptr();

@@ -18,7 +18,7 @@ struct SlotArgs {
   const int *free_blocks;   // [num_free], read when `grow`
   bool grow;                // take missing pages from free_blocks
   long long table_stride, num_free, num_blocks;
-  int batch, width, block_size;
+  int batch, width, block_size, block_shift;  // shift: log2 of the block size, or -1
   long long num_tokens;  // rows of the outputs
   void *slots, *positions;  // OT [num_tokens]
   int *request_ids;         // [num_tokens]

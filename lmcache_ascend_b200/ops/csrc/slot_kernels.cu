@@ -25,31 +25,38 @@ namespace lmc {
 namespace {
 
 constexpr int kSlotThreads = 512;
-constexpr int kTokensPerBlock = 2048;
+constexpr int kTokensPerBlock = 4096;
 
 enum SlotWhere : int { kWhereLength = 1, kWhereTable = 2, kWhereFree = 3, kWhereTotal = 4 };
 
 struct Need {
-  long long tokens, pages;
+  unsigned tokens, pages;
 };
 
-// Pages of `tokens` slots (< 2^32: two lengths below 2^31), in 32-bit divisions.
-__device__ __forceinline__ long long pages_of(long long tokens, int block_size) {
-  const unsigned t = static_cast<unsigned>(tokens), bs = static_cast<unsigned>(block_size);
-  return t / bs + (t % bs != 0);
+// Positions stay below 2^32 (two lengths below 2^31); a power of two, as block
+// sizes mostly are, takes a shift.
+__device__ __forceinline__ unsigned page_of(const SlotArgs &a, unsigned position) {
+  return a.block_shift >= 0 ? position >> a.block_shift
+                            : position / static_cast<unsigned>(a.block_size);
+}
+
+// Pages of `tokens` slots.
+__device__ __forceinline__ unsigned pages_of(const SlotArgs &a, unsigned tokens) {
+  const unsigned whole = page_of(a, tokens);
+  return whole + (tokens != whole * static_cast<unsigned>(a.block_size));
 }
 
 template <typename LT>
-__device__ __forceinline__ long long length_of(const void *p, int b) {
+__device__ __forceinline__ unsigned length_of(const void *p, int b) {
   const long long v = static_cast<long long>(static_cast<const LT *>(p)[b]);
   // a length below zero counts as zero; one past 2^31 - 1 as that
-  return v < 0 ? 0 : (v > 0x7fffffffll ? 0x7fffffffll : v);
+  return static_cast<unsigned>(v < 0 ? 0 : (v > 0x7fffffffll ? 0x7fffffffll : v));
 }
 
 template <typename LT>
 __device__ __forceinline__ Need need_of(const SlotArgs &a, int b) {
-  const long long c = length_of<LT>(a.ctx, b), n = length_of<LT>(a.fresh, b);
-  return {n, a.grow ? pages_of(c + n, a.block_size) - pages_of(c, a.block_size) : 0};
+  const unsigned c = length_of<LT>(a.ctx, b), n = length_of<LT>(a.fresh, b);
+  return {n, a.grow ? pages_of(a, c + n) - pages_of(a, c) : 0};
 }
 
 // Exclusive prefix of the request sums at each thread's segment of requests.
@@ -78,7 +85,9 @@ __global__ void __launch_bounds__(kSlotThreads) slot_mapping_kernel(SlotArgs a) 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int seg = (a.batch + kSlotThreads - 1) / kSlotThreads;
   const int b0 = min(a.batch, tid * seg), b1 = min(a.batch, b0 + seg);
-  Need mine = {0, 0};
+  struct {
+    long long tokens, pages;
+  } mine = {0, 0};
   for (int b = b0; b < b1; ++b) {
     const Need n = need_of<LT>(a, b);
     mine.tokens += n.tokens;
@@ -108,10 +117,10 @@ __global__ void __launch_bounds__(kSlotThreads) slot_mapping_kernel(SlotArgs a) 
     for (int b = b0; b < b1; ++b) {
       const Need n = need_of<LT>(a, b);
       if (b >= r0 && b < r1) {
-        const long long c = length_of<LT>(a.ctx, b);
+        const unsigned c = length_of<LT>(a.ctx, b);
         a.start[b] = static_cast<int>(t);
         a.taken[b] = static_cast<int>(p);
-        a.seq_lens[b] = static_cast<int>(min(c + n.tokens, 0x7fffffffll));
+        a.seq_lens[b] = static_cast<int>(min(c + n.tokens, 0x7fffffffu));
         if (static_cast<long long>(static_cast<const LT *>(a.ctx)[b]) != c ||
             static_cast<long long>(static_cast<const LT *>(a.fresh)[b]) != n.tokens)
           report_status(a.status, kStatusBadIndex, kWhereLength, b, 0);
@@ -143,8 +152,7 @@ __global__ void __launch_bounds__(kSlotThreads) slot_mapping_kernel(SlotArgs a) 
       p += n;
       n = need_of<LT>(a, ++b).pages;
     }
-    const long long c = length_of<LT>(a.ctx, b);
-    const long long col = pages_of(c, a.block_size) + (j - p);
+    const long long col = pages_of(a, length_of<LT>(a.ctx, b)) + (j - p);
     if (col < a.width)
       a.tables[b * a.table_stride + col] = j < a.num_free ? a.free_blocks[j] : -1;
     else
@@ -159,49 +167,51 @@ __global__ void __launch_bounds__(kSlotThreads) slot_mapping_kernel(SlotArgs a) 
       static_cast<long long>(blockIdx.x) * kTokensPerBlock + warp * (kTokensPerBlock / (kSlotThreads / 32));
   const long long t1 = min(a.num_tokens, t0 + kTokensPerBlock / (kSlotThreads / 32));
   if (t0 >= t1) return;
+  // (tokens and pages up to the last row of the outputs fit 32 bits)
   int b = 0;
-  long long start = 0, pages = 0, c = 0, have = 0;
+  unsigned start = 0, pages = 0, c = 0, have = 0;
   Need n = {0, 0};
   auto look_up = [&](int request) {
     b = request;
     c = length_of<LT>(a.ctx, b);
     n = need_of<LT>(a, b);
-    have = pages_of(c, a.block_size);
+    have = pages_of(a, c);
   };
   if (t0 < total_tokens) {
     const int g = last_leq(s.tokens, kSlotThreads, t0);
-    start = s.tokens[g], pages = s.pages[g];
+    start = static_cast<unsigned>(s.tokens[g]), pages = static_cast<unsigned>(s.pages[g]);
     look_up(g * seg);
   }
-  for (long long t = t0 + lane; t < t1; t += 32) {
-    if (t >= total_tokens) {  // rows behind the last request
+  const unsigned end = static_cast<unsigned>(min(t1, total_tokens));
+  for (unsigned t = static_cast<unsigned>(t0) + lane; t < static_cast<unsigned>(t1); t += 32) {
+    if (t >= end) {  // rows behind the last request
       slots[t] = -1;
       positions[t] = 0;
       a.request_ids[t] = -1;
       continue;
     }
-    while (t >= start + n.tokens) {
+    while (t - start >= n.tokens) {
       start += n.tokens;
       pages += n.pages;
       look_up(b + 1);
     }
-    const long long pos = c + (t - start);
-    const long long col = static_cast<unsigned>(pos) / static_cast<unsigned>(a.block_size);
-    long long page = -1;
-    if (col >= a.width) {
+    const unsigned pos = c + (t - start);
+    const unsigned col = page_of(a, pos);
+    int page = -1;
+    if (col >= static_cast<unsigned>(a.width)) {
       report_status(a.status, kStatusBadIndex, kWhereTable, b, col);
     } else if (a.grow && col >= have) {
-      const long long j = pages + (col - have);
+      const unsigned j = pages + (col - have);
       if (j < a.num_free) page = a.free_blocks[j];
     } else {
       page = a.tables[b * a.table_stride + col];
     }
-    long long slot = -1;
+    OT slot = -1;
     if (page >= 0 && page < a.num_blocks)
-      slot = page * a.block_size + (pos - col * a.block_size);
-    else if (col < a.width)
+      slot = static_cast<OT>(page) * a.block_size + static_cast<OT>(pos - col * a.block_size);
+    else if (col < static_cast<unsigned>(a.width))
       report_status(a.status, kStatusBadSlot, b, page, a.num_blocks);
-    slots[t] = static_cast<OT>(slot);
+    slots[t] = slot;
     positions[t] = static_cast<OT>(pos);
     a.request_ids[t] = b;
   }
