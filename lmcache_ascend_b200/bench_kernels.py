@@ -16,6 +16,8 @@ Cases (BASELINE shapes):
 * ``rope``: K re-rotation, 65536 tokens x 8 heads x 128.
 * ``c8``: DeepSeek-V3.2 indexer C8 cache <-> chunk packets, 61 layers.
 * ``push_loopback``: K9 on one GPU (Qwen3-32B TP4 shard, 16k tokens).
+* ``serving``: slot maps, rotary with cache writes, shared-prefix attention of a
+  Qwen3-32B decode batch, and CacheBlend's attention of recomputed rows.
 """
 
 from __future__ import annotations
@@ -360,7 +362,49 @@ def bench_push(small: bool):
     recv.check()
 
 
-CASES = {"gather": bench_gather_scatter, "offload": bench_offload, "cachegen": bench_cachegen,
+def bench_serving(small: bool):
+    from .ops import api
+    from .ops.reference import make_cos_sin_cache
+
+    H, KH, D, BS, B = 64, 8, 128, 16, 64
+    P, own = (2048, 128) if small else (16384, 512)
+    T = P
+    dt = torch.bfloat16
+    npb, nob = P // BS, own // BS
+    nb = npb + B * nob
+    kc = torch.randn(nb, BS, KH, D, device="cuda", dtype=dt)
+    vc = torch.randn(nb, BS, KH, D, device="cuda", dtype=dt)
+    ids = torch.randperm(nb, device="cuda").int()
+    tables = ids[npb:].view(B, nob).contiguous()
+    ctx = torch.full((B,), own - 1, device="cuda", dtype=torch.int32)
+    ms = _time(lambda: api.build_slot_mapping(ctx, torch.ones_like(ctx), tables, BS, B,
+                                              num_blocks=nb))
+    _emit("slot_mapping_decode", ms, B * 28, traffic_bytes=B * 28, batch=B)
+    qkv = torch.randn(T, (H + 2 * KH) * D, device="cuda", dtype=dt)
+    q, k, v = qkv.split([H * D, KH * D, KH * D], dim=1)
+    table = make_cos_sin_cache(T, D, 1e6).cuda()
+    pos = torch.arange(T, device="cuda")
+    slots = (ids[:npb].long()[pos // BS] * BS + pos % BS)
+    ms = _time(lambda: api.rotary_embedding_and_cache(pos, q, k, v, kc, vc, slots, D, table))
+    moved = qkv.numel() * 2
+    _emit("rotary_and_cache", ms, moved, tokens=T)
+    qd = torch.randn(B, H, D, device="cuda", dtype=dt)
+    lens = torch.full((B,), own, device="cuda", dtype=torch.int32)
+    ms = _time(lambda: api.shared_prefix_attention(qd, kc, vc, ids[:npb], P, tables, lens))
+    read = (P + B * own) * KH * D * 4
+    _emit("shared_prefix_attention", ms, read, traffic_bytes=read, batch=B, prefix=P, own=own,
+          tflops=round(4 * B * H * D * (P + own) / ms / 1e9, 1))
+    kk = torch.randn(T, 8, D, device="cuda", dtype=dt)
+    vv = torch.randn(T, 8, D, device="cuda", dtype=dt)
+    rows = torch.randperm(T, device="cuda")[:int(T * 0.15)].sort().values
+    qb = torch.randn(rows.numel(), 32, D, device="cuda", dtype=dt)
+    ms = _time(lambda: api.position_attention(qb, kk, vv, rows, pos))
+    _emit("position_attention", ms, kk.numel() * 4, traffic_bytes=kk.numel() * 4,
+          rows=rows.numel(), keys=T,
+          tflops=round(4 * 32 * D * float((rows + 1).sum()) / ms / 1e9, 1))
+
+
+CASES = {"serving": bench_serving, "gather": bench_gather_scatter, "offload": bench_offload, "cachegen": bench_cachegen,
          "cachegen_serde": bench_cachegen_serde,
          "rope": bench_rope, "c8": bench_c8, "push": bench_push}
 

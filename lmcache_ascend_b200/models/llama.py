@@ -22,6 +22,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from ..ops import api
 from ..ops.reference import make_cos_sin_cache
 
 
@@ -99,9 +100,12 @@ class DecoderLayer(nn.Module):
 
 class LlamaForBlend(nn.Module):
     def __init__(self, config: LlamaConfig, device="cpu", dtype=torch.float32, seed: int = 0,
-                 lm_head: bool = False):
+                 lm_head: bool = False, native_attention: bool = False):
         """Parameters are created on ``device`` in ``dtype`` (a 32B model is
-        built on the GPU directly) and drawn from N(0, 0.05^2)."""
+        built on the GPU directly) and drawn from N(0, 0.05^2).
+        ``native_attention``: prefill and blending rotate and attend with
+        ``ops.api.rotary_embedding`` / ``position_attention`` (on a GPU bf16 or
+        fp16 and head_dim 64 or 128) instead of PyTorch's."""
         super().__init__()
         torch.manual_seed(seed)
         if torch.device(device).type == "cuda":
@@ -124,6 +128,7 @@ class LlamaForBlend(nn.Module):
         self.head_size = config.head_dim
         self.device = torch.device(device)
         self.dtype = dtype
+        self.native_attention = native_attention
 
     # ---------------------------------------------------------------- rope
     def rope(self, positions: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
@@ -136,11 +141,15 @@ class LlamaForBlend(nn.Module):
         return torch.cat([x1 * cos - x2 * sin, x2 * cos + x1 * sin], dim=-1).to(x.dtype)
 
     def rotary_emb(self, positions, q, k):
+        if self.native_attention:
+            return api.rotary_embedding(positions, q, k, self.head_size, self.cos_sin_cache)
         return self.rope(positions, q), self.rope(positions, k)
 
     # ----------------------------------------------------------- attention
     def attend(self, q, k, v, q_pos, k_pos):
         """q [Tq, H, D] at q_pos; k, v [Tk, KH, D] at k_pos; causal by position."""
+        if self.native_attention:
+            return api.position_attention(q, k, v, q_pos, k_pos).reshape(q.shape[0], -1)
         c = self.config
         rep = c.num_heads // c.num_kv_heads
         kk = k.repeat_interleave(rep, dim=1)
@@ -204,6 +213,36 @@ class LlamaForBlend(nn.Module):
         if self.lm_head is None:
             return hs
         return self.lm_head(hs).argmax(dim=-1)
+
+    # ------------------------------------- decode of a batch on one prefix
+    @torch.no_grad()
+    def decode_batch(self, tokens: torch.Tensor, own_lens: torch.Tensor, kv_caches: List,
+                     block_tables: torch.Tensor, free_blocks: torch.Tensor,
+                     prefix_blocks: torch.Tensor, prefix_len: int, status=None):
+        """One new token for each request of a batch whose requests share a cached
+        prefix.  ``tokens`` [B]; ``own_lens`` (int32 [B]) tokens each request
+        already holds behind the prefix, in the blocks of its row of
+        ``block_tables`` (int32); blocks that the new tokens need come from
+        ``free_blocks`` and are written to the table.  Returns the greedy next
+        tokens [B] (the hidden states without ``lm_head``) and the step's
+        ``SlotMapping`` (``seq_lens``: own lengths after the step, ``taken[-1]``:
+        free blocks used).  No host synchronisation: the step can be captured."""
+        kc0 = kv_caches[0][0]
+        B = tokens.numel()
+        slots = api.build_slot_mapping(own_lens, torch.ones_like(own_lens), block_tables,
+                                       kc0.shape[1], B, free_blocks=free_blocks,
+                                       num_blocks=kc0.shape[0], status=status)
+        pos = slots.positions + prefix_len
+        h = self.embed_tokens(tokens.to(self.device))
+        for layer, (kc, vc) in zip(self.layers, kv_caches):
+            q, k, v = layer.qkv(h)
+            q = api.rotary_embedding_and_cache(pos, q, k, v, kc, vc, slots.slot_mapping,
+                                               self.head_size, self.cos_sin_cache, status=status)
+            o = api.shared_prefix_attention(q, kc, vc, prefix_blocks, prefix_len, block_tables,
+                                            slots.seq_lens, status=status)
+            h = layer.post(h, o.reshape(B, -1))
+        h = self.norm(h)
+        return (h if self.lm_head is None else self.lm_head(h).argmax(dim=-1)), slots
 
     # --------------------------------------------------- layerwise blending
     @torch.no_grad()

@@ -14,7 +14,10 @@ models/utils.py:15-64 ``infer_model_from_vllm`` / ``VLLMModelTracker``).
 Attention of the recomputed query rows over all key rows is causal by
 position (a query at position p sees keys at positions <= p), computed with
 ``scaled_dot_product_attention`` and grouped-query heads (reference
-blend/attention/attention.py:30-70, 150-190).
+blend/attention/attention.py:30-70, 150-190), or with
+``ops.api.position_attention`` when the engine's config sets
+``extra_config["blend_native_attention"]`` (no mask and no repeated heads in
+memory; bf16 or fp16 and head_dim 64 or 128).
 """
 
 from __future__ import annotations
@@ -26,6 +29,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from ...ops import api
 from ...utils.logging import init_logger
 
 logger = init_logger(__name__)
@@ -72,8 +76,10 @@ def _first(x):
 class LMCVLLMModel:
     """Layerwise blending forward over a vLLM decoder model's modules."""
 
-    def __init__(self, vllm_model: nn.Module, qk_norm: bool = False):
+    def __init__(self, vllm_model: nn.Module, qk_norm: bool = False,
+                 native_attention: bool = False):
         self.vllm_model = vllm_model
+        self.native_attention = native_attention
         inner = vllm_model.model
         start = getattr(inner, "start_layer", 0)
         end = getattr(inner, "end_layer", len(inner.layers))
@@ -120,6 +126,10 @@ class LMCVLLMModel:
     def attend(self, q, k, v, q_pos, k_pos) -> torch.Tensor:
         """q [Tq, H, D] at q_pos over k, v [Tk, KH, D] at k_pos, causal by
         position; returns [Tq, H * D]."""
+        if self.native_attention:
+            return api.position_attention(
+                q, k, v, q_pos, k_pos,
+                scale=getattr(self.layers[0].self_attn, "scaling", None)).reshape(q.shape[0], -1)
         c = self.config
         rep = c.num_heads // c.num_kv_heads
         mask = q_pos[:, None] >= k_pos[None, :]
@@ -168,13 +178,14 @@ class LMCVLLMModel:
         return _first(out)
 
 
-def infer_model_from_vllm(vllm_model: nn.Module) -> LMCVLLMModel:
+def infer_model_from_vllm(vllm_model: nn.Module,
+                          native_attention: bool = False) -> LMCVLLMModel:
     """The blending wrapper for a served vLLM model, chosen by class name."""
     name = type(vllm_model).__name__
     if name == "LlamaForCausalLM":
-        return LMCVLLMModel(vllm_model, qk_norm=False)
+        return LMCVLLMModel(vllm_model, qk_norm=False, native_attention=native_attention)
     if "Qwen3ForCausalLM" in name:
-        return LMCVLLMModel(vllm_model, qk_norm=True)
+        return LMCVLLMModel(vllm_model, qk_norm=True, native_attention=native_attention)
     raise NotImplementedError(f"CacheBlend does not support model type {name}")
 
 
@@ -200,7 +211,8 @@ def get_or_create_blender(instance_id: str, cache_engine, gpu_connector, config,
     if b is None:
         from .blender import LMCBlender
 
-        model = infer_model_from_vllm(VLLMModelTracker.get_model(instance_id))
+        model = infer_model_from_vllm(VLLMModelTracker.get_model(instance_id),
+                                      bool(config.extra_config.get("blend_native_attention")))
         b = _blenders[instance_id] = LMCBlender(cache_engine, gpu_connector, model, config,
                                                 kv_caches=_kv_pairs(kv_caches))
     return b
