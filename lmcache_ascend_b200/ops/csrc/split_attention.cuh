@@ -15,7 +15,7 @@
 
 namespace lmc {
 
-constexpr int kSplitWarps = 4, kSplitKeys = 16, kSplitRows = 16, kSplitStages = 3;
+constexpr int kSplitWarps = 4, kSplitKeys = 16, kSplitRows = 16, kSplitStages = 2;
 
 // Which keys and rows a pass covers.  Paged: prefix keys [pre_begin, pre_end),
 // then the own keys of the unit's request when `own`; a unit is a request, or all
@@ -93,8 +93,11 @@ __device__ __noinline__ void strict_paged_row(const PagedArgs &a, long long r) {
   row.finish(static_cast<T *>(a.out) + r * D, a.lse ? a.lse + r : nullptr);
 }
 
-template <typename T, int D, typename Args>
-__global__ void __launch_bounds__(kSplitWarps * 32, 2)
+// kShaped: a cap or a distance bias.  Three blocks per SM: twelve warps with a
+// stage each under way beat eight with two (64 requests on own keys of 64 to 1024,
+// 120 MB: 38 us so).
+template <typename T, int D, typename Args, bool kShaped>
+__global__ void __launch_bounds__(kSplitWarps * 32, 3)
     split_attention_kernel(const __grid_constant__ Args a, const __grid_constant__ SplitPass s) {
   constexpr bool kDense = __is_same(Args, PositionArgs);
   using L = SplitSmem<D>;
@@ -147,46 +150,49 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 2)
   const uint32_t ring_addr = smem_u32(ring);
   const int steps = (k1 - k0 + chunk - 1) / chunk;
 
-  // Pages (dense: indices) of the 16 keys of step `it` of this warp: lane i (and
-  // i + 16) key i; -1 where there is none.
-  auto key_page = [&](int it, int &off, bool &bad) -> int {
+  // Where the 16 keys of step `it` of this warp lie, in elements from the first:
+  // lane i (and i + 16) key i; -1 where there is none.
+  struct Place {
+    long long k, v;
+    bool bad;  // in a page outside the cache
+  };
+  auto place_of = [&](int it) -> Place {
     const int j = k0 + it * chunk + warp * kSplitKeys + (lane & 15);
-    bad = false;
-    off = 0;
-    if (j >= k1) return -1;
-    if constexpr (kDense) return j;
-    else {
-    const bool shared = j < pre;
-    const unsigned at = shared ? s.pre_begin + j : j - pre;
-    const unsigned col = at / static_cast<unsigned>(a.block_size);
-    off = static_cast<int>(at - col * a.block_size);
-    const int page = shared ? a.prefix_blocks[col] : a.tables[unit * a.table_stride + col];
-    if (page >= 0 && page < a.num_blocks) return page;
-    bad = true;
-    if (lane < 16) report_status(a.status, kStatusBadSlot, shared ? -1 : unit, col, page);
-    return -1;
+    if (j >= k1) return {-1, -1, false};
+    if constexpr (kDense) {
+      return {j * a.k_token, j * a.v_token, false};
+    } else {
+      const bool shared = j < pre;
+      const unsigned at = shared ? s.pre_begin + j : j - pre;
+      const unsigned col = at / static_cast<unsigned>(a.block_size);
+      const int off = static_cast<int>(at - col * a.block_size);
+      const int page = shared ? a.prefix_blocks[col] : a.tables[unit * a.table_stride + col];
+      if (page >= 0 && page < a.num_blocks)
+        return {page * a.k_block + off * a.k_slot, page * a.v_block + off * a.v_slot, false};
+      if (lane < 16) report_status(a.status, kStatusBadSlot, shared ? -1 : unit, col, page);
+      return {-1, -1, true};
     }
   };
-  auto load = [&](int it, int page, int off) {
+  const T *k_first = static_cast<const T *>(a.k) + kv * a.k_head + lane % kChunks * 8;
+  const T *v_first = static_cast<const T *>(a.v) + kv * a.v_head + lane % kChunks * 8;
+  bool alike;  // K and V rows lie at the same offsets
+  if constexpr (kDense)
+    alike = a.k_token == a.v_token;
+  else
+    alike = a.k_block == a.v_block && a.k_slot == a.v_slot;
+  auto load = [&](int it, const Place &p) {
     const uint32_t dst = ring_addr + (it % kSplitStages) * L::kStage;
     const int c = lane % kChunks;
     constexpr int kRowsAtOnce = 32 / kChunks;
 #pragma unroll
     for (int i = 0; i < kSplitKeys / kRowsAtOnce; ++i) {
       const int r = i * kRowsAtOnce + lane / kChunks;
-      const int pg = __shfl_sync(0xffffffffu, page, r), of = __shfl_sync(0xffffffffu, off, r);
-      const bool valid = pg >= 0;  // else zeros: nothing of the page is read
-      const long long p = valid ? pg : 0;
+      const long long ko = __shfl_sync(0xffffffffu, p.k, r);
+      const long long vo = alike ? ko : __shfl_sync(0xffffffffu, p.v, r);
+      const bool valid = ko >= 0;  // else zeros: nothing of the page is read
       const uint32_t at = r * (D * 2) + ((c & ~7) << 4) + (((c & 7) ^ (r & 7)) << 4);
-      const T *k = static_cast<const T *>(a.k) + kv * a.k_head + c * 8;
-      const T *v = static_cast<const T *>(a.v) + kv * a.v_head + c * 8;
-      if constexpr (kDense) {
-        k += p * a.k_token, v += p * a.v_token;
-      } else {
-        k += p * a.k_block + of * a.k_slot, v += p * a.v_block + of * a.v_slot;
-      }
-      cp_async16(dst + at, k, valid);
-      cp_async16(dst + L::kKeys + at, v, valid);
+      cp_async16(dst + at, k_first + (valid ? ko : 0), valid);
+      cp_async16(dst + L::kKeys + at, v_first + (valid ? vo : 0), valid);
     }
   };
 
@@ -194,20 +200,18 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 2)
   uint32_t bad_ring[kSplitStages];
 #pragma unroll
   for (int i = 0; i < kSplitStages; ++i) bad_ring[i] = 0;
-  int page, off;
-  bool bad;
+  Place next = {-1, -1, false};
 #pragma unroll
   for (int i = 0; i < kSplitStages - 1; ++i) {
     if (i < steps) {
-      page = key_page(i, off, bad);
-      bad_ring[i] = __ballot_sync(0xffffffffu, bad) & 0xffff;
-      load(i, page, off);
+      next = place_of(i);
+      bad_ring[i] = __ballot_sync(0xffffffffu, next.bad) & 0xffff;
+      load(i, next);
     }
     cp_async_commit();
   }
-  page = -1;
-  bad = false;
-  if (kSplitStages - 1 < steps) page = key_page(kSplitStages - 1, off, bad);
+  next = {-1, -1, false};
+  if (kSplitStages - 1 < steps) next = place_of(kSplitStages - 1);
 
   // Q as the A operand: row lane/4 (and + 8), columns 2 (lane % 4) of each 8.
   const int r0 = lane >> 2, r1 = r0 + 8, c0 = (lane & 3) * 2;
@@ -253,6 +257,13 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 2)
     place(r0, last0, at0);
     place(r1, last1, at1);
   }
+  // keys below this index, position and document are seen by all of the tile's rows
+  int all_last = 0, all_limit = 0;
+  if constexpr (kDense)
+    all_limit = __reduce_min_sync(0xffffffffu, min(r0 < rows ? mask0.limit : 2147483647,
+                                                   r1 < rows ? mask1.limit : 2147483647));
+  else
+    all_last = __reduce_min_sync(0xffffffffu, min(min(last0, last1), k1));
   // -slope times the distance between the row and pass key j
   auto bias = [&](bool second, int j, int kp) {
     if constexpr (kDense) {
@@ -288,14 +299,14 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 2)
       const int nx = it + kSplitStages - 1;
       __syncwarp();  // every lane is done with the stage that is filled next
       if (nx < steps) {
-        const uint32_t b = __ballot_sync(0xffffffffu, bad) & 0xffff;
+        const uint32_t b = __ballot_sync(0xffffffffu, next.bad) & 0xffff;
 #pragma unroll
         for (int i = 0; i < kSplitStages; ++i)
           if (nx % kSplitStages == i) bad_ring[i] = b;
-        load(nx, page, off);
+        load(nx, next);
       }
       cp_async_commit();
-      if (nx + 1 < steps) page = key_page(nx + 1, off, bad);
+      if (nx + 1 < steps) next = place_of(nx + 1);
     }
     const int kp_all = kp_next, kd_all = kd_next;
     if (it + 1 < steps) key_marks(it + 1);
@@ -318,33 +329,53 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 2)
 #pragma unroll
     for (int i = 0; i < kSplitStages; ++i)
       if (it % kSplitStages == i) bad_keys = bad_ring[i];
+    if constexpr (kShaped) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < 2; ++t) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int col = t * 8 + c0 + e, j = j0 + col;
-        bool out0 = j >= k1, out1 = out0;
-        int kp = 0;
-        if constexpr (kDense) {
-          kp = __shfl_sync(0xffffffffu, kp_all, col);
-          const int kd = __shfl_sync(0xffffffffu, kd_all, col);
-          out0 = out0 || kp >= mask0.limit || (a.k_doc && kd != mask0.doc);
-          out1 = out1 || kp >= mask1.limit || (a.k_doc && kd != mask1.doc);
-        } else {
-          const bool bad_key = (bad_keys >> col) & 1;
-          out0 = out0 || j >= last0 || bad_key;
-          out1 = out1 || j >= last1 || bad_key;
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float x = sc[t][2 * h + e];
+        for (int e = 0; e < 4; ++e) {
+          const int col = t * 8 + c0 + (e & 1);
+          float x = sc[t][e];
           if (cap_out > 0.f)
             x = fmaf(rcp(1.f + ex2(x * cap_in)), -2.f * cap_out, cap_out);
           else
             x *= scale;
-          if (a.slopes) x += bias(h == 1, j, kp);
-          if (h ? out1 : out0) x = -INFINITY;
-          sc[t][2 * h + e] = x;
+          const int kp = kDense ? __shfl_sync(0xffffffffu, kp_all, col) : 0;
+          if (a.slopes) x += bias(e >= 2, j0 + col, kp);
+          sc[t][e] = x;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[t][e] *= scale;
+    }
+    bool open;  // no key of this step is masked for any row
+    if constexpr (kDense)
+      open = j0 + kSplitKeys <= k1 && a.k_doc == nullptr &&
+             __reduce_max_sync(0xffffffffu, kp_all) < all_limit;
+    else
+      open = j0 + kSplitKeys <= all_last && bad_keys == 0;
+    if (!open) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int col = t * 8 + c0 + e, j = j0 + col;
+          bool out0 = j >= k1, out1 = out0;
+          if constexpr (kDense) {
+            const int kp = __shfl_sync(0xffffffffu, kp_all, col);
+            const int kd = __shfl_sync(0xffffffffu, kd_all, col);
+            out0 = out0 || kp >= mask0.limit || (a.k_doc && kd != mask0.doc);
+            out1 = out1 || kp >= mask1.limit || (a.k_doc && kd != mask1.doc);
+          } else {
+            const bool bad_key = (bad_keys >> col) & 1;
+            out0 = out0 || j >= last0 || bad_key;
+            out1 = out1 || j >= last1 || bad_key;
+          }
+          if (out0) sc[t][e] = -INFINITY;
+          if (out1) sc[t][2 + e] = -INFINITY;
         }
       }
     }
@@ -455,10 +486,10 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 2)
   wait_for_previous();
 }
 
-// Towards one wave of two blocks per SM, with 128 keys or more each: a block has
+// Towards one wave of three blocks per SM, with 128 keys or more each: a block has
 // a start and an end to pay whatever the length of its slice.
 inline int split_slices(long long blocks, long long keys) {
-  const long long want = std::min(296 / std::max(1ll, blocks), (keys + 127) / 128);
+  const long long want = std::min(444 / std::max(1ll, blocks), (keys + 127) / 128);
   return static_cast<int>(std::max(1ll, std::min(want, 64ll)));
 }
 
@@ -466,11 +497,13 @@ template <typename T, int D, typename Args>
 cudaError_t launch_split(const Args &a, const SplitPass &s, long long units, bool first,
                          cudaStream_t stream) {
   constexpr int kBytes = SplitSmem<D>::kBytes;
-  cudaError_t e = allow_smem(split_attention_kernel<T, D, Args>, kBytes);
+  auto kernel = a.softcap > 0.f || a.slopes != nullptr
+                    ? split_attention_kernel<T, D, Args, true>
+                    : split_attention_kernel<T, D, Args, false>;
+  cudaError_t e = allow_smem(kernel, kBytes);
   if (e != cudaSuccess) return e;
   const dim3 grid(static_cast<unsigned>(units * s.row_tiles * a.kv_heads), s.slices);
-  return launch_ordered(split_attention_kernel<T, D, Args>, grid, kSplitWarps * 32, kBytes, first,
-                        stream, a, s);
+  return launch_ordered(kernel, grid, kSplitWarps * 32, kBytes, first, stream, a, s);
 }
 
 template <typename T, int D>
