@@ -625,14 +625,9 @@ def rotary_embedding(positions: torch.Tensor, query: torch.Tensor,
     A position outside the table gives a zero row and is reported in ``status``.
     """
     if query.is_cuda:
-        if query_out is None:
-            query_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-        if key is not None and key_out is None:
-            key_out = torch.empty(key.shape, dtype=key.dtype, device=key.device)
-        native().rotary_embedding_and_cache(positions, query, key, None, None, None, None,
-                                            head_size, cos_sin_cache, is_neox, query_out, key_out,
-                                            status)
-        return query_out, key_out
+        return native().rotary_embedding_and_cache(
+            positions, query, key, None, None, None, None, head_size, cos_sin_cache, is_neox,
+            query_out, key_out, True, status)
 
     def turn(x, out):
         if x is None:
@@ -660,12 +655,9 @@ def rotary_embedding_and_cache(positions: torch.Tensor, query: torch.Tensor, key
     the cache, or a position outside the table, writes nothing to the pages and
     is reported in ``status``."""
     if query.is_cuda:
-        if query_out is None:
-            query_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-        native().rotary_embedding_and_cache(positions, query, key, value, key_cache, value_cache,
-                                            slot_mapping, head_size, cos_sin_cache, is_neox,
-                                            query_out, key_out, status)
-        return query_out
+        return native().rotary_embedding_and_cache(
+            positions, query, key, value, key_cache, value_cache, slot_mapping, head_size,
+            cos_sin_cache, is_neox, query_out, key_out, False, status)[0]
     q, k = rotary_embedding(positions, query, key, head_size, cos_sin_cache, is_neox, query_out,
                             key_out)
     for rows, cache in ((k, key_cache), (value, value_cache)):

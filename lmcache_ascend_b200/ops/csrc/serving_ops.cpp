@@ -1,6 +1,7 @@
 // Host side of the serving operators: argument checks, outputs and launches.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <algorithm>
@@ -31,6 +32,12 @@ DeviceStatus *checked_status(const c10::optional<at::Tensor> &status, const char
                   status->nbytes() >= kDeviceStatusBytes,
               op, ": status must be a contiguous tensor of >= 24 bytes on ", dev.str());
   return reinterpret_cast<DeviceStatus *>(status->data_ptr());
+}
+
+// A dense tensor on the device (without the dispatcher: a decode step's call
+// is mostly such overhead).
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const c10::Device &dev) {
+  return at::detail::empty_cuda(sizes, dtype, dev, c10::nullopt);
 }
 
 RowType row_type(at::ScalarType t) {
@@ -141,12 +148,11 @@ build_slot_mapping(const at::Tensor &context_lens, const at::Tensor &new_lens,
     TORCH_CHECK(free_blocks->dim() == 1, op, ": free_blocks must be [free]");
   }
   const c10::cuda::CUDAGuard guard(dev);
-  const auto opt = context_lens.options();
-  const auto it = opt.dtype(at::kInt);
-  const auto ot = opt.dtype(long_slots ? at::kLong : at::kInt);
-  auto slots = at::empty({num_tokens}, ot), positions = at::empty({num_tokens}, ot);
-  auto request_ids = at::empty({num_tokens}, it);
-  auto start = at::empty({B + 1}, it), seq_lens = at::empty({B}, it), taken = at::empty({B + 1}, it);
+  const auto slot_type = long_slots ? at::kLong : at::kInt;
+  auto slots = fresh({num_tokens}, slot_type, dev), positions = fresh({num_tokens}, slot_type, dev);
+  auto request_ids = fresh({num_tokens}, at::kInt, dev);
+  auto start = fresh({B + 1}, at::kInt, dev), seq_lens = fresh({B}, at::kInt, dev);
+  auto taken = fresh({B + 1}, at::kInt, dev);
   SlotArgs a;
   a.ctx = context_lens.data_ptr();
   a.fresh = new_lens.data_ptr();
@@ -175,18 +181,26 @@ build_slot_mapping(const at::Tensor &context_lens, const at::Tensor &new_lens,
   return {slots, positions, request_ids, start, seq_lens, taken};
 }
 
-// q_out = rotated q; the rotated k goes to k_out (optional) and, with caches and
-// a slot map, k and v go to their pages.
-void rotary_embedding_and_cache(
+// Returns q rotated and, when asked for, k rotated, in the given tensors or new
+// ones; with caches and a slot map k and v go to their pages.
+std::tuple<at::Tensor, c10::optional<at::Tensor>> rotary_embedding_and_cache(
     const at::Tensor &positions, const at::Tensor &query, const c10::optional<at::Tensor> &key,
     const c10::optional<at::Tensor> &value, const c10::optional<at::Tensor> &key_cache,
     const c10::optional<at::Tensor> &value_cache, const c10::optional<at::Tensor> &slot_mapping,
-    int64_t head_size, const at::Tensor &cos_sin_cache, bool is_neox, at::Tensor &query_out,
-    const c10::optional<at::Tensor> &key_out, const c10::optional<at::Tensor> &status) {
+    int64_t head_size, const at::Tensor &cos_sin_cache, bool is_neox,
+    const c10::optional<at::Tensor> &given_query_out,
+    const c10::optional<at::Tensor> &given_key_out, bool new_key_out,
+    const c10::optional<at::Tensor> &status) {
   const char *op = "rotary_embedding";
   TORCH_CHECK(query.is_cuda(), op, ": query must be on the device");
   const c10::Device dev = query.device();
   const auto dt = query.scalar_type();
+  const c10::cuda::CUDAGuard guard(dev);
+  const at::Tensor query_out =
+      given_query_out.has_value() ? *given_query_out : fresh(query.sizes(), dt, dev);
+  c10::optional<at::Tensor> key_out = given_key_out;
+  if (!key_out.has_value() && new_key_out && key.has_value())
+    key_out = fresh(key->sizes(), dt, dev);
   const int64_t D = head_size;
   TORCH_CHECK(D >= 1 && D <= 65536, op, ": bad head_size ", D);
   TORCH_CHECK(dt == at::kBFloat16 || dt == at::kHalf || dt == at::kFloat, op,
@@ -273,15 +287,15 @@ void rotary_embedding_and_cache(
   a.rot = static_cast<int>(rot);
   a.neox = is_neox;
   a.status = checked_status(status, op, dev);
-  if (T == 0 || a.heads + a.kv_heads == 0) return;
+  if (T == 0 || a.heads + a.kv_heads == 0) return {query_out, key_out};
   const int64_t es = query.element_size(), cs = cos_sin_cache.element_size();
   // 16-byte units: whole pairs of vectors in the head and in its rotated part,
   // and table rows whose halves start on 16 bytes
   vec = vec && D * es % 32 == 0 && D * es <= 32 * 256 && rot * es % 32 == 0 && rot / 2 * cs % 16 == 0 &&
         16 / es * cs % 16 == 0 && reinterpret_cast<uintptr_t>(a.table) % 16 == 0;
-  const c10::cuda::CUDAGuard guard(dev);
   C10_CUDA_CHECK(launch_rope_cache(a, row_type(dt), row_type(cos_sin_cache.scalar_type()), vec,
                                    at::cuda::getCurrentCUDAStream().stream()));
+  return {query_out, key_out};
 }
 
 std::tuple<at::Tensor, c10::optional<at::Tensor>> shared_prefix_attention(
@@ -326,10 +340,10 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> shared_prefix_attention(
   TORCH_CHECK(B * Tq * H <= 0x7fffffff, op, ": too many rows");
   const c10::cuda::CUDAGuard guard(dev);
   const at::Tensor q = with_vector_rows(q4);
-  auto out = at::empty(query.sizes(), query.options().memory_format(at::MemoryFormat::Contiguous));
+  auto out = fresh(query.sizes(), dt, dev);
   c10::optional<at::Tensor> lse;
   if (return_lse)
-    lse = at::empty(query.sizes().slice(0, query.dim() - 1), query.options().dtype(at::kFloat));
+    lse = fresh(query.sizes().slice(0, query.dim() - 1), at::kFloat, dev);
   if (B * H == 0) return {out, lse};
   PagedArgs a = {};
   a.q = q.data_ptr(), a.k = key_cache.data_ptr(), a.v = value_cache.data_ptr();
@@ -351,8 +365,8 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> shared_prefix_attention(
   a.width = static_cast<int>(block_tables.size(1));
   a.scale = static_cast<float>(scale), a.softcap = static_cast<float>(softcap);
   a.status = checked_status(status, op, dev);
-  const auto workspace = at::empty({shared_prefix_attention_workspace(a, static_cast<int>(D))},
-                                   query.options().dtype(at::kByte));
+  const auto workspace =
+      fresh({shared_prefix_attention_workspace(a, static_cast<int>(D))}, at::kByte, dev);
   C10_CUDA_CHECK(launch_shared_prefix_attention(a, row_type(dt), static_cast<int>(D),
                                                 workspace.data_ptr(),
                                                 at::cuda::getCurrentCUDAStream().stream()));
@@ -401,9 +415,9 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> position_attention(
   const at::Tensor q = with_vector_rows(query);
   const at::Tensor k = with_vector_rows(key);
   const at::Tensor v = with_vector_rows(value);
-  auto out = at::empty({Tq, H, D}, query.options());
+  auto out = fresh({Tq, H, D}, dt, dev);
   c10::optional<at::Tensor> lse;
-  if (return_lse) lse = at::empty({Tq, H}, query.options().dtype(at::kFloat));
+  if (return_lse) lse = fresh({Tq, H}, at::kFloat, dev);
   if (Tq == 0) return {out, lse};
   if (Tk == 0) {
     out.zero_();
@@ -429,8 +443,8 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> position_attention(
   a.heads = static_cast<int>(H), a.kv_heads = static_cast<int>(KH);
   a.causal = causal;
   a.scale = static_cast<float>(scale), a.softcap = static_cast<float>(softcap);
-  const auto workspace = at::empty({position_attention_workspace(a, static_cast<int>(D))},
-                                   query.options().dtype(at::kByte));
+  const auto workspace =
+      fresh({position_attention_workspace(a, static_cast<int>(D))}, at::kByte, dev);
   C10_CUDA_CHECK(launch_position_attention(a, row_type(dt), static_cast<int>(D),
                                            workspace.data_ptr(),
                                            at::cuda::getCurrentCUDAStream().stream()));
