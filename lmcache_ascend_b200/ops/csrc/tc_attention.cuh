@@ -8,7 +8,8 @@
 //   P = exp2(S c - m)    two threads per row, 64 keys each: S from TMEM to
 //                        registers, running maximum m (common) and sum l (of
 //                        each), P as 16-bit back over S in TMEM
-//   O = O + P V          tcgen05, P from TMEM, V as it lies (MN-major)
+//   O = O + P V          tcgen05, P from TMEM, V as it lies (MN-major); begun
+//                        when half of P is there
 // While one tile's scores are in the registers the tensor cores work on the
 // other's.  m only moves when the maximum grows by more than 2^8, so O in TMEM
 // is seldom rescaled (by the thread that owns the row; P stays below 2^8 and
@@ -263,7 +264,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       (reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBars);
   uint64_t *kv_full = bars, *kv_empty = bars + kStages, *s_full = bars + 2 * kStages,
-           *p_full = s_full + 2, *o_done = p_full + 2, *q_full = o_done + 2, *drain = q_full + 1;
+           *p_full = s_full + 2, *o_done = p_full + 2, *p_half = o_done + 2, *q_full = p_half + 2,
+           *drain = q_full + 1;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
   int *stopped = reinterpret_cast<int *>(tmem_slot + 1);
   int *seen = stopped + 1;  // limits and documents of the block's rows
@@ -289,7 +291,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     prefetch_map(&k_map), prefetch_map(&v_map);
     for (int i = 0; i < kStages; ++i) mbar_init(&kv_full[i], 1), mbar_init(&kv_empty[i], 1);
     for (int i = 0; i < 2; ++i)
-      mbar_init(&s_full[i], 1), mbar_init(&p_full[i], kTileThreads), mbar_init(&o_done[i], 1);
+      mbar_init(&s_full[i], 1), mbar_init(&p_half[i], kTileThreads),
+          mbar_init(&p_full[i], kTileThreads), mbar_init(&o_done[i], 1);
     mbar_init(q_full, kTileThreads * tiles);
     mbar_init(drain, 1);
     *stopped = 0;
@@ -403,12 +406,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       mma_commit(&s_full[t]);
     };
-    auto weigh = [&](int t, int st, bool accumulate) {
+    // keys 0-31 and 64-95 of a tile (part 0), or the others (part 1)
+    auto weigh = [&](int t, int st, int part, bool accumulate) {
 #pragma unroll
-      for (int k = 0; k < kTileN / 16; ++k)
+      for (int i = 0; i < 4; ++i) {
+        const int k = (i >> 1) * 4 + part * 2 + (i & 1);
         mma_ts(tmem + 2 * kTileN + t * D, tmem + t * kTileN + k * 8,
                smem_desc(kv_addr + st * L::kTile + k * 2048, kHalfBytes, 1024), kPV,
-               accumulate || k > 0);
+               accumulate || i > 0);
+      }
     };
     // One thread waits and issues: a vote per wait would cost as much as an mma.
     const int n = scan.count();
@@ -434,10 +440,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (t >= tiles) break;
-          ok = ok && lane_wait(&p_full[t], j & 1, stopped);
+          ok = ok && lane_wait(&p_half[t], j & 1, stopped);
           if (!ok) break;
           tc_fence_after();
-          weigh(t, v_st, j > 0);
+          weigh(t, v_st, 0, j > 0);
+          ok = lane_wait(&p_full[t], j & 1, stopped);
+          if (!ok) break;
+          tc_fence_after();
+          weigh(t, v_st, 1, true);
           if (more) score(t, k_st);
           if (t == tiles - 1) {
             mma_commit(&kv_empty[v_st]);
@@ -638,12 +648,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const float off = (m == -INFINITY ? 0.f : m) - lift;
       const f32x2 c2 = pack2(c, c), off2 = pack2(-off, -off);
       f32x2 l0 = pack2(0.f, 0.f), l1 = l0;
-      // the weights, some of them by the polynomial
-      auto weights = [&](auto some_fma) {
-        uint32_t p[32];
+      // the weights of 32 keys, some of them by the polynomial; the product may
+      // start with the first 32
+      auto weights = [&](int part, auto some_fma) {
+        uint32_t p[16];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const f32x2 v = fma2(pack2(s[2 * i], s[2 * i + 1]), c2, off2);
+        for (int i = 0; i < 16; ++i) {
+          const int k = part * 32 + 2 * i;
+          const f32x2 v = fma2(pack2(s[k], s[k + 1]), c2, off2);
           float e, f;
           if (decltype(some_fma)::value && i % 8 >= 8 - kFmaOf8) {
             exp2_fma(v, e, f);
@@ -657,18 +669,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             l0 = add2(l0, pack2(e, f));
           p[i] = pair_from_float<T>(e, f);
         }
-        tmem_st32(s_addr + half * (kKeys / 2), p);
+        tmem_st16(s_addr + half * (kKeys / 2) + part * 16, p);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(part == 0 ? &p_half[x] : &p_full[x]);
       };
       if (whole)
-        weights(Yes{});
+        weights(0, Yes{}), weights(1, Yes{});
       else
-        weights(No{});
+        weights(0, No{}), weights(1, No{});
       float u0, u1;
       unpack2(add2(l0, l1), u0, u1);
       l += u0 + u1;
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(&p_full[x]);
       ++j;
     }
     // ------------------------------------------------------------- result
