@@ -81,16 +81,24 @@ struct TcSmem {
   static constexpr int kBytes = kRowAt + 1024 + 1024;  // + alignment to the swizzle's 1 KB
 };
 
-// True in all threads of a row tile if it is in any of them.
-__device__ __forceinline__ bool tile_any(int tile, bool v) {
+// True in all of `kThreads` threads that meet at a barrier if it is in any of them.
+template <int kThreads>
+__device__ __forceinline__ bool any_of(int barrier, bool v) {
   uint32_t r;
   asm volatile(
       "{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\n"
       "barrier.cta.red.or.pred q, %2, %3, p;\nselp.u32 %0, 1, 0, q;\n}"
       : "=r"(r)
-      : "r"(v ? 1u : 0u), "r"(1 + tile), "n"(kTileThreads)
+      : "r"(v ? 1u : 0u), "r"(barrier), "n"(kThreads)
       : "memory");
   return r != 0;
+}
+// The threads of a row tile, and the two warps that share 32 of its rows.
+__device__ __forceinline__ bool tile_any(int tile, bool v) {
+  return any_of<kTileThreads>(1 + tile, v);
+}
+__device__ __forceinline__ bool pair_any(int tile, int rows, bool v) {
+  return any_of<64>(3 + tile * 4 + rows, v);
 }
 
 struct RowRef {
@@ -620,10 +628,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       t1 = fmaxf(fmaxf(t1, s[kKeys - 2]), s[kKeys - 1]);
       const float top = fmaf(fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)), c, lift);
       // O is rescaled when a row's maximum has grown (also at its first finite
-      // score), by both of its threads alike
-      if (tile_any(x, top > m + kLazy || !ok)) {
+      // score), by both of its threads alike.  The meeting also keeps a warp from
+      // writing weights over scores that the other has not read.
+      if (pair_any(x, warp & 3, top > m + kLazy || !ok)) {
         *mine = top;
-        if (tile_any(x, !ok)) {
+        if (pair_any(x, warp & 3, !ok)) {
           ok = false;
           break;
         }
