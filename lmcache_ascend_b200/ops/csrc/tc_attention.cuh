@@ -16,7 +16,8 @@
 // sums are fp32, so nothing is lost).
 //
 // Roles: warps 0-7 and 8-15 one row tile each, warp 16 issues the mma, warp 17
-// the TMA loads through a ring of four 128-key stages (K and V alternate); they
+// the TMA loads through a ring of two stages, each with the K of a tile and the V
+// of the one before, which one turn of the mma loop uses (one wait for both); they
 // give registers to the others (640 threads x 96 at launch = 512 x 112 + 128 x
 // 32).  Eight warps a tile, because a tile's chain (scores, weights, product,
 // next scores) is bound by the latency of the weights: with a thread per row
@@ -29,7 +30,7 @@
 namespace lmc {
 
 constexpr int kTileM = 128, kTileN = 128, kBlockRows = 256;
-constexpr int kStages = 4;
+constexpr int kStages = 2;  // of a key tile's K and the V of the tile before it
 constexpr int kTcThreads = 640, kMmaWarp = 16, kLoadWarp = 17;
 constexpr int kTileThreads = 256;  // of one row tile: two per row
 struct Yes { static constexpr bool value = true; };
@@ -73,8 +74,8 @@ struct TcSmem {
   static constexpr int kTile = kTileN * D * 2;
   static constexpr int kQ = 0;  // two row tiles; at the end their results pass through
   static constexpr int kQTile = kTileM * 256;
-  static constexpr int kKV = 2 * kQTile;             // kStages key tiles
-  static constexpr int kBars = kKV + kStages * kTile;
+  static constexpr int kKV = 2 * kQTile;             // kStages times K, V
+  static constexpr int kBars = kKV + kStages * 2 * kTile;
   static constexpr int kXch = kBars + 256;    // two floats per row
   static constexpr int kQAt = kXch + 2048;    // where each row's query lies
   static constexpr int kRowAt = kQAt + 2048;  // and its result, -1 behind the last row
@@ -365,36 +366,40 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp == kLoadWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
     // ------------------------------------------------------------- loader
-    int tile, it = 0;
-    bool whole, ok = true;
+    int tile = 0, before = -1, it = 0;
+    bool whole, ok = true, more = true;
     const int boxes = kDense ? 1 : max(1, kTileN / a.block_size);
-    while (ok && scan.next(tile, whole)) {
-#pragma unroll 1
-      for (int kv = 0; kv < 2; ++kv, ++it) {
-        const int st = it % kStages;
-        if (it >= kStages) ok = wait_or_stop(&kv_empty[st], (it / kStages - 1) & 1, stopped);
-        if (!ok) break;
-        uint8_t *dst = smem + L::kKV + st * L::kTile;
-        const CUtensorMap *map = kv ? &v_map : &k_map;
-        if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], L::kTile);
-        __syncwarp();
-        if (kDense) {
-          if (lane < kHalves)
-            tma_load_3d(dst + lane * kHalfBytes, map, lane * 64, kv_head, tile * kTileN,
-                        &kv_full[st]);
-        } else if (lane < boxes) {
-          // a page, or 128 slots of a larger one; an id outside the cache reads zeros
-          const int box_rows = min(kTileN, a.block_size);
-          const int j = tile * kTileN + lane * box_rows;
-          const int col = j / a.block_size;
-          int page = a.pages[col];
-          if (page < 0 || page >= a.num_blocks) page = a.num_blocks;
+    auto fetch = [&](uint8_t *dst, const CUtensorMap *map, int of, uint64_t *bar) {
+      if (kDense) {
+        if (lane < kHalves)
+          tma_load_3d(dst + lane * kHalfBytes, map, lane * 64, kv_head, of * kTileN, bar);
+      } else if (lane < boxes) {
+        // a page, or 128 slots of a larger one; an id outside the cache reads zeros
+        const int box_rows = min(kTileN, a.block_size);
+        const int j = of * kTileN + lane * box_rows;
+        const int col = j / a.block_size;
+        int page = a.pages[col];
+        if (page < 0 || page >= a.num_blocks) page = a.num_blocks;
 #pragma unroll
-          for (int h = 0; h < kHalves; ++h)
-            tma_load_4d(dst + h * kHalfBytes + lane * box_rows * 128, map, h * 64, kv_head,
-                        j - col * a.block_size, page, &kv_full[st]);
-        }
+        for (int h = 0; h < kHalves; ++h)
+          tma_load_4d(dst + h * kHalfBytes + lane * box_rows * 128, map, h * 64, kv_head,
+                      j - col * a.block_size, page, bar);
       }
+    };
+    while (more) {
+      more = scan.next(tile, whole);
+      if (!more && before < 0) break;  // no tiles
+      const int st = it % kStages;
+      if (it >= kStages) ok = wait_or_stop(&kv_empty[st], (it / kStages - 1) & 1, stopped);
+      if (!ok) break;
+      uint8_t *dst = smem + L::kKV + st * 2 * L::kTile;
+      if (lane == 0)
+        mbar_arrive_expect_tx(&kv_full[st], (more ? L::kTile : 0) + (before >= 0 ? L::kTile : 0));
+      __syncwarp();
+      if (more) fetch(dst, &k_map, tile, &kv_full[st]);
+      if (before >= 0) fetch(dst + L::kTile, &v_map, before, &kv_full[st]);
+      before = tile;
+      ++it;
     }
     // loads in flight land before the block's memory is given back
     for (int i = max(0, it - kStages); i < it; ++i)
@@ -410,7 +415,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int k = 0; k < D / 16; ++k) {
         const uint32_t off = (k >> 2) * kHalfBytes + (k & 3) * 32;
         mma_ss(tmem + t * kTileN, smem_desc(q_addr + t * L::kQTile + off, 16, 1024),
-               smem_desc(kv_addr + st * L::kTile + off, 16, 1024), kQK, k > 0);
+               smem_desc(kv_addr + st * 2 * L::kTile + off, 16, 1024), kQK, k > 0);
       }
       mma_commit(&s_full[t]);
     };
@@ -420,7 +425,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int i = 0; i < 4; ++i) {
         const int k = (i >> 1) * 4 + part * 2 + (i & 1);
         mma_ts(tmem + 2 * kTileN + t * D, tmem + t * kTileN + k * 8,
-               smem_desc(kv_addr + st * L::kTile + k * 2048, kHalfBytes, 1024), kPV,
+               smem_desc(kv_addr + (st * 2 + 1) * L::kTile + k * 2048, kHalfBytes, 1024), kPV,
                accumulate || i > 0);
       }
     };
@@ -437,34 +442,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           mma_commit(&kv_empty[0]);
         }
       }
-      int v_st = 1, v_phase = 0;
+      int st = 1, phase = 0;  // of V_j and K_{j + 1}
 #pragma unroll 1
       for (int j = 0; ok && j < n; ++j) {
         const bool more = j + 1 < n;
-        int k_st = v_st + 1, k_phase = v_phase;
-        if (k_st == kStages) k_st = 0, k_phase ^= 1;
-        ok = lane_wait(&kv_full[v_st], v_phase, stopped);
-        if (ok && more) ok = lane_wait(&kv_full[k_st], k_phase, stopped);
+        ok = lane_wait(&kv_full[st], phase, stopped);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (t >= tiles) break;
           ok = ok && lane_wait(&p_half[t], j & 1, stopped);
           if (!ok) break;
           tc_fence_after();
-          weigh(t, v_st, 0, j > 0);
+          weigh(t, st, 0, j > 0);
           ok = lane_wait(&p_full[t], j & 1, stopped);
           if (!ok) break;
           tc_fence_after();
-          weigh(t, v_st, 1, true);
-          if (more) score(t, k_st);
-          if (t == tiles - 1) {
-            mma_commit(&kv_empty[v_st]);
-            if (more) mma_commit(&kv_empty[k_st]);
-          }
+          weigh(t, st, 1, true);
+          if (more) score(t, st);
+          if (t == tiles - 1) mma_commit(&kv_empty[st]);
           if (!more) mma_commit(&o_done[t]);
         }
-        v_st = k_st + 1, v_phase = k_phase;
-        if (v_st == kStages) v_st = 0, v_phase ^= 1;
+        if (++st == kStages) st = 0, phase ^= 1;
       }
       if (!ok) {  // only after a wait that ran out: let the mma in flight end
         mma_commit(drain);
