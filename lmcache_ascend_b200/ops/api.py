@@ -665,6 +665,13 @@ def rotary_embedding_and_cache(positions: torch.Tensor, query: torch.Tensor, key
     return q
 
 
+def _check_scores(scale, softcap):
+    if not 0 < scale < float("inf"):
+        raise ValueError("scale must be positive and finite")
+    if not 0 <= softcap < float("inf"):
+        raise ValueError("softcap must be >= 0 (0: none)")
+
+
 def _attention_result(query, out, lse, return_lse):
     out = out.to(query.dtype)
     return (out, lse.float()) if return_lse else out
@@ -703,6 +710,7 @@ def shared_prefix_attention(query: torch.Tensor, key_cache: torch.Tensor,
             query, key_cache, value_cache, prefix_blocks, prefix_len, block_tables, seq_lens,
             scale, softcap, alibi_slopes, return_lse, status)
         return (out, lse) if return_lse else out
+    _check_scores(scale, softcap)
     if query.dim() not in (3, 4) or query.shape[-2] % key_cache.shape[2]:
         raise ValueError("query must be [B, H, D] or [B, q_len, H, D] with whole head groups")
     if prefix_len < 0 or prefix_blocks.numel() * key_cache.shape[1] < prefix_len:
@@ -726,7 +734,8 @@ def position_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
     CacheBlend recomputes over the blended keys, or packed documents.
 
     ``query`` [Tq, H, D] at ``q_positions``; ``key`` / ``value`` [Tk, KV heads, D]
-    at ``k_positions`` (int32 or int64; default 0, 1, 2, ...), in any order.  A
+    at ``k_positions`` (int32 or int64, within 32 bits; default 0, 1, 2, ...), in
+    any order.  A
     row sees a key when the key's position is at most its own (unless not
     ``causal``) or below its ``q_prefix_lens`` (int32 [Tq]), and, with
     ``q_documents`` / ``k_documents`` (int32), both are in the same document;
@@ -744,6 +753,7 @@ def position_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
             query, key, value, q_positions, k_positions, scale, softcap, alibi_slopes,
             q_documents, k_documents, q_prefix_lens, causal, return_lse)
         return (out, lse) if return_lse else out
+    _check_scores(scale, softcap)
     if query.dim() != 3 or key.dim() != 3 or query.shape[1] % key.shape[1]:
         raise ValueError("query [Tq, H, D] and key [Tk, KV heads, D] with whole head groups")
     if (q_documents is None) != (k_documents is None):

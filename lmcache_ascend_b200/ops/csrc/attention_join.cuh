@@ -3,6 +3,7 @@
 // with o_s normalised in its slice and L_s the base-2 log of its sum.  One warp
 // per row, fp32.
 #pragma once
+#include <algorithm>
 #include <mutex>
 #include <set>
 #include <utility>
@@ -82,16 +83,15 @@ inline void set_scores(TcArgs &t, float scale, float softcap) {
   t.scale_log2 = scale * kLog2e;
   t.cap_out = softcap * kLog2e;
   const double u = softcap > 0.f ? static_cast<double>(scale) / softcap : 0.;
+  t.cap_u = static_cast<float>(u);
   t.cap_in = static_cast<float>(2. * kLog2e * u);
   // tanh(u) / u for |u| <= 0.6 in powers of u^2 (relative minimax by the Remez
-  // exchange, degree 4: 7.3e-8), as x / s in powers of s^2.  The powers of a cap
-  // that is very wide for its scale leave the fp32 range: it takes the general form.
+  // exchange, degree 4: 7.3e-8), times the score's scale
   constexpr double kRatio[5] = {0.9999999268689601, -0.33332309974406227, 0.13310173658056346,
                                 -0.0521014801204608, 0.015475427495065024};
-  double f = static_cast<double>(scale) * kLog2e;
-  for (int i = 0; i < 5; ++i, f *= u * u)
-    t.cap_poly[i].x = t.cap_poly[i].y = static_cast<float>(kRatio[i] * f);
-  t.cap_small = u >= 1e-4 ? static_cast<float>(0.6 / u) : -1.f;
+  for (int i = 0; i < 5; ++i)
+    t.cap_poly[i].x = t.cap_poly[i].y = static_cast<float>(kRatio[i] * scale * kLog2e);
+  t.cap_small = static_cast<float>(0.6 / std::max(u, 1e-37));
 }
 
 // Lets a kernel use `bytes` of shared memory on the current device; asked of the

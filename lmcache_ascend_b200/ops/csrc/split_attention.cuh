@@ -285,7 +285,8 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
   };
   if (steps > 0) key_marks(0);
   const float scale = a.scale * kLog2e;
-  const float cap_in = a.softcap > 0.f ? 2.f * kLog2e * a.scale / a.softcap : 0.f;
+  const float cap_u = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
+  const float cap_in = 2.f * kLog2e * cap_u;
   const float cap_out = a.softcap * kLog2e;
 
   float o[D / 8][4];
@@ -336,10 +337,16 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
         for (int e = 0; e < 4; ++e) {
           const int col = t * 8 + c0 + (e & 1);
           float x = sc[t][e];
-          if (cap_out > 0.f)
-            x = fmaf(rcp(1.f + ex2(x * cap_in)), -2.f * cap_out, cap_out);
-          else
+          if (cap_out > 0.f) {
+            // tanh(u) = 1 - 2 / (1 + e^2u) is off by some 2^-22 of the cap: below
+            // u = 1/8 the series (next term 1.3e-9 of u)
+            const float u = x * cap_u, w = u * u;
+            const float small = fmaf(fmaf(fmaf(-17.f / 315.f, w, 2.f / 15.f), w, -1.f / 3.f), w, 1.f);
+            x = fabsf(u) < 0.125f ? x * scale * small
+                                  : fmaf(rcp(1.f + ex2(x * cap_in)), -2.f * cap_out, cap_out);
+          } else {
             x *= scale;
+          }
           const int kp = kDense ? __shfl_sync(0xffffffffu, kp_all, col) : 0;
           if (a.slopes) x += bias(e >= 2, j0 + col, kp);
           sc[t][e] = x;

@@ -52,9 +52,9 @@ struct TcArgs {
   long long q_batch, q_token, q_head;
   int tokens, q_len, heads, group;
   int k_tiles, tiles_per_slice, slices;
-  // x = s scale_log2, or cap_out tanh(s cap_u) with cap_in = 2 cap_u log2 e; for
-  // |s| up to cap_small x = s P(s^2)
-  float scale_log2, cap_in, cap_out, cap_small;
+  // x = s scale_log2, or cap_out tanh(u) with u = s cap_u and cap_in = 2 cap_u log2 e;
+  // for |s| up to cap_small x = s P(u^2)
+  float scale_log2, cap_u, cap_in, cap_out, cap_small;
   float2 cap_poly[5];
   // dense keys (prepared arrays, padded to whole tiles)
   PositionArgs pos;
@@ -531,7 +531,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // x = s c in log2 units, unless it is only scaled (then c goes into exp2)
       if (kCap) {
         // tanh by an odd polynomial while every score of the warp's rows is small
-        // against the cap, as they mostly are: three FMA slots a score instead of
+        // against the cap, as they mostly are: four FMA slots a score instead of
         // the exponential and reciprocal of tanh(u) = 1 - 2 / (1 + e^2u)
         float big = 0.f;
 #pragma unroll
@@ -539,11 +539,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           big = fmaxf(fmaxf(big, fabsf(s[i])), fabsf(s[i + 1]));
         if (__all_sync(0xffffffffu, big <= a.cap_small)) {
           f32x2 k[5];
+          const f32x2 cap_u = pack2(a.cap_u, a.cap_u);
 #pragma unroll
           for (int i = 0; i < 5; ++i) k[i] = pack2(a.cap_poly[i].x, a.cap_poly[i].y);
 #pragma unroll
           for (int i = 0; i < kKeys; i += 2) {
-            const f32x2 v = pack2(s[i], s[i + 1]), w = mul2(v, v);
+            const f32x2 v = pack2(s[i], s[i + 1]), u = mul2(v, cap_u), w = mul2(u, u);
             unpack2(mul2(v, fma2(fma2(fma2(fma2(k[4], w, k[3]), w, k[2]), w, k[1]), w, k[0])),
                     s[i], s[i + 1]);
           }

@@ -7,7 +7,7 @@ e = eps / 2 of the type (half a step):
 * the weights are rounded to the type before the product: e * sum p|v|;
 * the scores are fp32 sums of exact products: off by at most
   dx = D 2^-23 * scale * max sum_d |q_d k_d| (plus 2^-22 of the largest shaped
-  score, and 2^-20 of the cap), which scales a weight and the sum: 2 dx sum p|v|;
+  score, and 2^-20 of the cap or, below it, the largest score), which scales a weight and the sum: 2 dx sum p|v|;
 * exponentials, fp32 sums and joins of partial results: 2^-16 sum p|v|;
 * float16 weights below the normal range: 2^-25 per key, times max|v|;
 * the result's own rounding: e |o| (and 2^-25 below float16's normal range).
@@ -38,7 +38,7 @@ def _bounds(ref, q, k, v, dtype, scale, softcap, slopes, reach):
     top = min(reachable, softcap or reachable)
     if slopes is not None:
         top += float(slopes.abs().max()) * reach
-    dx = D * 2.0 ** -23 * reachable + 2.0 ** -22 * top + 2.0 ** -20 * softcap
+    dx = D * 2.0 ** -23 * reachable + 2.0 ** -22 * top + 2.0 ** -20 * min(softcap, reachable)
     e = torch.finfo(dtype).eps / 2
     n_keys = reach + 1
     tol = (e + 2 * dx + 2.0 ** -16) * a + e * o.abs() + 1e-30
@@ -116,7 +116,7 @@ def test_cpu_forms_and_refusals():
     t, n = torch.tensor([[1], [2]], dtype=torch.int32), torch.tensor([1, 3], dtype=torch.int32)
     out, lse = api.shared_prefix_attention(q, kc, kc, one, 4, t, n, return_lse=True)
     assert out.shape == q.shape and lse.shape == (2, 4) and out.dtype == q.dtype
-    for bad in (dict(prefix_len=5), dict(prefix_len=-1), dict(query=q[0]), dict(query=q[:, :3])):
+    for bad in (dict(scale=0.0), dict(softcap=-1.0), dict(prefix_len=5), dict(prefix_len=-1), dict(query=q[0]), dict(query=q[:, :3])):
         kw = dict(query=q, key_cache=kc, value_cache=kc, prefix_blocks=one, prefix_len=4,
                   block_tables=t, seq_lens=n)
         with pytest.raises(ValueError):
@@ -188,6 +188,10 @@ PREFIX = [
     (130, 1, 8, 8, 128, 256, 1111, [1 + i % 3 for i in range(130)], BF, 0.0, False, "plain"),
     (50, 1, 20, 2, 128, 8, 640, [i for i in range(50)], BF, 10.0, True, "plain"),
     (1, 1, 8, 2, 128, 16, 20, [9000], BF, 0.0, False, "plain"),
+    # caps far above the scores, and below them
+    (3, 1, 8, 2, 64, 16, 40, [7, 8, 9], FP, 1e6, False, "plain"),
+    (80, 1, 16, 1, 64, 16, 3057, [3] * 80, FP, 1e5, False, "plain"),
+    (80, 1, 16, 1, 128, 16, 2000, [3] * 80, FP, 1.0, True, "plain"),
 ]
 
 
@@ -300,7 +304,7 @@ def test_prefix_kernel_refusals():
                 dict(prefix_len=33), dict(prefix_len=-1), dict(prefix_blocks=prefix.long()),
                 dict(block_tables=tables[:1]), dict(block_tables=tables.long()),
                 dict(seq_lens=lens[:1]), dict(seq_lens=lens.long()), dict(softcap=-1.0),
-                dict(softcap=math.nan), dict(scale=math.inf),
+                dict(softcap=math.nan), dict(scale=math.inf), dict(scale=0.0), dict(scale=-1.0),
                 dict(alibi_slopes=torch.zeros(3, device="cuda")),
                 dict(alibi_slopes=torch.zeros(4, device="cuda").half()),
                 dict(status=torch.zeros(3, dtype=torch.int64))):
@@ -366,7 +370,14 @@ POSITION = [
     (333, 333, 8, 8, 64, BF, 0.0, False, "padded"),
     (640, 1500, 5, 1, 128, BF, 20.0, False, "interleaved"),
     (1000, 1000, 2, 1, 128, FP, 0.0, False, "causal"),
-    (5, 3000 - 7, 2, 2, 64, BF, 0.0, False, "subset"),
+    (5, 2993, 2, 2, 64, BF, 0.0, False, "subset"),
+    # the same kinds again above the split kernel's sizes
+    (1200, 2500, 8, 2, 64, BF, 0.0, True, "subset"),
+    (2000, 2000, 6, 1, 128, FP, 30.0, True, "documents"),
+    (1500, 1500, 7, 1, 64, BF, 0.0, False, "padded"),
+    (1300, 1700, 8, 1, 128, FP, 5.0, True, "shuffled"),
+    (1600, 1600, 8, 2, 128, BF, 0.0, True, "prefix"),
+    (1100, 1900, 8, 4, 64, FP, 1e5, True, "all"),
 ]
 
 
@@ -442,10 +453,10 @@ def test_position_kernel(case):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
-@pytest.mark.parametrize("Tq,H,D", [(300, 2, 64), (20, 4, 128)])
-def test_position_kernel_masked_keys_hold_anything(value, Tq, H, D):
+@pytest.mark.parametrize("Tq,H,D,T", [(300, 2, 64, 300), (20, 4, 128, 300),
+                                      (2200, 8, 64, 2200), (1000, 8, 128, 2200)])
+def test_position_kernel_masked_keys_hold_anything(value, Tq, H, D, T):
     """A key or value of NaN or infinity reaches the rows that see it, no other."""
-    T = 300
     q, k, v, qp, kp, kw = _position_case(Tq, T, H, 1, D, BF, "documents")
     clean_k, clean_v = k.clone(), v.clone()
     hit_k, hit_v = 77, 210
