@@ -314,17 +314,23 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
     cp_async_wait<kSplitStages - 1>();
     __syncwarp();
     const uint32_t kb = ring_addr + (it % kSplitStages) * L::kStage, vb = kb + L::kKeys;
-    float sc[2][4];
+    float sc[2][4], odd[2][4];  // two chains of products each
 #pragma unroll
-    for (int t = 0; t < 2; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sc[t][e] = odd[t][e] = 0.f;
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
       const int r = (lane & 7) + ((lane >> 4) << 3), c = k * 2 + ((lane >> 3) & 1);
       uint32_t b[4];
       ldmatrix4(b, kb + r * (D * 2) + ((c & ~7) << 4) + (((c & 7) ^ (r & 7)) << 4));
-      mma_16816<T>(sc[0], q[k], b[0], b[1]);
-      mma_16816<T>(sc[1], q[k], b[2], b[3]);
+      mma_16816<T>(k & 1 ? odd[0] : sc[0], q[k], b[0], b[1]);
+      mma_16816<T>(k & 1 ? odd[1] : sc[1], q[k], b[2], b[3]);
     }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sc[t][e] += odd[t][e];
     const int j0 = k0 + it * chunk + warp * kSplitKeys;
     uint32_t bad_keys = 0;
 #pragma unroll
@@ -493,10 +499,15 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
   wait_for_previous();
 }
 
-// Towards one wave of three blocks per SM, with 128 keys or more each: a block has
-// a start and an end to pay whatever the length of its slice.
+// Towards one wave of three blocks per SM, with 128 keys or more each, and not at
+// all below 384 keys: a second part costs a join.  Measured (us, 8 KV heads of 128,
+// one part / parts of 128 / of 256): 16 requests on 500 tokens 15.8 / 11.1 / 15.8,
+// one row on 1024 keys 19.4 / 7.5 / 9.2, 38 rows of 32 heads on 257 keys
+// 10.2 / 11.7.  A deeper ring (six stages) changed none of these: a step's own
+// chain of instructions takes its 0.9 us.
 inline int split_slices(long long blocks, long long keys) {
-  const long long want = std::min(444 / std::max(1ll, blocks), (keys + 127) / 128);
+  if (keys < 384) return 1;
+  const long long want = std::min(444 / std::max(1ll, blocks), keys / 128);
   return static_cast<int>(std::max(1ll, std::min(want, 64ll)));
 }
 
