@@ -88,7 +88,8 @@ cudaError_t launch(const PositionArgs &a, void *workspace, cudaStream_t stream) 
   if (p.split) {
     float *part_o = p.slices > 1 ? static_cast<float *>(workspace) : nullptr;
     float *part_lse = part_o + p.slices * rows * D;
-    const SplitPass s = {0, 0, false, a.q_tokens, p.row_tiles, p.slices, part_o, part_lse};
+    const SplitPass s = {0, 0, false, a.q_tokens, p.row_tiles, p.slices,
+                         a.heads / a.kv_heads, part_o, part_lse};
     cudaError_t e = launch_split<T, D>(a, s, 1, true, stream);
     if (e != cudaSuccess || p.slices == 1) return e;
     return launch_ordered(join_position_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)),

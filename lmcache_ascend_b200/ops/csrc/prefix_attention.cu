@@ -61,7 +61,7 @@ template <typename T, int D>
 cudaError_t launch(const PagedArgs &a, void *workspace, cudaStream_t stream) {
   const PrefixPlan p = plan_of(a);
   const long long rows = static_cast<long long>(a.batch) * a.q_len * a.heads;
-  const int slices = p.tc_slices + p.pre_slices + p.own_slices;
+  const int slices = p.tc_slices + p.pre_slices + p.own_slices, group = a.heads / a.kv_heads;
   float *part_o = static_cast<float *>(workspace);
   float *part_lse = part_o + slices * rows * D;
   cudaError_t e = cudaSuccess;
@@ -93,13 +93,13 @@ cudaError_t launch(const PagedArgs &a, void *workspace, cudaStream_t stream) {
   int first = p.tc_slices;
   if (p.pre_slices) {
     const SplitPass s = {0, static_cast<int>(a.prefix_len), false, a.batch * a.q_len, p.pre_tiles,
-                         p.pre_slices, part_o + first * rows * D, part_lse + first * rows};
+                         p.pre_slices, group, part_o + first * rows * D, part_lse + first * rows};
     e = launch_split<T, D>(a, s, 1, true, stream);
     if (e != cudaSuccess) return e;
     first += p.pre_slices;
   }
   const SplitPass s = {p.own_begin, static_cast<int>(a.prefix_len), true, a.q_len, p.own_tiles,
-                       p.own_slices, slices > 1 ? part_o + first * rows * D : nullptr,
+                       p.own_slices, group, slices > 1 ? part_o + first * rows * D : nullptr,
                        part_lse + first * rows};
   e = launch_split<T, D>(a, s, a.batch, first == 0, stream);
   if (e != cudaSuccess || slices == 1) return e;

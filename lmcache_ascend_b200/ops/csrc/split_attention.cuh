@@ -23,7 +23,7 @@ constexpr int kSplitWarps = 4, kSplitKeys = 16, kSplitRows = 16, kSplitStages = 
 struct SplitPass {
   int pre_begin, pre_end;
   bool own;
-  int unit_tokens, row_tiles, slices;
+  int unit_tokens, row_tiles, slices, group;  // group: heads per KV head
   float *part_o, *part_lse;  // first slice of this pass; null: write the result
 };
 
@@ -105,12 +105,12 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
   extern __shared__ __align__(128) uint8_t smem[];
   let_next_start();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int group = a.heads / a.kv_heads;
-  const int slice = blockIdx.y;
-  int u = blockIdx.x;
-  const int kv = u % a.kv_heads;
-  u /= a.kv_heads;
-  const int row_tile = u % s.row_tiles, unit = u / s.row_tiles;
+  const int group = s.group, slice = blockIdx.y;
+  // KV heads next to each other run together: their rows share DRAM pages
+  const unsigned tile = blockIdx.x / static_cast<unsigned>(a.kv_heads);
+  const int kv = blockIdx.x - tile * a.kv_heads;
+  const int unit = s.row_tiles == 1 ? tile : tile / static_cast<unsigned>(s.row_tiles);
+  const int row_tile = tile - unit * s.row_tiles;
   int n = 0, pre = 0, own_keys = 0, total;
   long long all_rows;
   if constexpr (kDense) {
@@ -131,17 +131,37 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
   const int per = ((total + s.slices - 1) / s.slices + chunk - 1) / chunk * chunk;
   const int k0 = min(total, slice * per), k1 = min(total, k0 + per);
 
-  // row r of this tile: token and head (rows past the unit's are not stored)
-  const int rows = s.unit_tokens * group - row_tile * kSplitRows;
-  auto token_of = [&](int r) { return unit * s.unit_tokens + (row_tile * kSplitRows + r) / group; };
-  auto head_of = [&](int r) { return kv * group + (row_tile * kSplitRows + r) % group; };
+  // this lane's two rows of the tile, r0 and r1 (rows past the unit's are not
+  // stored); the tile's result rows, -1 past the last
+  __shared__ int result_row[kSplitRows];
+  const int rows = min(kSplitRows, s.unit_tokens * group - row_tile * kSplitRows);
+  const int r0 = lane >> 2, r1 = r0 + 8, c0 = (lane & 3) * 2;
+  struct LaneRow {
+    int token, head;
+    bool valid;
+  };
+  auto lane_row = [&](int r) -> LaneRow {
+    const int at = row_tile * kSplitRows + r, t = at / group;
+    return {unit * s.unit_tokens + t, kv * group + at - t * group, r < rows};
+  };
+  const LaneRow row0 = lane_row(r0), row1 = lane_row(r1);
+  if (threadIdx.x < 32 && (lane & 3) == 0) {
+    result_row[r0] = row0.valid ? row0.token * a.heads + row0.head : -1;
+    result_row[r1] = row1.valid ? row1.token * a.heads + row1.head : -1;
+  }
+  RawMask raw0 = {0, 0, 0}, raw1 = {0, 0, 0};
+  if constexpr (kDense) {
+    if (row0.valid) raw0 = load_mask(a, row0.token);
+    if (row1.valid) raw1 = load_mask(a, row1.token);
+  }
   float *part_o = s.part_o + static_cast<long long>(slice) * all_rows * D;
   float *part_lse = s.part_lse + static_cast<long long>(slice) * all_rows;
   const bool direct = s.part_o == nullptr;
   if (k0 >= k1 && !direct) {  // no keys: an empty part
-    if (threadIdx.x < kSplitRows && static_cast<int>(threadIdx.x) < rows)
-      part_lse[static_cast<long long>(token_of(threadIdx.x)) * a.heads + head_of(threadIdx.x)] =
-          -INFINITY;
+    if (threadIdx.x < 32 && (lane & 3) == 0) {
+      if (row0.valid) part_lse[result_row[r0]] = -INFINITY;
+      if (row1.valid) part_lse[result_row[r1]] = -INFINITY;
+    }
     wait_for_previous();
     return;
   }
@@ -151,17 +171,17 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
   const int steps = (k1 - k0 + chunk - 1) / chunk;
 
   // Where the 16 keys of step `it` of this warp lie, in elements from the first:
-  // lane i (and i + 16) key i; -1 where there is none.
+  // lane i (and i + 16) key i; -1 where there is none.  (Paged.)
   struct Place {
     long long k, v;
     bool bad;  // in a page outside the cache
   };
   auto place_of = [&](int it) -> Place {
-    const int j = k0 + it * chunk + warp * kSplitKeys + (lane & 15);
-    if (j >= k1) return {-1, -1, false};
     if constexpr (kDense) {
-      return {j * a.k_token, j * a.v_token, false};
+      return {0, 0, false};  // a row's place is its index
     } else {
+      const int j = k0 + it * chunk + warp * kSplitKeys + (lane & 15);
+      if (j >= k1) return {-1, -1, false};
       const bool shared = j < pre;
       const unsigned at = shared ? s.pre_begin + j : j - pre;
       const unsigned col = at / static_cast<unsigned>(a.block_size);
@@ -184,12 +204,20 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
     const uint32_t dst = ring_addr + (it % kSplitStages) * L::kStage;
     const int c = lane % kChunks;
     constexpr int kRowsAtOnce = 32 / kChunks;
+    const int j0 = k0 + it * chunk + warp * kSplitKeys;
 #pragma unroll
     for (int i = 0; i < kSplitKeys / kRowsAtOnce; ++i) {
       const int r = i * kRowsAtOnce + lane / kChunks;
-      const long long ko = __shfl_sync(0xffffffffu, p.k, r);
-      const long long vo = alike ? ko : __shfl_sync(0xffffffffu, p.v, r);
-      const bool valid = ko >= 0;  // else zeros: nothing of the page is read
+      long long ko, vo;
+      bool valid;  // else zeros: nothing is read
+      if constexpr (kDense) {
+        valid = j0 + r < k1;
+        ko = (j0 + r) * a.k_token, vo = alike ? ko : (j0 + r) * a.v_token;
+      } else {
+        ko = __shfl_sync(0xffffffffu, p.k, r);
+        vo = alike ? ko : __shfl_sync(0xffffffffu, p.v, r);
+        valid = ko >= 0;
+      }
       const uint32_t at = r * (D * 2) + ((c & ~7) << 4) + (((c & 7) ^ (r & 7)) << 4);
       cp_async16(dst + at, k_first + (valid ? ko : 0), valid);
       cp_async16(dst + L::kKeys + at, v_first + (valid ? vo : 0), valid);
@@ -214,16 +242,15 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
   if (kSplitStages - 1 < steps) next = place_of(kSplitStages - 1);
 
   // Q as the A operand: row lane/4 (and + 8), columns 2 (lane % 4) of each 8.
-  const int r0 = lane >> 2, r1 = r0 + 8, c0 = (lane & 3) * 2;
   uint32_t q[D / 16][4];
-  auto q_row = [&](int r) -> const T * {
-    const int t = token_of(r);
-    const T *p = static_cast<const T *>(a.q) + head_of(r) * a.q_head;
-    if constexpr (kDense) return p + t * a.q_token;
-    else return p + t / a.q_len * a.q_batch + t % a.q_len * a.q_token;
+  auto q_row = [&](const LaneRow &r) -> const T * {
+    if (!r.valid) return nullptr;
+    const T *p = static_cast<const T *>(a.q) + r.head * a.q_head;
+    if constexpr (kDense) return p + r.token * a.q_token;
+    else return p + r.token / a.q_len * a.q_batch + r.token % a.q_len * a.q_token;
   };
   {
-    const T *p0 = r0 < rows ? q_row(r0) : nullptr, *p1 = r1 < rows ? q_row(r1) : nullptr;
+    const T *p0 = q_row(row0), *p1 = q_row(row1);
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
       const int c = k * 16 + c0;
@@ -240,28 +267,28 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
   int last0 = total, last1 = total;
   float slope0 = 0.f, slope1 = 0.f, at0 = 0.f, at1 = 0.f;
   if (a.slopes) {
-    slope0 = r0 < rows ? a.slopes[head_of(r0)] * kLog2e : 0.f;
-    slope1 = r1 < rows ? a.slopes[head_of(r1)] * kLog2e : 0.f;
+    slope0 = row0.valid ? a.slopes[row0.head] * kLog2e : 0.f;
+    slope1 = row1.valid ? a.slopes[row1.head] * kLog2e : 0.f;
   }
   if constexpr (kDense) {
-    if (r0 < rows) mask0 = row_mask(a, token_of(r0));
-    if (r1 < rows) mask1 = row_mask(a, token_of(r1));
+    mask0 = row_mask(a, raw0);
+    mask1 = row_mask(a, raw1);
   } else {
-    auto place = [&](int r, int &last, float &at) {
-      if (r >= rows) return;
-      const int t = token_of(r), b = t / a.q_len, i = t - b * a.q_len;
+    auto place = [&](const LaneRow &r, int &last, float &at) {
+      if (!r.valid) return;
+      const int b = s.own ? unit : r.token / a.q_len, i = r.token - b * a.q_len;
       if (s.own) last = pre + max(0, min(own_keys, n - a.q_len + i + 1));
       if (a.slopes)
         at = static_cast<float>(a.prefix_len + max(0, a.own_lens[b]) - a.q_len + i);
     };
-    place(r0, last0, at0);
-    place(r1, last1, at1);
+    place(row0, last0, at0);
+    place(row1, last1, at1);
   }
   // keys below this index, position and document are seen by all of the tile's rows
   int all_last = 0, all_limit = 0;
   if constexpr (kDense)
-    all_limit = __reduce_min_sync(0xffffffffu, min(r0 < rows ? mask0.limit : 2147483647,
-                                                   r1 < rows ? mask1.limit : 2147483647));
+    all_limit = __reduce_min_sync(0xffffffffu, min(row0.valid ? mask0.limit : 2147483647,
+                                                   row1.valid ? mask1.limit : 2147483647));
   else
     all_last = __reduce_min_sync(0xffffffffu, min(min(last0, last1), k1));
   // -slope times the distance between the row and pass key j
@@ -449,7 +476,10 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
     *reinterpret_cast<float2 *>(w0 + 8 * D) = make_float2(o[d][2], o[d][3]);
   }
   __syncthreads();
-  for (int r = warp; r < min(rows, kSplitRows); r += kSplitWarps) {
+  uint32_t again = 0;
+  auto finish = [&](int i) {
+    const int r = warp + i * kSplitWarps;
+    const long long row = result_row[r];
     float m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int w = 0; w < kSplitWarps; ++w) m = fmaxf(m, wm[w * kSplitRows + r]);
@@ -461,37 +491,56 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
       l = fmaf(f[w], wl[w * kSplitRows + r], l);
     }
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : NAN);
-    const long long row = static_cast<long long>(token_of(r)) * a.heads + head_of(r);
     bool finite = true;
-    for (int d = lane * 4; d < D; d += 128) {
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int kEach = D / 32;  // elements of a lane
+    float acc[kEach];
 #pragma unroll
-      for (int w = 0; w < kSplitWarps; ++w) {
-        const float4 v = *reinterpret_cast<const float4 *>(wo + (w * kSplitRows + r) * D + d);
-        acc.x = fmaf(f[w], v.x, acc.x), acc.y = fmaf(f[w], v.y, acc.y);
-        acc.z = fmaf(f[w], v.z, acc.z), acc.w = fmaf(f[w], v.w, acc.w);
-      }
-      acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
-      if (direct) {
-        const uint2 w = make_uint2(pair_from_float<T>(acc.x, acc.y),
-                                   pair_from_float<T>(acc.z, acc.w));
-        *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + row * D + d) = w;
-        const float big = fmaxf(fmaxf(fabsf(acc.x), fabsf(acc.y)), fmaxf(fabsf(acc.z), fabsf(acc.w)));
-        finite = finite && big <= 3.4028235e38f && acc.x + acc.y + acc.z + acc.w ==
-                                                       acc.x + acc.y + acc.z + acc.w;
-      } else {
-        *reinterpret_cast<float4 *>(part_o + row * D + d) = acc;
+    for (int e = 0; e < kEach; ++e) acc[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kSplitWarps; ++w) {
+      const float2 *v = reinterpret_cast<const float2 *>(wo + (w * kSplitRows + r) * D + lane * kEach);
+#pragma unroll
+      for (int e = 0; e < kEach / 2; ++e) {
+        acc[2 * e] = fmaf(f[w], v[e].x, acc[2 * e]);
+        acc[2 * e + 1] = fmaf(f[w], v[e].y, acc[2 * e + 1]);
       }
     }
-    if (lane == 0) {
-      const float log2_sum = l == 0.f ? -INFINITY : m + log2f(l);
-      if (!direct) part_lse[row] = log2_sum;
-      else if (a.lse) a.lse[row] = log2_sum * kLn2;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      acc[e] *= inv;
+      finite = finite && fabsf(acc[e]) <= 3.4028235e38f;
     }
-    if (direct && !__all_sync(0xffffffffu, finite)) {
-      __syncwarp();  // the row written above is written again
+    if (row >= 0) {
+#pragma unroll
+      for (int e = 0; e < kEach / 2; ++e) {
+        if (direct)
+          reinterpret_cast<uint32_t *>(static_cast<T *>(a.out) + row * D + lane * kEach)[e] =
+              pair_from_float<T>(acc[2 * e], acc[2 * e + 1]);
+        else
+          reinterpret_cast<float2 *>(part_o + row * D + lane * kEach)[e] =
+              make_float2(acc[2 * e], acc[2 * e + 1]);
+      }
+      if (lane == 0) {
+        const float log2_sum = l == 0.f ? -INFINITY : m + log2f(l);
+        if (!direct) part_lse[row] = log2_sum;
+        else if (a.lse) a.lse[row] = log2_sum * kLn2;
+      }
+      if (direct && !__all_sync(0xffffffffu, finite)) again |= 1u << i;
+    }
+  };
+  finish(0);
+  if (rows > kSplitWarps) {
+    // side by side: one row after the other they cost more than two steps
+#pragma unroll
+    for (int i = 1; i < kSplitRows / kSplitWarps; ++i) finish(i);
+  }
+  if (again) {
+    __syncwarp();  // the rows written above are written again
+    for (int i = 0; i < kSplitRows / kSplitWarps; ++i) {
+      if (!((again >> i) & 1)) continue;
+      const int row = result_row[warp + i * kSplitWarps];
       if constexpr (kDense)
-        strict_position_row<T, D>(a, token_of(r), head_of(r));
+        strict_position_row<T, D>(a, row / a.heads, row % a.heads);
       else
         strict_paged_row<T, D>(a, row);
     }

@@ -128,15 +128,27 @@ __device__ __forceinline__ int clamp_pos(long long p) {
   return static_cast<int>(min(max(p, -2147483646ll), 2147483645ll));
 }
 
-__device__ __forceinline__ RowMask row_mask(const PositionArgs &p, int token) {
-  const long long at = position_at(p.q_pos, p.long_q_pos, token);
-  const int prefix = p.q_prefix ? p.q_prefix[token] : 0;
-  const int doc = p.q_doc ? p.q_doc[token] : 0;
+// What a row's mask is made of, as it is loaded: several loads can be under way
+// before the first is used.
+struct RawMask {
+  long long at;
+  int prefix, doc;
+};
+
+__device__ __forceinline__ RawMask load_mask(const PositionArgs &p, int token) {
+  RawMask r;
+  r.at = position_at(p.q_pos, p.long_q_pos, token);
+  r.prefix = p.q_prefix ? p.q_prefix[token] : 0;
+  r.doc = p.q_doc ? p.q_doc[token] : 0;
+  return r;
+}
+
+__device__ __forceinline__ RowMask row_mask(const PositionArgs &p, const RawMask &r) {
   RowMask m;
-  m.pos = clamp_pos(at);
+  m.pos = clamp_pos(r.at);
   m.limit = p.causal ? m.pos + 1 : 2147483647;
-  if (p.q_prefix) m.limit = max(m.limit, prefix);
-  m.doc = doc;
+  if (p.q_prefix) m.limit = max(m.limit, r.prefix);
+  m.doc = r.doc;
   if (m.doc < 0) m.limit = kSeesNothing;  // a padding row
   return m;
 }
@@ -179,7 +191,7 @@ __device__ __forceinline__ void visible_keys(const RowMask &row, int kp0, int kp
 // infinity in its value is not, so only keys that the row sees may take part.
 template <typename T, int D>
 __device__ __forceinline__ void strict_position_row(const PositionArgs &a, int token, int h) {
-  const RowMask m = row_mask(a, token);
+  const RowMask m = row_mask(a, load_mask(a, token));
   const int kv = h / (a.heads / a.kv_heads);
   WarpRow<T, D> row;
   row.start(static_cast<const T *>(a.q) + token * a.q_token + h * a.q_head);
@@ -320,6 +332,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   int *row_at = reinterpret_cast<int *>(smem + L::kRowAt) + x * kTileM;
   if (warp < kMmaWarp && x < tiles) {
     ref = row_ref(a, kv_head, rho0 + x * kTileM + row_in_tile);
+    RawMask raw = {0, 0, 0};
+    if (kDense && ref.valid) raw = load_mask(a.pos, ref.token);
     if (half == 0) {
       const int b = ref.token / a.q_len;
       q_at[row_in_tile] = b * a.q_batch + (ref.token - b * a.q_len) * a.q_token +
@@ -338,7 +352,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     if (kDense) {
       mask.limit = lim_hi;
-      if (ref.valid) mask = row_mask(a.pos, ref.token);
+      if (ref.valid) mask = row_mask(a.pos, raw);
       const bool in_doc = ref.valid && mask.doc >= 0;
       lim_lo = __reduce_min_sync(0xffffffffu, ref.valid ? mask.limit : lim_lo);
       lim_hi = __reduce_max_sync(0xffffffffu, in_doc ? mask.limit : lim_hi);
