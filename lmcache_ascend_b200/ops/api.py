@@ -701,7 +701,7 @@ def shared_prefix_attention(query: torch.Tensor, key_cache: torch.Tensor,
     sum.  A row that sees no key is zero with -inf.  Keys in a block outside the
     cache, or past the end of a table row, are left out and reported in
     ``status``.  On the device: bfloat16 or float16, D of 64 or 128, 16-byte
-    aligned cache rows.
+    aligned cache rows, forward only.
     """
     if scale is None:
         scale = query.shape[-1] ** -0.5
@@ -744,7 +744,7 @@ def position_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
 
     Returns [Tq, H, D] and, with ``return_lse``, the fp32 log of each row's sum;
     a row that sees no key is zero with -inf.  On the device: bfloat16 or
-    float16, D of 64 or 128.
+    float16, D of 64 or 128, forward only.
     """
     if scale is None:
         scale = query.shape[-1] ** -0.5

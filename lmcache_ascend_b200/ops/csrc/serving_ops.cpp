@@ -40,6 +40,13 @@ at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const c10::Device 
   return at::detail::empty_cuda(sizes, dtype, dev, c10::nullopt);
 }
 
+// The operators are forward only: an input that asks for gradients would lose them.
+void check_no_grad(const char *op, std::initializer_list<const at::Tensor *> inputs) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const at::Tensor *t : inputs)
+    TORCH_CHECK(!t->requires_grad(), op, ": forward only, and an input requires grad");
+}
+
 RowType row_type(at::ScalarType t) {
   return t == at::kFloat ? RowType::kFloat
          : t == at::kBFloat16 ? RowType::kBFloat16 : RowType::kHalf;
@@ -195,6 +202,9 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> rotary_embedding_and_cache(
   TORCH_CHECK(query.is_cuda(), op, ": query must be on the device");
   const c10::Device dev = query.device();
   const auto dt = query.scalar_type();
+  check_no_grad(op, {&query});
+  if (key.has_value()) check_no_grad(op, {&*key});
+  if (value.has_value()) check_no_grad(op, {&*value});
   const c10::cuda::CUDAGuard guard(dev);
   const at::Tensor query_out =
       given_query_out.has_value() ? *given_query_out : fresh(query.sizes(), dt, dev);
@@ -308,6 +318,7 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> shared_prefix_attention(
   TORCH_CHECK(query.is_cuda(), op, ": query must be on the device");
   const c10::Device dev = query.device();
   const auto dt = query.scalar_type();
+  check_no_grad(op, {&query, &key_cache, &value_cache});
   TORCH_CHECK(query.dim() == 3 || query.dim() == 4, op,
               ": query must be [B, H, D] or [B, q_len, H, D]");
   const at::Tensor q4 = query.dim() == 3 ? query.unsqueeze(1) : query;
@@ -383,6 +394,7 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> position_attention(
   TORCH_CHECK(query.is_cuda(), op, ": query must be on the device");
   const c10::Device dev = query.device();
   const auto dt = query.scalar_type();
+  check_no_grad(op, {&query, &key, &value});
   TORCH_CHECK(query.dim() == 3, op, ": query must be [Tq, H, D]");
   const int64_t Tq = query.size(0), H = query.size(1), D = query.size(2);
   TORCH_CHECK(key.dim() == 3 && key.sizes() == value.sizes() && key.size(2) == D &&

@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
   using L = SplitSmem<D>;
   constexpr int kChunks = D / 8;  // 16-byte chunks of a row
   extern __shared__ __align__(128) uint8_t smem[];
-  let_next_start();
+  if (s.part_o != nullptr) let_next_start();  // a join or another pass follows
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int group = s.group, slice = blockIdx.y;
   // KV heads next to each other run together: their rows share DRAM pages
@@ -265,7 +265,8 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
   // document.
   RowMask mask0 = {0, 0, 0}, mask1 = {0, 0, 0};
   int last0 = total, last1 = total;
-  float slope0 = 0.f, slope1 = 0.f, at0 = 0.f, at1 = 0.f;
+  float slope0 = 0.f, slope1 = 0.f;
+  long long at0 = 0, at1 = 0;  // paged rows' positions
   if (a.slopes) {
     slope0 = row0.valid ? a.slopes[row0.head] * kLog2e : 0.f;
     slope1 = row1.valid ? a.slopes[row1.head] * kLog2e : 0.f;
@@ -274,12 +275,11 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
     mask0 = row_mask(a, raw0);
     mask1 = row_mask(a, raw1);
   } else {
-    auto place = [&](const LaneRow &r, int &last, float &at) {
+    auto place = [&](const LaneRow &r, int &last, long long &at) {
       if (!r.valid) return;
       const int b = s.own ? unit : r.token / a.q_len, i = r.token - b * a.q_len;
       if (s.own) last = pre + max(0, min(own_keys, n - a.q_len + i + 1));
-      if (a.slopes)
-        at = static_cast<float>(a.prefix_len + max(0, a.own_lens[b]) - a.q_len + i);
+      if (a.slopes) at = a.prefix_len + max(0, a.own_lens[b]) - a.q_len + i;
     };
     place(row0, last0, at0);
     place(row1, last1, at1);
@@ -297,8 +297,9 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
       const long long at = second ? mask1.pos : mask0.pos;
       return -(second ? slope1 : slope0) * fabsf(static_cast<float>(at - kp));
     } else {
-      const float at = static_cast<float>(j < pre ? s.pre_begin + j : a.prefix_len + (j - pre));
-      return -(second ? slope1 : slope0) * fabsf((second ? at1 : at0) - at);
+      const long long at = j < pre ? s.pre_begin + j : a.prefix_len + (j - pre);
+      return -(second ? slope1 : slope0) *
+             fabsf(static_cast<float>((second ? at1 : at0) - at));
     }
   };
   // dense: position and document of key lane % 16 of a step

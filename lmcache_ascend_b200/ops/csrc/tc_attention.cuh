@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int t_begin = slice * a.tiles_per_slice;
   const int t_end = min(a.k_tiles, t_begin + a.tiles_per_slice);
 
-  let_next_start();
+  if (a.slices) let_next_start();
   if (warp == kMmaWarp) tmem_alloc(tmem_slot, 512);
   if (warp == kLoadWarp && lane == 0) {
     prefetch_map(&k_map), prefetch_map(&v_map);
@@ -495,6 +495,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
     if (x < tiles) {
+    // (one level less indented than it is nested)
     // ------------------------------------------------------------- softmax
     const uint32_t lane_base = static_cast<uint32_t>(warp & 3) << 21;
     constexpr int kKeys = kTileN / 2;  // of this thread
@@ -505,12 +506,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const float *other = xch + (1 - half) * kTileM + row_in_tile;
     float m = -INFINITY, l = 0.f;
     const float slope = kBias && ref.valid ? a.slopes[ref.head] * kLog2e : 0.f;
-    float q_place = 0.f;  // position in the prefix, for the distance bias
-    int own = 0;
-    if (!kDense && ref.valid) {
+    long long q_place = 0;  // position behind the prefix, for the distance bias
+    if (!kDense && kBias && ref.valid) {
       const int b = ref.token / a.q_len;
-      own = max(0, a.own_lens[b]) - a.q_len + (ref.token - b * a.q_len);
-      q_place = static_cast<float>(a.prefix_len + own);
+      q_place = a.prefix_len + max(0, a.own_lens[b]) - a.q_len + (ref.token - b * a.q_len);
     }
     cp_async_commit();
     cp_async_wait<0>();
@@ -588,7 +587,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           at = static_cast<float>(static_cast<long long>(mask.pos) - a.stats[tile].pos_min) -
                (run ? static_cast<float>(half * kKeys) : 0.f);
         } else {
-          at = q_place - static_cast<float>(key0);
+          at = static_cast<float>(q_place - key0);
         }
         const bool before = kDense ? mask.limit <= mask.pos + 1 || at >= kKeys : at >= kKeys - 1;
         if (run && __all_sync(0xffffffffu, before || !ref.valid)) {

@@ -246,6 +246,19 @@ def test_prefix_kernel_bad_pages_are_left_out_and_reported(B, P):
 
 
 @pytest.mark.gpu
+def test_inputs_that_ask_for_gradients_are_refused():
+    q, k, v, qp, kp, _ = _position_case(8, 30, 4, 2, 64, BF, "subset")
+    d = [x.cuda() for x in (q, k, v, qp, kp)]
+    for i in range(3):
+        g = list(d)
+        g[i] = d[i].clone().requires_grad_()
+        with pytest.raises(RuntimeError, match="forward only"):
+            api.position_attention(*g)
+        with torch.no_grad():
+            api.position_attention(*g)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,value", [(BF, torch.finfo(BF).min), (FP, torch.finfo(FP).min),
                                          (BF, math.inf)])
 def test_prefix_kernel_unused_slots_hold_anything(dtype, value):
