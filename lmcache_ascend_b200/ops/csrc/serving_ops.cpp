@@ -47,6 +47,16 @@ void check_no_grad(const char *op, std::initializer_list<const at::Tensor *> inp
     TORCH_CHECK(!t->requires_grad(), op, ": forward only, and an input requires grad");
 }
 
+// `n` elements of `base` from `first` on, as a tensor of their own (a view without
+// the dispatcher).
+at::Tensor part_of(const at::Tensor &base, int64_t first, int64_t n) {
+  auto t = at::detail::make_tensor<c10::TensorImpl>(
+      c10::TensorImpl::VIEW, c10::Storage(base.storage()), base.key_set(), base.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(first);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return t;
+}
+
 RowType row_type(at::ScalarType t) {
   return t == at::kFloat ? RowType::kFloat
          : t == at::kBFloat16 ? RowType::kBFloat16 : RowType::kHalf;
@@ -156,10 +166,16 @@ build_slot_mapping(const at::Tensor &context_lens, const at::Tensor &new_lens,
   }
   const c10::cuda::CUDAGuard guard(dev);
   const auto slot_type = long_slots ? at::kLong : at::kInt;
-  auto slots = fresh({num_tokens}, slot_type, dev), positions = fresh({num_tokens}, slot_type, dev);
-  auto request_ids = fresh({num_tokens}, at::kInt, dev);
-  auto start = fresh({B + 1}, at::kInt, dev), seq_lens = fresh({B}, at::kInt, dev);
-  auto taken = fresh({B + 1}, at::kInt, dev);
+  // six results in two allocations, each on 128 bytes
+  auto even = [](int64_t n) { return (n + 31) / 32 * 32; };
+  const auto wide = fresh({2 * even(num_tokens)}, slot_type, dev);
+  const auto slots = part_of(wide, 0, num_tokens);
+  const auto positions = part_of(wide, even(num_tokens), num_tokens);
+  const auto narrow = fresh({even(num_tokens) + 3 * even(B + 1)}, at::kInt, dev);
+  const auto request_ids = part_of(narrow, 0, num_tokens);
+  const auto start = part_of(narrow, even(num_tokens), B + 1);
+  const auto seq_lens = part_of(narrow, even(num_tokens) + even(B + 1), B);
+  const auto taken = part_of(narrow, even(num_tokens) + 2 * even(B + 1), B + 1);
   SlotArgs a;
   a.ctx = context_lens.data_ptr();
   a.fresh = new_lens.data_ptr();

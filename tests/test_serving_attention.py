@@ -188,6 +188,9 @@ PREFIX = [
     (130, 1, 8, 8, 128, 256, 1111, [1 + i % 3 for i in range(130)], BF, 0.0, False, "plain"),
     (50, 1, 20, 2, 128, 8, 640, [i for i in range(50)], BF, 10.0, True, "plain"),
     (1, 1, 8, 2, 128, 16, 20, [9000], BF, 0.0, False, "plain"),
+    # many heads on one KV head, not a multiple of the row tiles
+    (3, 2, 96, 1, 64, 16, 200, [5, 6, 7], BF, 0.0, False, "plain"),
+    (20, 1, 96, 1, 128, 64, 1500, [1 + i for i in range(20)], FP, 0.0, True, "heads"),
     # caps far above the scores, and below them
     (3, 1, 8, 2, 64, 16, 40, [7, 8, 9], FP, 1e6, False, "plain"),
     (80, 1, 16, 1, 64, 16, 3057, [3] * 80, FP, 1e5, False, "plain"),
@@ -384,6 +387,8 @@ POSITION = [
     (640, 1500, 5, 1, 128, BF, 20.0, False, "interleaved"),
     (1000, 1000, 2, 1, 128, FP, 0.0, False, "causal"),
     (5, 2993, 2, 2, 64, BF, 0.0, False, "subset"),
+    (40, 300, 96, 1, 64, BF, 0.0, False, "subset"),
+    (130, 700, 96, 1, 128, FP, 0.0, False, "shuffled"),
     # the same kinds again above the split kernel's sizes
     (1200, 2500, 8, 2, 64, BF, 0.0, True, "subset"),
     (2000, 2000, 6, 1, 128, FP, 30.0, True, "documents"),
