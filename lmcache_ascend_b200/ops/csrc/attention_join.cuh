@@ -116,19 +116,25 @@ cudaError_t allow_smem(Kernel kernel, int bytes) {
 // it ends (it hides the launch and fills the SMs that are done).  Every kernel
 // calls wait_for_previous() before it reads what an earlier one of the call
 // wrote, and in any case before its blocks end, so that they complete in order.
+// `cluster`: blocks of a cluster along y.
 template <typename... Params, typename... Args>
 cudaError_t launch_ordered(void (*kernel)(Params...), dim3 grid, unsigned threads, int smem,
-                           bool first, cudaStream_t stream, const Args &...args) {
+                           bool first, cudaStream_t stream, int cluster, const Args &...args) {
   cudaLaunchConfig_t config = {};
   config.gridDim = grid;
   config.blockDim = dim3(threads);
   config.dynamicSmemBytes = static_cast<size_t>(smem);
   config.stream = stream;
-  cudaLaunchAttribute attribute = {};
-  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &attribute;
-  config.numAttrs = first ? 0 : 1;
+  cudaLaunchAttribute attributes[2] = {};
+  config.attrs = attributes;
+  if (!first) {
+    attributes[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[config.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attributes[config.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attributes[config.numAttrs++].val.clusterDim = {1, static_cast<unsigned>(cluster), 1};
+  }
   return cudaLaunchKernelEx(&config, kernel, Params(args)...);
 }
 
@@ -143,7 +149,7 @@ cudaError_t launch_tc(const CUtensorMap &k_map, const CUtensorMap &v_map, const 
   constexpr int kBytes = TcSmem<D>::kBytes;
   cudaError_t e = allow_smem(kernel, kBytes);
   if (e != cudaSuccess) return e;
-  return launch_ordered(kernel, dim3(grid), kTcThreads, kBytes, first, stream, k_map, v_map, t);
+  return launch_ordered(kernel, dim3(grid), kTcThreads, kBytes, first, stream, 1, k_map, v_map, t);
 }
 
 }  // namespace lmc

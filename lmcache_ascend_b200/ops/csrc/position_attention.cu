@@ -86,14 +86,15 @@ cudaError_t launch(const PositionArgs &a, void *workspace, cudaStream_t stream) 
   const Plan p = plan_of(a);
   const long long rows = static_cast<long long>(a.q_tokens) * a.heads;
   if (p.split) {
-    float *part_o = p.slices > 1 ? static_cast<float *>(workspace) : nullptr;
-    float *part_lse = part_o + p.slices * rows * D;
+    const bool joined = p.slices > kMostClustered;  // else the parts join in a cluster
+    float *part_o = joined ? static_cast<float *>(workspace) : nullptr;
+    float *part_lse = joined ? part_o + p.slices * rows * D : nullptr;
     const SplitPass s = {0, 0, false, a.q_tokens, p.row_tiles, p.slices,
                          a.heads / a.kv_heads, part_o, part_lse};
     cudaError_t e = launch_split<T, D>(a, s, 1, true, stream);
-    if (e != cudaSuccess || p.slices == 1) return e;
+    if (e != cudaSuccess || !joined) return e;
     return launch_ordered(join_position_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)),
-                          128, 0, false, stream, a, part_o, part_lse, p.slices);
+                          128, 0, false, stream, 1, a, part_o, part_lse, p.slices);
   }
   char *w = static_cast<char *>(workspace);
   TileStats *stats = reinterpret_cast<TileStats *>(w);
@@ -128,7 +129,7 @@ cudaError_t launch(const PositionArgs &a, void *workspace, cudaStream_t stream) 
   cudaError_t e = launch_tc<T, D, true>(k_map, v_map, t, grid, false, stream);
   if (e != cudaSuccess || !p.slices) return e;
   return launch_ordered(join_position_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128,
-                        0, false, stream, a, t.part_o, t.part_lse, p.slices);
+                        0, false, stream, 1, a, t.part_o, t.part_lse, p.slices);
 }
 
 }  // namespace
@@ -136,7 +137,7 @@ cudaError_t launch(const PositionArgs &a, void *workspace, cudaStream_t stream) 
 long long position_attention_workspace(const PositionArgs &a, int dim) {
   const Plan p = plan_of(a);
   if (p.split)
-    return p.slices == 1 ? 0 : p.slices * static_cast<long long>(a.q_tokens) * a.heads * (dim + 1) * 4;
+    return p.slices <= kMostClustered ? 0 : p.slices * static_cast<long long>(a.q_tokens) * a.heads * (dim + 1) * 4;
   return p.tiles * static_cast<long long>(sizeof(TileStats)) + p.keys * 12 + (p.tiles + 3) / 4 * 16 +
          p.slices * static_cast<long long>(a.q_tokens) * a.heads * (dim + 1) * 4;
 }

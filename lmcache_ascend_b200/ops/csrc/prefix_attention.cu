@@ -21,7 +21,10 @@ struct PrefixPlan {
 // 11.8 / 15.9, 1024 steps 17.5 / 20.3 and 22.2 / 24.8, 2000 steps 20.1 / 25.0
 // (one request), 4096 steps 36.1 / 26.4.
 constexpr long long kSplitSteps = 2000;
-constexpr long long kFewSteps = 600;
+// ... and up to which every request reads it with its own keys, in one pass (16 on
+// 500 tokens, 1024 steps: 11.0 us against 11.2 in two passes, with one launch for
+// three; 4 on 500: 7.8 against 9.6).
+constexpr long long kFewSteps = 1200;
 
 PrefixPlan plan_of(const PagedArgs &a) {
   PrefixPlan p = {};
@@ -35,8 +38,7 @@ PrefixPlan plan_of(const PagedArgs &a) {
   const long long prefix_steps = (prefix + kSplitWarps * kSplitKeys - 1) / (kSplitWarps * kSplitKeys);
   const long long request_tiles = (a.q_len * group + kSplitRows - 1) / kSplitRows;
   if (a.batch * request_tiles * a.kv_heads * prefix_steps <= kFewSteps) {
-    // short enough for every request to read the prefix with its own keys (one
-    // pass): 4 requests on 500 tokens, 8 KV heads: 9.6 us in two passes
+    // one pass
   } else if (boxes && prefix >= kTileN && row_tiles * a.kv_heads * prefix_steps > kSplitSteps) {
     p.tiles = prefix / kTileN;
     p.groups = static_cast<int>((tokens * group + kBlockRows - 1) / kBlockRows);
@@ -57,11 +59,17 @@ PrefixPlan plan_of(const PagedArgs &a) {
   return p;
 }
 
+// One pass of few parts per row needs no workspace: they join in a cluster.
+bool needs_join(const PrefixPlan &p) {
+  return p.tc_slices + p.pre_slices > 0 || p.own_slices > kMostClustered;
+}
+
 template <typename T, int D>
 cudaError_t launch(const PagedArgs &a, void *workspace, cudaStream_t stream) {
   const PrefixPlan p = plan_of(a);
   const long long rows = static_cast<long long>(a.batch) * a.q_len * a.heads;
   const int slices = p.tc_slices + p.pre_slices + p.own_slices, group = a.heads / a.kv_heads;
+  const bool joined = needs_join(p);
   float *part_o = static_cast<float *>(workspace);
   float *part_lse = part_o + slices * rows * D;
   cudaError_t e = cudaSuccess;
@@ -99,12 +107,12 @@ cudaError_t launch(const PagedArgs &a, void *workspace, cudaStream_t stream) {
     first += p.pre_slices;
   }
   const SplitPass s = {p.own_begin, static_cast<int>(a.prefix_len), true, a.q_len, p.own_tiles,
-                       p.own_slices, group, slices > 1 ? part_o + first * rows * D : nullptr,
+                       p.own_slices, group, joined ? part_o + first * rows * D : nullptr,
                        part_lse + first * rows};
   e = launch_split<T, D>(a, s, a.batch, first == 0, stream);
-  if (e != cudaSuccess || slices == 1) return e;
+  if (e != cudaSuccess || !joined) return e;
   return launch_ordered(join_paged_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0,
-                        false, stream, a, part_o, part_lse, slices);
+                        false, stream, 1, a, part_o, part_lse, slices);
 }
 
 }  // namespace
@@ -112,7 +120,7 @@ cudaError_t launch(const PagedArgs &a, void *workspace, cudaStream_t stream) {
 long long shared_prefix_attention_workspace(const PagedArgs &a, int dim) {
   const PrefixPlan p = plan_of(a);
   const int slices = p.tc_slices + p.pre_slices + p.own_slices;
-  return slices == 1 ? 0
+  return !needs_join(p) ? 0
                      : static_cast<long long>(slices) * a.batch * a.q_len * a.heads * (dim + 1) * 4;
 }
 

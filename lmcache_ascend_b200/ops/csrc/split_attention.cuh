@@ -9,7 +9,9 @@
 // 16 rows, 16 flop a byte, so it is bound by the reads and the small
 // instruction loses nothing.  Any block size, page order and stride; dense keys
 // for few rows or short calls, where the tensor-core kernel's 256-row blocks
-// would wait most of the time.  With one slice the block writes the result.
+// would wait most of the time.  Up to eight slices of a row are one cluster: its
+// blocks join their parts through shared memory and write the result; more go
+// through memory and a join kernel.
 #pragma once
 #include "attention_join.cuh"
 
@@ -24,8 +26,33 @@ struct SplitPass {
   int pre_begin, pre_end;
   bool own;
   int unit_tokens, row_tiles, slices, group;  // group: heads per KV head
-  float *part_o, *part_lse;  // first slice of this pass; null: write the result
+  // first slice of this pass; null: write the result (the blocks of a row's slices
+  // are then one cluster and join through shared memory)
+  float *part_o, *part_lse;
 };
+constexpr int kMostClustered = 8;  // blocks of a cluster that every GPU takes
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+// The same shared-memory place in block `rank` of the cluster.
+__device__ __forceinline__ uint32_t in_block(uint32_t addr, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr)
+               : "memory");
+  return v;
+}
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -62,8 +89,8 @@ struct SplitSmem {
   static constexpr int kStage = 2 * kKeys;
   static constexpr int kWarp = kSplitStages * kStage;
   static constexpr int kBytes = kSplitWarps * kWarp;
-  // the join at the end: each warp's output and statistics
-  static_assert(kBytes >= kSplitWarps * kSplitRows * (D + 2) * 4, "join fits in the rings");
+  // the join at the end: each warp's output and statistics, then the block's
+  static_assert(kBytes >= (kSplitWarps + 1) * kSplitRows * (D + 2) * 4, "join fits in the rings");
 };
 
 // A row of the batch by the definition, on one warp: when a joined result holds
@@ -477,10 +504,38 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
     *reinterpret_cast<float2 *>(w0 + 8 * D) = make_float2(o[d][2], o[d][3]);
   }
   __syncthreads();
+  constexpr int kEach = D / 32;  // elements of a lane
   uint32_t again = 0;
+  // a row's result from its sum, the sum of its weights and their maximum
+  auto write = [&](int i, int row, float (&acc)[kEach], float m, float l) {
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : NAN);
+    bool finite = true;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      acc[e] *= inv;
+      finite = finite && fabsf(acc[e]) <= 3.4028235e38f;
+    }
+    const long long at = static_cast<long long>(row) * D + lane * kEach;
+#pragma unroll
+    for (int e = 0; e < kEach / 2; ++e) {
+      if (direct)
+        reinterpret_cast<uint32_t *>(static_cast<T *>(a.out) + at)[e] =
+            pair_from_float<T>(acc[2 * e], acc[2 * e + 1]);
+      else
+        reinterpret_cast<float2 *>(part_o + at)[e] = make_float2(acc[2 * e], acc[2 * e + 1]);
+    }
+    if (lane == 0) {
+      const float log2_sum = l == 0.f ? -INFINITY : m + log2f(l);
+      if (!direct) part_lse[row] = log2_sum;
+      else if (a.lse) a.lse[row] = log2_sum * kLn2;
+    }
+    if (direct && !__all_sync(0xffffffffu, finite)) again |= 1u << i;
+  };
+  const bool clustered = direct && s.slices > 1;
+  float *bo = wl + kSplitWarps * kSplitRows;  // the block's [16][D], maxima and sums
+  float *bm = bo + kSplitRows * D, *bl = bm + kSplitRows;
   auto finish = [&](int i) {
     const int r = warp + i * kSplitWarps;
-    const long long row = result_row[r];
     float m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int w = 0; w < kSplitWarps; ++w) m = fmaxf(m, wm[w * kSplitRows + r]);
@@ -491,9 +546,6 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
       f[w] = ex2(wm[w * kSplitRows + r] - base);
       l = fmaf(f[w], wl[w * kSplitRows + r], l);
     }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : NAN);
-    bool finite = true;
-    constexpr int kEach = D / 32;  // elements of a lane
     float acc[kEach];
 #pragma unroll
     for (int e = 0; e < kEach; ++e) acc[e] = 0.f;
@@ -506,27 +558,14 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
         acc[2 * e + 1] = fmaf(f[w], v[e].y, acc[2 * e + 1]);
       }
     }
+    if (clustered) {
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      acc[e] *= inv;
-      finite = finite && fabsf(acc[e]) <= 3.4028235e38f;
-    }
-    if (row >= 0) {
-#pragma unroll
-      for (int e = 0; e < kEach / 2; ++e) {
-        if (direct)
-          reinterpret_cast<uint32_t *>(static_cast<T *>(a.out) + row * D + lane * kEach)[e] =
-              pair_from_float<T>(acc[2 * e], acc[2 * e + 1]);
-        else
-          reinterpret_cast<float2 *>(part_o + row * D + lane * kEach)[e] =
-              make_float2(acc[2 * e], acc[2 * e + 1]);
-      }
-      if (lane == 0) {
-        const float log2_sum = l == 0.f ? -INFINITY : m + log2f(l);
-        if (!direct) part_lse[row] = log2_sum;
-        else if (a.lse) a.lse[row] = log2_sum * kLn2;
-      }
-      if (direct && !__all_sync(0xffffffffu, finite)) again |= 1u << i;
+      for (int e = 0; e < kEach / 2; ++e)
+        reinterpret_cast<float2 *>(bo + r * D + lane * kEach)[e] =
+            make_float2(acc[2 * e], acc[2 * e + 1]);
+      if (lane == 0) bm[r] = m, bl[r] = l;
+    } else if (result_row[r] >= 0) {
+      write(i, result_row[r], acc, m, l);
     }
   };
   finish(0);
@@ -535,11 +574,43 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
 #pragma unroll
     for (int i = 1; i < kSplitRows / kSplitWarps; ++i) finish(i);
   }
+  if (clustered) {
+    // the rows are dealt to the cluster's blocks, which read the others' parts
+    cluster_sync();
+    for (int i = 0, r = slice * kSplitWarps + warp; r < rows; ++i, r += s.slices * kSplitWarps) {
+      const uint32_t m_at = smem_u32(bm + r), l_at = smem_u32(bl + r);
+      const uint32_t o_at = smem_u32(bo + r * D + lane * kEach);
+      float ms[kMostClustered], m = -INFINITY, l = 0.f, acc[kEach];
+#pragma unroll
+      for (int b = 0; b < kMostClustered; ++b) {
+        ms[b] = b < s.slices ? ld_cluster(in_block(m_at, b)) : -INFINITY;
+        m = fmaxf(m, ms[b]);
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) acc[e] = 0.f;
+#pragma unroll
+      for (int b = 0; b < kMostClustered; ++b) {
+        if (b >= s.slices) continue;
+        const float f = ex2(ms[b] - base);
+        l = fmaf(f, ld_cluster(in_block(l_at, b)), l);
+#pragma unroll
+        for (int e = 0; e < kEach / 2; ++e) {
+          const float2 v = ld_cluster2(in_block(o_at, b) + e * 8);
+          acc[2 * e] = fmaf(f, v.x, acc[2 * e]);
+          acc[2 * e + 1] = fmaf(f, v.y, acc[2 * e + 1]);
+        }
+      }
+      write(i, result_row[r], acc, m, l);
+    }
+    cluster_sync();  // no block leaves while another reads its memory
+  }
   if (again) {
     __syncwarp();  // the rows written above are written again
     for (int i = 0; i < kSplitRows / kSplitWarps; ++i) {
       if (!((again >> i) & 1)) continue;
-      const int row = result_row[warp + i * kSplitWarps];
+      const int row = result_row[clustered ? (i * s.slices + slice) * kSplitWarps + warp
+                                           : warp + i * kSplitWarps];
       if constexpr (kDense)
         strict_position_row<T, D>(a, row / a.heads, row % a.heads);
       else
@@ -549,15 +620,16 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
   wait_for_previous();
 }
 
-// Towards one wave of three blocks per SM, with 128 keys or more each, and not at
-// all below 384 keys: a second part costs a join.  Measured (us, 8 KV heads of 128,
-// one part / parts of 128 / of 256): 16 requests on 500 tokens 15.8 / 11.1 / 15.8,
-// one row on 1024 keys 19.4 / 7.5 / 9.2, 38 rows of 32 heads on 257 keys
-// 10.2 / 11.7.  A deeper ring (six stages) changed none of these: a step's own
-// chain of instructions takes its 0.9 us.
+// Towards one wave of three blocks per SM, with 128 keys or more each; eight parts
+// rather than up to sixteen, because a cluster joins them in the same launch.
+// Measured (us, 8 KV heads of 128): 16 requests on 500 tokens 15.8 in one part, 11.0
+// in parts of 128; one row on 1024 keys 19.4 / 6.9; one row on 257 keys 7.8 / 7.0,
+// but 38 rows of 32 heads on them (80 blocks) 9.4 / 10.0.  A deeper ring (six stages)
+// changed none of these: a step's own chain of instructions takes its 0.8 us.
 inline int split_slices(long long blocks, long long keys) {
-  if (keys < 384) return 1;
-  const long long want = std::min(444 / std::max(1ll, blocks), keys / 128);
+  if (keys < 256 || (keys < 384 && blocks > 74)) return 1;
+  long long want = std::min(444 / std::max(1ll, blocks), keys / 128);
+  if (want > kMostClustered && want <= 2 * kMostClustered) want = kMostClustered;
   return static_cast<int>(std::max(1ll, std::min(want, 64ll)));
 }
 
@@ -571,7 +643,8 @@ cudaError_t launch_split(const Args &a, const SplitPass &s, long long units, boo
   cudaError_t e = allow_smem(kernel, kBytes);
   if (e != cudaSuccess) return e;
   const dim3 grid(static_cast<unsigned>(units * s.row_tiles * a.kv_heads), s.slices);
-  return launch_ordered(kernel, grid, kSplitWarps * 32, kBytes, first, stream, a, s);
+  return launch_ordered(kernel, grid, kSplitWarps * 32, kBytes, first, stream,
+                        s.part_o == nullptr ? s.slices : 1, a, s);
 }
 
 template <typename T, int D>
