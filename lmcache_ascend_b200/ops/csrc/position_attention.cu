@@ -29,7 +29,7 @@ __global__ void __launch_bounds__(kTileN)
   if (threadIdx.x == 0) first = p;
   __syncthreads();
   const bool one_apart =
-      __syncthreads_and(!in || static_cast<long long>(p) == static_cast<long long>(first) + threadIdx.x);
+      __syncthreads_and(!in || p - static_cast<long long>(first) == threadIdx.x);
   lo = min(min(edge[0][0], edge[0][1]), min(edge[0][2], edge[0][3]));
   pos32[i] = p;
   doc32[i] = d;
@@ -137,7 +137,9 @@ cudaError_t launch(const PositionArgs &a, void *workspace, cudaStream_t stream) 
 long long position_attention_workspace(const PositionArgs &a, int dim) {
   const Plan p = plan_of(a);
   if (p.split)
-    return p.slices <= kMostClustered ? 0 : p.slices * static_cast<long long>(a.q_tokens) * a.heads * (dim + 1) * 4;
+    return p.slices <= kMostClustered
+               ? 0
+               : p.slices * static_cast<long long>(a.q_tokens) * a.heads * (dim + 1) * 4;
   return p.tiles * static_cast<long long>(sizeof(TileStats)) + p.keys * 12 + (p.tiles + 3) / 4 * 16 +
          p.slices * static_cast<long long>(a.q_tokens) * a.heads * (dim + 1) * 4;
 }

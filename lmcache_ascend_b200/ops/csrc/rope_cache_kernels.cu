@@ -109,8 +109,9 @@ __device__ __forceinline__ void load_table(const CT *p, float *f) {
 
 // 16-byte units.  Needs dim % (2 VE) == 0 and rot % (2 VE) == 0, aligned rows and
 // at most kRopeThreads units per head.  `heads` counts those of q, k and v; a
-// block takes `per_block` of them in a row, up to kHeadsPerThread a thread.  Its rows are looked up first (position, page), so that its data
-// and table loads wait for nothing but their own memory.
+// block takes `per_block` of them in a row, up to kHeadsPerThread a thread.  Its
+// rows are looked up first (position, page), so that its data and table loads wait
+// for nothing but their own memory.
 template <typename T, typename CT>
 __global__ void __launch_bounds__(kRopeThreads, 5)
     rope_cache_vec_kernel(RopeArgs a, int heads, int per_block) {
@@ -278,8 +279,9 @@ cudaError_t launch(const RopeArgs &a, bool vec, cudaStream_t stream) {
     const long long blocks = (all + per_block - 1) / per_block;
     if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
     const int rows = static_cast<int>((per_block + heads - 2) / heads + 1);  // at most, of a block
-    rope_cache_vec_kernel<T, CT><<<static_cast<unsigned>(blocks), kRopeThreads, rows * 24, stream>>>(
-        a, static_cast<int>(heads), static_cast<int>(per_block));
+    rope_cache_vec_kernel<T, CT>
+        <<<static_cast<unsigned>(blocks), kRopeThreads, rows * 24, stream>>>(
+            a, static_cast<int>(heads), static_cast<int>(per_block));
   } else {
     const long long units = a.num_tokens * heads * ((a.dim + 1) / 2);
     const long long blocks = std::min((units + kRopeThreads - 1) / kRopeThreads, 148ll * 32);

@@ -234,11 +234,12 @@ cudaError_t launch_slot_mapping(const SlotArgs &a, bool long_lens, bool long_slo
   // one to eight new tokens 16.1 -> 6.1 us against blocks of kMostTokens, while 1M
   // tokens took 12.0 us instead of 9.1 on three blocks per SM
   const long long even = (a.num_tokens + 148 * 2 - 1) / (148 * 2);
-  const int per_block = static_cast<int>(
-      std::min(1ll * kMostTokens, std::max(1ll, (even + kSlotThreads - 1) / kSlotThreads) * kSlotThreads));
+  const long long turns = std::max(1ll, (even + kSlotThreads - 1) / kSlotThreads);
+  const int per_block = static_cast<int>(std::min(1ll * kMostTokens, turns * kSlotThreads));
   const unsigned grid =
       static_cast<unsigned>(std::max(1ll, (a.num_tokens + per_block - 1) / per_block));
-#define LMC_SLOTS(LT, OT) slot_mapping_kernel<LT, OT><<<grid, kSlotThreads, 0, stream>>>(a, per_block)
+#define LMC_SLOTS(LT, OT) \
+  slot_mapping_kernel<LT, OT><<<grid, kSlotThreads, 0, stream>>>(a, per_block)
   if (!long_lens) {
     if (long_slots) LMC_SLOTS(int, long long); else LMC_SLOTS(int, int);
   } else {

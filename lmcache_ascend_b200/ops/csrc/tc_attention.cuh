@@ -495,312 +495,311 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
     if (x < tiles) {
-    // (one level less indented than it is nested)
-    // ------------------------------------------------------------- softmax
-    const uint32_t lane_base = static_cast<uint32_t>(warp & 3) << 21;
-    constexpr int kKeys = kTileN / 2;  // of this thread
-    const uint32_t s_addr = tmem + lane_base + x * kTileN;
-    const uint32_t o_addr = tmem + lane_base + 2 * kTileN + x * D + half * (D / 2);
-    float *xch = reinterpret_cast<float *>(smem + L::kXch) + x * 2 * kTileM;
-    float *mine = xch + half * kTileM + row_in_tile;
-    const float *other = xch + (1 - half) * kTileM + row_in_tile;
-    float m = -INFINITY, l = 0.f;
-    const float slope = kBias && ref.valid ? a.slopes[ref.head] * kLog2e : 0.f;
-    long long q_place = 0;  // position behind the prefix, for the distance bias
-    if (!kDense && kBias && ref.valid) {
-      const int b = ref.token / a.q_len;
-      q_place = a.prefix_len + max(0, a.own_lens[b]) - a.q_len + (ref.token - b * a.q_len);
-    }
-    cp_async_commit();
-    cp_async_wait<0>();
-    fence_proxy_async_smem();
-    mbar_arrive(q_full);
-    int tile, j = 0;
-    bool whole, ok = true;
-    while (scan.next(tile, whole)) {
-      const int key0 = tile * kTileN + half * kKeys;
-      // masks while the scores are computed
-      uint32_t vis0 = 0xffffffffu, vis1 = 0xffffffffu;
-      if (kDense && !whole) {
-        const int kp0 = a.k_pos32[key0 + lane], kp1 = a.k_pos32[key0 + 32 + lane];
-        const bool docs = a.k_doc32 != nullptr;
-        const int kd0 = docs ? a.k_doc32[key0 + lane] : 0;
-        const int kd1 = docs ? a.k_doc32[key0 + 32 + lane] : 0;
-        visible_keys(mask, kp0, kp1, kd0, kd1, docs, vis0, vis1);
+      // ------------------------------------------------------------- softmax
+      const uint32_t lane_base = static_cast<uint32_t>(warp & 3) << 21;
+      constexpr int kKeys = kTileN / 2;  // of this thread
+      const uint32_t s_addr = tmem + lane_base + x * kTileN;
+      const uint32_t o_addr = tmem + lane_base + 2 * kTileN + x * D + half * (D / 2);
+      float *xch = reinterpret_cast<float *>(smem + L::kXch) + x * 2 * kTileM;
+      float *mine = xch + half * kTileM + row_in_tile;
+      const float *other = xch + (1 - half) * kTileM + row_in_tile;
+      float m = -INFINITY, l = 0.f;
+      const float slope = kBias && ref.valid ? a.slopes[ref.head] * kLog2e : 0.f;
+      long long q_place = 0;  // position behind the prefix, for the distance bias
+      if (!kDense && kBias && ref.valid) {
+        const int b = ref.token / a.q_len;
+        q_place = a.prefix_len + max(0, a.own_lens[b]) - a.q_len + (ref.token - b * a.q_len);
       }
-      uint32_t bad = 0;  // pages of this tile that lie outside the cache
-      if (!kDense) {
-        const int boxes = max(1, kTileN / a.block_size);
-        bool out_of_cache = false;
-        if (lane < boxes) {
-          const int page =
-              a.pages[(tile * kTileN + lane * min(kTileN, a.block_size)) / a.block_size];
-          out_of_cache = page < 0 || page >= a.num_blocks;
-          if (out_of_cache) report_status(a.status, kStatusBadSlot, -1, tile, page);
+      cp_async_commit();
+      cp_async_wait<0>();
+      fence_proxy_async_smem();
+      mbar_arrive(q_full);
+      int tile, j = 0;
+      bool whole, ok = true;
+      while (scan.next(tile, whole)) {
+        const int key0 = tile * kTileN + half * kKeys;
+        // masks while the scores are computed
+        uint32_t vis0 = 0xffffffffu, vis1 = 0xffffffffu;
+        if (kDense && !whole) {
+          const int kp0 = a.k_pos32[key0 + lane], kp1 = a.k_pos32[key0 + 32 + lane];
+          const bool docs = a.k_doc32 != nullptr;
+          const int kd0 = docs ? a.k_doc32[key0 + lane] : 0;
+          const int kd1 = docs ? a.k_doc32[key0 + 32 + lane] : 0;
+          visible_keys(mask, kp0, kp1, kd0, kd1, docs, vis0, vis1);
         }
-        bad = __ballot_sync(0xffffffffu, out_of_cache);
-      }
-      ok = wait_or_stop(&s_full[x], j & 1, stopped);
-      tc_fence_after();
-      float s[kKeys];
-#pragma unroll
-      for (int c = 0; c < kKeys / 32; ++c)
-        tmem_ld32(s_addr + half * kKeys + c * 32, reinterpret_cast<uint32_t(&)[32]>(s[c * 32]));
-      tmem_wait_ld();
-      // x = s c in log2 units, unless it is only scaled (then c goes into exp2)
-      if (kCap) {
-        // tanh by an odd polynomial while every score of the warp's rows is small
-        // against the cap, as they mostly are: four FMA slots a score instead of
-        // the exponential and reciprocal of tanh(u) = 1 - 2 / (1 + e^2u)
-        float big = 0.f;
-#pragma unroll
-        for (int i = 0; i < kKeys; i += 2)
-          big = fmaxf(fmaxf(big, fabsf(s[i])), fabsf(s[i + 1]));
-        if (__all_sync(0xffffffffu, big <= a.cap_small)) {
-          f32x2 k[5];
-          const f32x2 cap_u = pack2(a.cap_u, a.cap_u);
-#pragma unroll
-          for (int i = 0; i < 5; ++i) k[i] = pack2(a.cap_poly[i].x, a.cap_poly[i].y);
-#pragma unroll
-          for (int i = 0; i < kKeys; i += 2) {
-            const f32x2 v = pack2(s[i], s[i + 1]), u = mul2(v, cap_u), w = mul2(u, u);
-            unpack2(mul2(v, fma2(fma2(fma2(fma2(k[4], w, k[3]), w, k[2]), w, k[1]), w, k[0])),
-                    s[i], s[i + 1]);
+        uint32_t bad = 0;  // pages of this tile that lie outside the cache
+        if (!kDense) {
+          const int boxes = max(1, kTileN / a.block_size);
+          bool out_of_cache = false;
+          if (lane < boxes) {
+            const int page =
+                a.pages[(tile * kTileN + lane * min(kTileN, a.block_size)) / a.block_size];
+            out_of_cache = page < 0 || page >= a.num_blocks;
+            if (out_of_cache) report_status(a.status, kStatusBadSlot, -1, tile, page);
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < kKeys; ++i)
-            s[i] = fmaf(rcp(1.f + ex2(s[i] * a.cap_in)), -2.f * a.cap_out, a.cap_out);
+          bad = __ballot_sync(0xffffffffu, out_of_cache);
         }
-      } else if (kBias) {
+        ok = wait_or_stop(&s_full[x], j & 1, stopped);
+        tc_fence_after();
+        float s[kKeys];
 #pragma unroll
-        for (int i = 0; i < kKeys; ++i) s[i] *= a.scale_log2;
-      }
-      float lift = 0.f;  // what all scores of this row and tile still lack
-      if (kBias) {
-        // -slope |p - p_j|; for keys one apart at or before the row, slope j plus
-        // a constant (what else is in the tile is masked)
-        bool run = true;
-        float at;  // the row's place counted from this thread's first key
-        if (kDense) {
-          run = a.k_run[tile] != 0;
-          at = static_cast<float>(static_cast<long long>(mask.pos) - a.stats[tile].pos_min) -
-               (run ? static_cast<float>(half * kKeys) : 0.f);
-        } else {
-          at = static_cast<float>(q_place - key0);
-        }
-        const bool before = kDense ? mask.limit <= mask.pos + 1 || at >= kKeys : at >= kKeys - 1;
-        if (run && __all_sync(0xffffffffu, before || !ref.valid)) {
-          lift = -slope * at;
-          const f32x2 sl = pack2(slope, slope), two = pack2(2.f, 2.f);
-          f32x2 n = pack2(0.f, 1.f);
-#pragma unroll
-          for (int i = 0; i < kKeys; i += 2) {
-            unpack2(fma2(sl, n, pack2(s[i], s[i + 1])), s[i], s[i + 1]);
-            n = add2(n, two);
-          }
-        } else if (run) {
-#pragma unroll
-          for (int i = 0; i < kKeys; ++i)
-            s[i] = fmaf(-slope, fabsf(at - static_cast<float>(i)), s[i]);
-        } else {
-          const float4 *rel = reinterpret_cast<const float4 *>(a.k_rel + key0);
-#pragma unroll
-          for (int i = 0; i < kKeys / 4; ++i) {
-            const float4 p = rel[i];
-            s[4 * i] = fmaf(-slope, fabsf(at - p.x), s[4 * i]);
-            s[4 * i + 1] = fmaf(-slope, fabsf(at - p.y), s[4 * i + 1]);
-            s[4 * i + 2] = fmaf(-slope, fabsf(at - p.z), s[4 * i + 2]);
-            s[4 * i + 3] = fmaf(-slope, fabsf(at - p.w), s[4 * i + 3]);
-          }
-        }
-      }
-      if (kDense && !whole) {
-        if (__any_sync(0xffffffffu, vis0 != 0xffffffffu)) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (!((vis0 >> i) & 1)) s[i] = -INFINITY;
-        }
-        if (__any_sync(0xffffffffu, vis1 != 0xffffffffu)) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (!((vis1 >> i) & 1)) s[32 + i] = -INFINITY;
-        }
-      }
-      if (!kDense && bad) {
-        const int rows_of = min(kTileN, a.block_size);
-#pragma unroll
-        for (int i = 0; i < kKeys; ++i)
-          if ((bad >> ((half * kKeys + i) / rows_of)) & 1) s[i] = -INFINITY;
-      }
-      const float c = kCap || kBias ? 1.f : a.scale_log2;
-      float t0 = s[0], t1 = s[1], t2 = s[2], t3 = s[3];
-#pragma unroll
-      for (int i = 4; i + 7 < kKeys; i += 8) {
-        t0 = fmaxf(fmaxf(t0, s[i]), s[i + 1]);
-        t1 = fmaxf(fmaxf(t1, s[i + 2]), s[i + 3]);
-        t2 = fmaxf(fmaxf(t2, s[i + 4]), s[i + 5]);
-        t3 = fmaxf(fmaxf(t3, s[i + 6]), s[i + 7]);
-      }
-      t0 = fmaxf(fmaxf(t0, s[kKeys - 4]), s[kKeys - 3]);
-      t1 = fmaxf(fmaxf(t1, s[kKeys - 2]), s[kKeys - 1]);
-      const float top = fmaf(fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)), c, lift);
-      // O is rescaled when a row's maximum has grown (also at its first finite
-      // score), by both of its threads alike.  The meeting also keeps a warp from
-      // writing weights over scores that the other has not read.
-      if (pair_any(x, warp & 3, top > m + kLazy || !ok)) {
-        *mine = top;
-        if (pair_any(x, warp & 3, !ok)) {
-          ok = false;
-          break;
-        }
-        const float both = fmaxf(top, *other);
-        const bool grow = both > m + kLazy;
-        const float to = grow ? both : m;
-        const float keep = grow ? ex2(m - to) : 1.f;
-        m = to;
-        l *= keep;
-        if (j > 0) {  // the score barrier also covers the last product into O
-#pragma unroll 1
-          for (int k = 0; k < D / 64; ++k) {
-            uint32_t o[32];
-            tmem_ld32(o_addr + k * 32, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
-            tmem_st32(o_addr + k * 32, o);
-          }
-        }
-      }
-      const float off = (m == -INFINITY ? 0.f : m) - lift;
-      const f32x2 c2 = pack2(c, c), off2 = pack2(-off, -off);
-      f32x2 l0 = pack2(0.f, 0.f), l1 = l0;
-      // the weights of 32 keys, some of them by the polynomial; the product may
-      // start with the first 32
-      auto weights = [&](int part, auto some_fma) {
-        uint32_t p[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int k = part * 32 + 2 * i;
-          const f32x2 v = fma2(pack2(s[k], s[k + 1]), c2, off2);
-          float e, f;
-          if (decltype(some_fma)::value && i % 8 >= 8 - kFmaOf8) {
-            exp2_fma(v, e, f);
-          } else {
-            unpack2(v, e, f);
-            e = ex2(e), f = ex2(f);
-          }
-          if (i & 1)
-            l1 = add2(l1, pack2(e, f));
-          else
-            l0 = add2(l0, pack2(e, f));
-          p[i] = pair_from_float<T>(e, f);
-        }
-        tmem_st16(s_addr + half * (kKeys / 2) + part * 16, p);
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(part == 0 ? &p_half[x] : &p_full[x]);
-      };
-      if (whole)
-        weights(0, Yes{}), weights(1, Yes{});
-      else
-        weights(0, No{}), weights(1, No{});
-      float u0, u1;
-      unpack2(add2(l0, l1), u0, u1);
-      l += u0 + u1;
-      ++j;
-    }
-    // ------------------------------------------------------------- result
-    if (ok && j > 0) ok = wait_or_stop(&o_done[x], 0, stopped);
-    tc_fence_after();
-    if (ok || j == 0) *mine = l;  // (after a break nobody reads it)
-    ok = !tile_any(x, !ok);
-    if (ok) l += *other;
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : NAN);
-    const long long row = row_at[row_in_tile];
-    bool finite = true;
-    // 64 columns at a time (32 of each half) through the tile's share of Q's
-    // memory, so that stores to the rows run along them
-    uint8_t *stage = smem + L::kQ + x * L::kQTile;
-#pragma unroll 1
-    for (int k = 0; k < D / 64; ++k) {
-      float o[32];
-      if (ok && j > 0) {
-        tmem_ld32(o_addr + k * 32, reinterpret_cast<uint32_t(&)[32]>(o));
+        for (int c = 0; c < kKeys / 32; ++c)
+          tmem_ld32(s_addr + half * kKeys + c * 32, reinterpret_cast<uint32_t(&)[32]>(s[c * 32]));
         tmem_wait_ld();
-      }
+        // x = s c in log2 units, unless it is only scaled (then c goes into exp2)
+        if (kCap) {
+          // tanh by an odd polynomial while every score of the warp's rows is small
+          // against the cap, as they mostly are: four FMA slots a score instead of
+          // the exponential and reciprocal of tanh(u) = 1 - 2 / (1 + e^2u)
+          float big = 0.f;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        o[i] = ok ? (j > 0 ? o[i] * inv : 0.f) : NAN;
-        finite = finite && fabsf(o[i]) <= 3.4028235e38f;
-      }
-      const int swz = row_in_tile & 7;
-      if (a.slices == 0) {
-        uint8_t *w = stage + row_in_tile * 128;
+          for (int i = 0; i < kKeys; i += 2)
+            big = fmaxf(fmaxf(big, fabsf(s[i])), fabsf(s[i + 1]));
+          if (__all_sync(0xffffffffu, big <= a.cap_small)) {
+            f32x2 k[5];
+            const f32x2 cap_u = pack2(a.cap_u, a.cap_u);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          int4 v;
-          v.x = pair_from_float<T>(o[8 * i], o[8 * i + 1]);
-          v.y = pair_from_float<T>(o[8 * i + 2], o[8 * i + 3]);
-          v.z = pair_from_float<T>(o[8 * i + 4], o[8 * i + 5]);
-          v.w = pair_from_float<T>(o[8 * i + 6], o[8 * i + 7]);
-          *reinterpret_cast<int4 *>(w + (((half * 4 + i) ^ swz) << 4)) = v;
+            for (int i = 0; i < 5; ++i) k[i] = pack2(a.cap_poly[i].x, a.cap_poly[i].y);
+#pragma unroll
+            for (int i = 0; i < kKeys; i += 2) {
+              const f32x2 v = pack2(s[i], s[i + 1]), u = mul2(v, cap_u), w = mul2(u, u);
+              unpack2(mul2(v, fma2(fma2(fma2(fma2(k[4], w, k[3]), w, k[2]), w, k[1]), w, k[0])),
+                      s[i], s[i + 1]);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i)
+              s[i] = fmaf(rcp(1.f + ex2(s[i] * a.cap_in)), -2.f * a.cap_out, a.cap_out);
+          }
+        } else if (kBias) {
+#pragma unroll
+          for (int i = 0; i < kKeys; ++i) s[i] *= a.scale_log2;
         }
-      } else {
-        uint8_t *w = stage + half * kHalfBytes + row_in_tile * 128;
+        float lift = 0.f;  // what all scores of this row and tile still lack
+        if (kBias) {
+          // -slope |p - p_j|; for keys one apart at or before the row, slope j plus
+          // a constant (what else is in the tile is masked)
+          bool run = true;
+          float at;  // the row's place counted from this thread's first key
+          if (kDense) {
+            run = a.k_run[tile] != 0;
+            at = static_cast<float>(static_cast<long long>(mask.pos) - a.stats[tile].pos_min) -
+                 (run ? static_cast<float>(half * kKeys) : 0.f);
+          } else {
+            at = static_cast<float>(q_place - key0);
+          }
+          const bool before = kDense ? mask.limit <= mask.pos + 1 || at >= kKeys : at >= kKeys - 1;
+          if (run && __all_sync(0xffffffffu, before || !ref.valid)) {
+            lift = -slope * at;
+            const f32x2 sl = pack2(slope, slope), two = pack2(2.f, 2.f);
+            f32x2 n = pack2(0.f, 1.f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          *reinterpret_cast<float4 *>(w + ((i ^ swz) << 4)) =
-              make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-      }
-      tile_any(x, false);
-      const int in_tile = tid & (kTileThreads - 1);
-      if (a.slices == 0) {
+            for (int i = 0; i < kKeys; i += 2) {
+              unpack2(fma2(sl, n, pack2(s[i], s[i + 1])), s[i], s[i + 1]);
+              n = add2(n, two);
+            }
+          } else if (run) {
 #pragma unroll
-        for (int i = 0; i < kTileM * 8 / kTileThreads; ++i) {
-          const int r = (in_tile >> 3) + i * (kTileThreads / 8), v = in_tile & 7;
-          if (row_at[r] < 0) continue;
-          st_v4(static_cast<T *>(a.out) + static_cast<long long>(row_at[r]) * D +
-                    (v >> 2) * (D / 2) + k * 32 + (v & 3) * 8,
-                *reinterpret_cast<const int4 *>(stage + r * 128 + ((v ^ (r & 7)) << 4)));
+            for (int i = 0; i < kKeys; ++i)
+              s[i] = fmaf(-slope, fabsf(at - static_cast<float>(i)), s[i]);
+          } else {
+            const float4 *rel = reinterpret_cast<const float4 *>(a.k_rel + key0);
+#pragma unroll
+            for (int i = 0; i < kKeys / 4; ++i) {
+              const float4 p = rel[i];
+              s[4 * i] = fmaf(-slope, fabsf(at - p.x), s[4 * i]);
+              s[4 * i + 1] = fmaf(-slope, fabsf(at - p.y), s[4 * i + 1]);
+              s[4 * i + 2] = fmaf(-slope, fabsf(at - p.z), s[4 * i + 2]);
+              s[4 * i + 3] = fmaf(-slope, fabsf(at - p.w), s[4 * i + 3]);
+            }
+          }
         }
-      } else {
-        float *part = a.part_o + static_cast<long long>(slice) * a.tokens * a.heads * D;
+        if (kDense && !whole) {
+          if (__any_sync(0xffffffffu, vis0 != 0xffffffffu)) {
 #pragma unroll
-        for (int i = 0; i < kTileM * 16 / kTileThreads; ++i) {
-          const int r = (in_tile >> 4) + i * (kTileThreads / 16), v = in_tile & 15;
-          if (row_at[r] < 0) continue;
-          st_v4(part + static_cast<long long>(row_at[r]) * D + (v >> 3) * (D / 2) + k * 32 +
-                    (v & 7) * 4,
-                *reinterpret_cast<const int4 *>(stage + (v >> 3) * kHalfBytes + r * 128 +
-                                                (((v & 7) ^ (r & 7)) << 4)));
+            for (int i = 0; i < 32; ++i)
+              if (!((vis0 >> i) & 1)) s[i] = -INFINITY;
+          }
+          if (__any_sync(0xffffffffu, vis1 != 0xffffffffu)) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!((vis1 >> i) & 1)) s[32 + i] = -INFINITY;
+          }
         }
+        if (!kDense && bad) {
+          const int rows_of = min(kTileN, a.block_size);
+#pragma unroll
+          for (int i = 0; i < kKeys; ++i)
+            if ((bad >> ((half * kKeys + i) / rows_of)) & 1) s[i] = -INFINITY;
+        }
+        const float c = kCap || kBias ? 1.f : a.scale_log2;
+        float t0 = s[0], t1 = s[1], t2 = s[2], t3 = s[3];
+#pragma unroll
+        for (int i = 4; i + 7 < kKeys; i += 8) {
+          t0 = fmaxf(fmaxf(t0, s[i]), s[i + 1]);
+          t1 = fmaxf(fmaxf(t1, s[i + 2]), s[i + 3]);
+          t2 = fmaxf(fmaxf(t2, s[i + 4]), s[i + 5]);
+          t3 = fmaxf(fmaxf(t3, s[i + 6]), s[i + 7]);
+        }
+        t0 = fmaxf(fmaxf(t0, s[kKeys - 4]), s[kKeys - 3]);
+        t1 = fmaxf(fmaxf(t1, s[kKeys - 2]), s[kKeys - 1]);
+        const float top = fmaf(fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)), c, lift);
+        // O is rescaled when a row's maximum has grown (also at its first finite
+        // score), by both of its threads alike.  The meeting also keeps a warp from
+        // writing weights over scores that the other has not read.
+        if (pair_any(x, warp & 3, top > m + kLazy || !ok)) {
+          *mine = top;
+          if (pair_any(x, warp & 3, !ok)) {
+            ok = false;
+            break;
+          }
+          const float both = fmaxf(top, *other);
+          const bool grow = both > m + kLazy;
+          const float to = grow ? both : m;
+          const float keep = grow ? ex2(m - to) : 1.f;
+          m = to;
+          l *= keep;
+          if (j > 0) {  // the score barrier also covers the last product into O
+#pragma unroll 1
+            for (int k = 0; k < D / 64; ++k) {
+              uint32_t o[32];
+              tmem_ld32(o_addr + k * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+              tmem_st32(o_addr + k * 32, o);
+            }
+          }
+        }
+        const float off = (m == -INFINITY ? 0.f : m) - lift;
+        const f32x2 c2 = pack2(c, c), off2 = pack2(-off, -off);
+        f32x2 l0 = pack2(0.f, 0.f), l1 = l0;
+        // the weights of 32 keys, some of them by the polynomial; the product may
+        // start with the first 32
+        auto weights = [&](int part, auto some_fma) {
+          uint32_t p[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int k = part * 32 + 2 * i;
+            const f32x2 v = fma2(pack2(s[k], s[k + 1]), c2, off2);
+            float e, f;
+            if (decltype(some_fma)::value && i % 8 >= 8 - kFmaOf8) {
+              exp2_fma(v, e, f);
+            } else {
+              unpack2(v, e, f);
+              e = ex2(e), f = ex2(f);
+            }
+            if (i & 1)
+              l1 = add2(l1, pack2(e, f));
+            else
+              l0 = add2(l0, pack2(e, f));
+            p[i] = pair_from_float<T>(e, f);
+          }
+          tmem_st16(s_addr + half * (kKeys / 2) + part * 16, p);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(part == 0 ? &p_half[x] : &p_full[x]);
+        };
+        if (whole)
+          weights(0, Yes{}), weights(1, Yes{});
+        else
+          weights(0, No{}), weights(1, No{});
+        float u0, u1;
+        unpack2(add2(l0, l1), u0, u1);
+        l += u0 + u1;
+        ++j;
       }
-      if (k + 1 < D / 64) tile_any(x, false);
-    }
-    if (ref.valid && half == 0) {
-      if (a.slices == 0) {
-        if (a.lse) a.lse[row] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
-      } else {
-        a.part_lse[static_cast<long long>(slice) * a.tokens * a.heads + row] =
-            l == 0.f ? -INFINITY : m + log2f(l);
-      }
-    }
-    if (kDense && a.slices == 0 && ok) {
-      const bool wrong = ref.valid && !finite;
-      if (tile_any(x, wrong)) {  // what was written above is written again below
-        *mine = wrong ? 1.f : 0.f;
+      // ------------------------------------------------------------- result
+      if (ok && j > 0) ok = wait_or_stop(&o_done[x], 0, stopped);
+      tc_fence_after();
+      if (ok || j == 0) *mine = l;  // (after a break nobody reads it)
+      ok = !tile_any(x, !ok);
+      if (ok) l += *other;
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : NAN);
+      const long long row = row_at[row_in_tile];
+      bool finite = true;
+      // 64 columns at a time (32 of each half) through the tile's share of Q's
+      // memory, so that stores to the rows run along them
+      uint8_t *stage = smem + L::kQ + x * L::kQTile;
+#pragma unroll 1
+      for (int k = 0; k < D / 64; ++k) {
+        float o[32];
+        if (ok && j > 0) {
+          tmem_ld32(o_addr + k * 32, reinterpret_cast<uint32_t(&)[32]>(o));
+          tmem_wait_ld();
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          o[i] = ok ? (j > 0 ? o[i] * inv : 0.f) : NAN;
+          finite = finite && fabsf(o[i]) <= 3.4028235e38f;
+        }
+        const int swz = row_in_tile & 7;
+        if (a.slices == 0) {
+          uint8_t *w = stage + row_in_tile * 128;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            int4 v;
+            v.x = pair_from_float<T>(o[8 * i], o[8 * i + 1]);
+            v.y = pair_from_float<T>(o[8 * i + 2], o[8 * i + 3]);
+            v.z = pair_from_float<T>(o[8 * i + 4], o[8 * i + 5]);
+            v.w = pair_from_float<T>(o[8 * i + 6], o[8 * i + 7]);
+            *reinterpret_cast<int4 *>(w + (((half * 4 + i) ^ swz) << 4)) = v;
+          }
+        } else {
+          uint8_t *w = stage + half * kHalfBytes + row_in_tile * 128;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<float4 *>(w + ((i ^ swz) << 4)) =
+                make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        }
         tile_any(x, false);
-        uint32_t again =
-            half == 0 ? __ballot_sync(0xffffffffu, *mine + *other > 0.f) : 0u;
-        while (again) {
-          const int src = __ffs(again) - 1;
-          again &= again - 1;
-          strict_position_row<T, D>(a.pos, __shfl_sync(0xffffffffu, ref.token, src),
-                                    __shfl_sync(0xffffffffu, ref.head, src));
+        const int in_tile = tid & (kTileThreads - 1);
+        if (a.slices == 0) {
+#pragma unroll
+          for (int i = 0; i < kTileM * 8 / kTileThreads; ++i) {
+            const int r = (in_tile >> 3) + i * (kTileThreads / 8), v = in_tile & 7;
+            if (row_at[r] < 0) continue;
+            st_v4(static_cast<T *>(a.out) + static_cast<long long>(row_at[r]) * D +
+                      (v >> 2) * (D / 2) + k * 32 + (v & 3) * 8,
+                  *reinterpret_cast<const int4 *>(stage + r * 128 + ((v ^ (r & 7)) << 4)));
+          }
+        } else {
+          float *part = a.part_o + static_cast<long long>(slice) * a.tokens * a.heads * D;
+#pragma unroll
+          for (int i = 0; i < kTileM * 16 / kTileThreads; ++i) {
+            const int r = (in_tile >> 4) + i * (kTileThreads / 16), v = in_tile & 15;
+            if (row_at[r] < 0) continue;
+            st_v4(part + static_cast<long long>(row_at[r]) * D + (v >> 3) * (D / 2) + k * 32 +
+                      (v & 7) * 4,
+                  *reinterpret_cast<const int4 *>(stage + (v >> 3) * kHalfBytes + r * 128 +
+                                                  (((v & 7) ^ (r & 7)) << 4)));
+          }
+        }
+        if (k + 1 < D / 64) tile_any(x, false);
+      }
+      if (ref.valid && half == 0) {
+        if (a.slices == 0) {
+          if (a.lse) a.lse[row] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+        } else {
+          a.part_lse[static_cast<long long>(slice) * a.tokens * a.heads + row] =
+              l == 0.f ? -INFINITY : m + log2f(l);
         }
       }
-    }
+      if (kDense && a.slices == 0 && ok) {
+        const bool wrong = ref.valid && !finite;
+        if (tile_any(x, wrong)) {  // what was written above is written again below
+          *mine = wrong ? 1.f : 0.f;
+          tile_any(x, false);
+          uint32_t again =
+              half == 0 ? __ballot_sync(0xffffffffu, *mine + *other > 0.f) : 0u;
+          while (again) {
+            const int src = __ffs(again) - 1;
+            again &= again - 1;
+            strict_position_row<T, D>(a.pos, __shfl_sync(0xffffffffu, ref.token, src),
+                                      __shfl_sync(0xffffffffu, ref.head, src));
+          }
+        }
+      }
     }
   }
   tc_fence_before();
