@@ -138,14 +138,14 @@ cudaError_t launch_ordered(void (*kernel)(Params...), dim3 grid, unsigned thread
   return cudaLaunchKernelEx(&config, kernel, Params(args)...);
 }
 
-template <typename T, int D, bool kDense>
+template <typename T, int D, bool kDense, bool kDocs>
 cudaError_t launch_tc(const CUtensorMap &k_map, const CUtensorMap &v_map, const TcArgs &t,
                       unsigned grid, bool first, cudaStream_t stream) {
   const bool cap = t.cap_out > 0.f, bias = t.slopes != nullptr;
-  auto kernel = cap ? (bias ? tc_attention_kernel<T, D, kDense, true, true>
-                            : tc_attention_kernel<T, D, kDense, true, false>)
-                    : (bias ? tc_attention_kernel<T, D, kDense, false, true>
-                            : tc_attention_kernel<T, D, kDense, false, false>);
+  auto kernel = cap ? (bias ? tc_attention_kernel<T, D, kDense, kDocs, true, true>
+                            : tc_attention_kernel<T, D, kDense, kDocs, true, false>)
+                    : (bias ? tc_attention_kernel<T, D, kDense, kDocs, false, true>
+                            : tc_attention_kernel<T, D, kDense, kDocs, false, false>);
   constexpr int kBytes = TcSmem<D>::kBytes;
   cudaError_t e = allow_smem(kernel, kBytes);
   if (e != cudaSuccess) return e;

@@ -126,7 +126,8 @@ cudaError_t launch(const PositionArgs &a, void *workspace, cudaStream_t stream) 
       !encode_rows(&v_map, kBf16, a.v, 3, dims, vs, box))
     return cudaErrorInvalidValue;
   const unsigned grid = static_cast<unsigned>(p.groups) * a.kv_heads * std::max(1, p.slices);
-  cudaError_t e = launch_tc<T, D, true>(k_map, v_map, t, grid, false, stream);
+  cudaError_t e = t.k_doc32 ? launch_tc<T, D, true, true>(k_map, v_map, t, grid, false, stream)
+                            : launch_tc<T, D, true, false>(k_map, v_map, t, grid, false, stream);
   if (e != cudaSuccess || !p.slices) return e;
   return launch_ordered(join_position_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128,
                         0, false, stream, 1, a, t.part_o, t.part_lse, p.slices);

@@ -95,7 +95,7 @@ cudaError_t launch(const PagedArgs &a, void *workspace, cudaStream_t stream) {
         !encode_rows(&v_map, kBf16, a.v, 4, dims, vs, box))
       return cudaErrorInvalidValue;
     const unsigned grid = static_cast<unsigned>(p.groups) * a.kv_heads * p.tc_slices;
-    e = launch_tc<T, D, false>(k_map, v_map, t, grid, true, stream);
+    e = launch_tc<T, D, false, false>(k_map, v_map, t, grid, true, stream);
     if (e != cudaSuccess) return e;
   }
   int first = p.tc_slices;
