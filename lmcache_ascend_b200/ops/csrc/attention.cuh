@@ -105,8 +105,8 @@ struct WarpRow {
     x *= scale;
     if (cap > 0.f) x = cap * tanhf(x / cap);
     x = (x - bias) * kLog2e;
-    const float top = fmaxf(m, x);
-    if (top == -INFINITY) return;  // a score of -inf before any other
+    if (x == -INFINITY && m == -INFINITY) return;  // before any other score
+    const float top = fmaxf(m, x);  // (a NaN score leaves m and makes its weight NaN)
     const float keep = exp2f(m - top), w = exp2f(x - top);
     m = top;
     l = l * keep + w;

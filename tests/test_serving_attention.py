@@ -500,6 +500,68 @@ def test_position_kernel_masked_keys_hold_anything(value, Tq, H, D, T):
     _check(got[keep.cuda()], lse[keep.cuda()], o[keep], e[keep], tol[keep], tl[keep])
 
 
+# Dense calls of every form: one part, parts joined in a cluster and in memory, the
+# tensor-core kernel whole and in slices.
+FORMS = [(20, 200, 8, 2, 64), (20, 300, 4, 2, 128), (1, 6000, 4, 2, 64), (400, 700, 16, 2, 128),
+         (500, 850, 16, 2, 64), (300, 3000, 16, 2, 64)]
+# ... and paged: B, Tq, H, KH, D, P
+PAGED_FORMS = [(3, 1, 8, 2, 64, 20), (2, 1, 8, 2, 64, 500), (1, 1, 8, 2, 128, 6000),
+               (30, 1, 32, 2, 128, 1000), (40, 1, 32, 2, 64, 1700)]
+
+
+def _check_with_nan(got, lse, want):
+    """NaN exactly where the oracle has it, the others within the tolerance."""
+    o, e, tol, tl = want
+    hit = torch.isnan(e)
+    assert torch.equal(torch.isnan(lse.cpu()), hit)
+    assert bool(torch.isnan(got.cpu()[hit]).all())
+    _check(got.cpu()[~hit], lse.cpu()[~hit], o[~hit], e[~hit], tol[~hit], tl[~hit])
+    return hit
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("where", ["query", "first key"])
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_position_kernel_nan_scores_reach_their_rows(form, where):
+    Tq, Tk, H, KH, D = form
+    q, k, v, qp, kp, kw = _position_case(Tq, Tk, H, KH, D, BF, "subset")
+    if where == "query":
+        q[Tq // 2, 1, 5] = math.nan
+    else:
+        k[0, 0, 7] = math.nan  # every row sees key 0
+
+    def ref(q_, k_, v_):
+        return R.position_attention_ref(q_, k_, v_, qp, kp, D ** -0.5, compute=torch.float64)
+
+    want = _bounds(ref, q, k, v, BF, D ** -0.5, 0.0, None, Tk)
+    hit = _check_with_nan(*_run_position(q, k, v, qp, kp, kw, BF, 0.0, None), want)
+    assert int(hit.sum()) == (1 if where == "query" else Tq * H // KH)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("where", ["query", "first key", "first own key"])
+@pytest.mark.parametrize("form", PAGED_FORMS, ids=str)
+def test_prefix_kernel_nan_scores_reach_their_rows(form, where):
+    B, Tq, H, KH, D, P = form
+    q, kc, vc, prefix, tables, lens = _prefix_case(B, Tq, H, KH, D, 16, P, [20] * B, FP)
+    if where == "query":
+        q[B // 2, 1, 5] = math.nan
+    else:
+        page = prefix[0] if where == "first key" else tables[B - 1, 0]
+        kc[int(page), 0, 0, 7] = math.nan
+
+    def ref(q_, k_, v_):
+        return R.shared_prefix_attention_ref(q_, k_, v_, prefix, P, tables, lens, D ** -0.5,
+                                             compute=torch.float64)
+
+    want = _bounds(ref, q, kc, vc, FP, D ** -0.5, 0.0, None, P + 20)
+    got, lse = api.shared_prefix_attention(q.cuda(), kc.cuda(), vc.cuda(), prefix.cuda(), P,
+                                           tables.cuda(), lens.cuda(), return_lse=True)
+    hit = _check_with_nan(got, lse, want)
+    assert int(hit.sum()) == (1 if where == "query" else
+                              (B if where == "first key" else 1) * H // KH)
+
+
 @pytest.mark.gpu
 def test_position_kernel_unaligned_rows_and_far_positions():
     q, k, v, qp, kp, kw = _position_case(100, 300, 4, 2, 64, BF, "subset")
