@@ -6,6 +6,7 @@
 #include <tuple>
 
 #include "mem_kernels.h"
+#include "serving_ops.h"
 
 namespace lmc {
 // mem_alloc.cpp
@@ -242,6 +243,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rotary_embedding_and_cache", &rotary_embedding_and_cache);
   m.def("shared_prefix_attention", &shared_prefix_attention);
   m.def("position_attention", &position_attention);
+  m.def("log2_of_sum", &log2_of_sum);
 
   m.def("layerwise_prefill_dma_copy", &dma_copy_batch);
   m.def("layerwise_prefill_dma_copy_diagnose", &dma_copy_batch_timed);

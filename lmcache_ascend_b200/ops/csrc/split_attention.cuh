@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
         reinterpret_cast<float2 *>(part_o + at)[e] = make_float2(acc[2 * e], acc[2 * e + 1]);
     }
     if (lane == 0) {
-      const float log2_sum = l == 0.f ? -INFINITY : m + log2f(l);
+      const float log2_sum = log2_of_sum(true, m, l);
       if (!direct) part_lse[row] = log2_sum;
       else if (a.lse) a.lse[row] = log2_sum * kLn2;
     }

@@ -796,13 +796,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       if (ref.valid && half == 0) {
         if (a.slices == 0) {
-          if (a.lse) a.lse[row] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+          if (a.lse) a.lse[row] = log2_of_sum(ok, m, l) * kLn2;
         } else {
           a.part_lse[static_cast<long long>(slice) * a.tokens * a.heads + row] =
-              l == 0.f ? -INFINITY : m + log2f(l);
+              log2_of_sum(ok, m, l);
         }
       }
-      if (kDense && a.slices == 0 && ok) {
+      if (!ok && row_in_tile == 0 && half == 0)
+        report_status(a.status, kStatusMbarTimeout, kv_head, row_group, slice);
+      if (kDense && a.slices == 0) {
         const bool wrong = ref.valid && !finite;
         if (tile_any(x, wrong)) {  // what was written above is written again below
           *mine = wrong ? 1.f : 0.f;

@@ -129,6 +129,16 @@ def test_cpu_forms_and_refusals():
         api.position_attention(q[0], k, k, torch.tensor([0, 4]))
 
 
+@pytest.mark.skipif(not ops.native_available(), reason="native module not built")
+def test_part_whose_wait_ran_out_is_not_taken_for_an_empty_one():
+    """A join leaves parts of -inf out; a NaN makes it compute the row again."""
+    log = ops.native().log2_of_sum
+    assert log(True, -math.inf, 0.0) == -math.inf
+    assert log(True, 3.0, 0.25) == 1.0
+    for m, l in ((-math.inf, 0.0), (3.0, 0.25), (3.0, 0.0)):
+        assert math.isnan(log(False, m, l))
+
+
 # ------------------------------------------------------------ shared prefix
 def _prefix_case(B, Tq, H, KH, D, bs, P, own, dtype, seed=0, layout="plain", junk=math.nan):
     """A paged batch whose unused slots hold ``junk``."""
