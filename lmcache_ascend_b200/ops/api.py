@@ -698,7 +698,8 @@ def shared_prefix_attention(query: torch.Tensor, key_cache: torch.Tensor,
     the distance (fp32 [H]).
 
     Returns [B, ..., H, D] and, with ``return_lse``, the fp32 log of each row's
-    sum.  A row that sees no key is zero with -inf.  Keys in a block outside the
+    sum.  A row that sees no key is zero with -inf; one whose scores are all -inf
+    is NaN.  Keys in a block outside the
     cache, or past the end of a table row, are left out and reported in
     ``status``.  On the device: bfloat16 or float16, D of 64 or 128, 16-byte
     aligned cache rows, forward only.
@@ -743,7 +744,8 @@ def position_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
     :func:`shared_prefix_attention`.
 
     Returns [Tq, H, D] and, with ``return_lse``, the fp32 log of each row's sum;
-    a row that sees no key is zero with -inf.  On the device: bfloat16 or
+    a row that sees no key is zero with -inf, one whose scores are all -inf is
+    NaN.  On the device: bfloat16 or
     float16, D of 64 or 128, forward only.
     """
     if scale is None:

@@ -6,7 +6,8 @@
 //   x_j = x_j - slope_h * |p - p_j|                            (distance bias)
 //   o = sum_j exp(x_j - lse) v_j,   lse = log sum_j exp(x_j)
 // with every sum and statistic in fp32 and one rounding of o to the row's type.
-// A row that sees no key is zero with lse = -inf.  Keys it does not see are
+// A row that sees no key is zero with lse = -inf; one whose scores are all -inf has
+// no weights and is NaN.  Keys it does not see are
 // never multiplied by a zero weight: whatever their rows hold stays out.
 #pragma once
 #include <cuda_bf16.h>
@@ -73,6 +74,7 @@ template <typename T, int D>
 struct WarpRow {
   static constexpr int E = D / 32;
   float q[E], o[E], m, l;
+  bool lowest;  // there was a score of -inf before any other
 
   __device__ __forceinline__ void load(const T *p, float *f) const {
     const uint32_t *w = reinterpret_cast<const uint32_t *>(p + (threadIdx.x & 31) * E);
@@ -89,6 +91,7 @@ struct WarpRow {
     for (int i = 0; i < E; ++i) o[i] = 0.f;
     m = -INFINITY;
     l = 0.f;
+    lowest = false;
   }
 
   // bias is subtracted after the cap
@@ -105,7 +108,10 @@ struct WarpRow {
     x *= scale;
     if (cap > 0.f) x = cap * tanhf(x / cap);
     x = (x - bias) * kLog2e;
-    if (x == -INFINITY && m == -INFINITY) return;  // before any other score
+    if (x == -INFINITY && m == -INFINITY) {
+      lowest = true;
+      return;
+    }
     const float top = fmaxf(m, x);  // (a NaN score leaves m and makes its weight NaN)
     const float keep = exp2f(m - top), w = exp2f(x - top);
     m = top;
@@ -115,13 +121,14 @@ struct WarpRow {
   }
 
   __device__ __forceinline__ void finish(T *row, float *lse) const {
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    // scores of -inf only have no weights: NaN
+    const float inv = l == 0.f ? (lowest ? NAN : 0.f) : 1.f / l;
     uint32_t *w = reinterpret_cast<uint32_t *>(row + (threadIdx.x & 31) * E);
 #pragma unroll
     for (int i = 0; i < E / 2; ++i)
       w[i] = pair_from_float<T>(o[2 * i] * inv, o[2 * i + 1] * inv);
     if (lse != nullptr && (threadIdx.x & 31) == 0)
-      *lse = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+      *lse = l == 0.f ? (lowest ? NAN : -INFINITY) : m * kLn2 + logf(l);
   }
 };
 

@@ -13,10 +13,11 @@ constexpr int kDeviceStatusBytes = 24;
 
 // Base-2 log of a row's sum from its maximum m and the sum l of its weights; -inf
 // for a row without keys.  Such a part is left out of a join, so a row whose wait
-// ran out (`whole` false) must not have it even where l is still 0: its log is NaN,
-// and the join computes the row again.
+// ran out (`whole` false) must not have it even where l is still 0, nor one whose
+// scores are all -inf (it has weights, but no maximum): their log is NaN, and the
+// join computes the row again.
 __host__ __device__ inline float log2_of_sum(bool whole, float m, float l) {
-  if (!whole) return NAN;
+  if (!whole || (l != 0.f && m == -INFINITY)) return NAN;
   return l == 0.f ? -INFINITY : m + log2f(l);
 }
 

@@ -425,6 +425,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
              __reduce_max_sync(0xffffffffu, kp_all) < all_limit;
     else
       open = j0 + kSplitKeys <= all_last && bad_keys == 0;
+    bool sees0 = open, sees1 = open;  // one of this lane's keys
     if (!open) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -444,6 +445,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
           }
           if (out0) sc[t][e] = -INFINITY;
           if (out1) sc[t][2 + e] = -INFINITY;
+          sees0 = sees0 || !out0, sees1 = sees1 || !out1;
         }
       }
     }
@@ -463,7 +465,10 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
 #pragma unroll
       for (int d = 0; d < D / 8; ++d) o[d][0] *= f0, o[d][1] *= f0, o[d][2] *= f1, o[d][3] *= f1;
     }
-    const float off0 = m0 == -INFINITY ? 0.f : m0, off1 = m1 == -INFINITY ? 0.f : m1;
+    // no finite score yet: zero weights, or NaN ones for keys that are seen and have
+    // scores of -inf (they lead the row to the definition)
+    const float off0 = m0 == -INFINITY && !sees0 ? 0.f : m0;
+    const float off1 = m1 == -INFINITY && !sees1 ? 0.f : m1;
     uint32_t p[4];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {

@@ -527,6 +527,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           visible_keys(mask, kp0, kp1, kd0, kd1, kDocs, vis0, vis1);
         }
         uint32_t bad = 0;  // pages of this tile that lie outside the cache
+        bool some_page = true;
         if (!kDense) {
           const int boxes = max(1, kTileN / a.block_size);
           bool out_of_cache = false;
@@ -537,6 +538,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (out_of_cache) report_status(a.status, kStatusBadSlot, -1, tile, page);
           }
           bad = __ballot_sync(0xffffffffu, out_of_cache);
+          some_page = __popc(bad) < boxes;
         }
         ok = wait_or_stop(&s_full[x], j & 1, stopped);
         tc_fence_after();
@@ -679,7 +681,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
           }
         }
-        const float off = (m == -INFINITY ? 0.f : m) - lift;
+        // Without a finite score yet: zero weights for a row that sees no key of its
+        // half of this tile; one that does has only scores of -inf there, and NaN
+        // weights (-inf less -inf) lead it to the definition.
+        const bool sees = kDense ? whole || (vis0 | vis1) != 0 : some_page;
+        const float off = (m == -INFINITY && !sees ? 0.f : m) - lift;
         const f32x2 c2 = pack2(c, c), off2 = pack2(-off, -off);
         f32x2 l0 = pack2(0.f, 0.f), l1 = l0;
         // the weights of 32 keys, some of them by the polynomial; the product may

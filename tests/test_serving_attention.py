@@ -135,6 +135,7 @@ def test_part_whose_wait_ran_out_is_not_taken_for_an_empty_one():
     log = ops.native().log2_of_sum
     assert log(True, -math.inf, 0.0) == -math.inf
     assert log(True, 3.0, 0.25) == 1.0
+    assert math.isnan(log(True, -math.inf, 0.25))  # scores of -inf only
     for m, l in ((-math.inf, 0.0), (3.0, 0.25), (3.0, 0.0)):
         assert math.isnan(log(False, m, l))
 
@@ -570,6 +571,49 @@ def test_prefix_kernel_nan_scores_reach_their_rows(form, where):
     hit = _check_with_nan(got, lse, want)
     assert int(hit.sum()) == (1 if where == "query" else
                               (B if where == "first key" else 1) * H // KH)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_position_kernel_scores_of_minus_infinity(form):
+    """They take no part beside a finite score; a row that sees nothing else has
+    no weights: NaN, unlike a row that sees no key."""
+    Tq, Tk, H, KH, D = form
+    q, k, v, qp, kp, kw = _position_case(Tq, Tk, H, KH, D, BF, "subset")
+    q[..., 0] = 1.0
+    k[:Tk // 2, 0, 0] = -math.inf
+    qp[0] = Tk // 2 - 1
+    if Tq > 1:
+        qp[-1] = -1
+
+    def ref(q_, k_, v_):
+        return R.position_attention_ref(q_, k_, v_, qp, kp, D ** -0.5, compute=torch.float64)
+
+    want = _bounds(ref, q, k, v, BF, D ** -0.5, 0.0, None, Tk)
+    hit = _check_with_nan(*_run_position(q, k, v, qp, kp, kw, BF, 0.0, None), want)
+    sees = (qp >= 0) & (qp < Tk // 2)
+    assert int(hit.sum()) == int(sees.sum()) * H // KH
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", PAGED_FORMS, ids=str)
+def test_prefix_kernel_scores_of_minus_infinity(form):
+    B, Tq, H, KH, D, P = form
+    own = [20 + b % 9 for b in range(B)]
+    q, kc, vc, prefix, tables, lens = _prefix_case(B, Tq, H, KH, D, 16, P, own, BF)
+    q[..., 0] = 1.0
+    kc[prefix.long(), :, 0, 0] = -math.inf
+    kc[tables[B - 1, :2].long(), :, 0, 0] = -math.inf
+
+    def ref(q_, k_, v_):
+        return R.shared_prefix_attention_ref(q_, k_, v_, prefix, P, tables, lens, D ** -0.5,
+                                             compute=torch.float64)
+
+    want = _bounds(ref, q, kc, vc, BF, D ** -0.5, 0.0, None, P + 30)
+    got, lse = api.shared_prefix_attention(q.cuda(), kc.cuda(), vc.cuda(), prefix.cuda(), P,
+                                           tables.cuda(), lens.cuda(), return_lse=True)
+    hit = _check_with_nan(got, lse, want)
+    assert int(hit.sum()) == H // KH
 
 
 @pytest.mark.gpu
