@@ -467,8 +467,8 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
     }
     // no finite score yet: zero weights, or NaN ones for keys that are seen and have
     // scores of -inf (they lead the row to the definition)
-    const float off0 = m0 == -INFINITY && !sees0 ? 0.f : m0;
-    const float off1 = m1 == -INFINITY && !sees1 ? 0.f : m1;
+    const float off0 = (m0 == -INFINITY && !sees0 ? 0.f : m0) - kRaised<T>;
+    const float off1 = (m1 == -INFINITY && !sees1 ? 0.f : m1) - kRaised<T>;
     uint32_t p[4];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -530,7 +530,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
         reinterpret_cast<float2 *>(part_o + at)[e] = make_float2(acc[2 * e], acc[2 * e + 1]);
     }
     if (lane == 0) {
-      const float log2_sum = log2_of_sum(true, m, l);
+      const float log2_sum = log2_of_sum(true, m - kRaised<T>, l);
       if (!direct) part_lse[row] = log2_sum;
       else if (a.lse) a.lse[row] = log2_sum * kLn2;
     }

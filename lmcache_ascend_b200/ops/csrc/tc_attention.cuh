@@ -12,8 +12,8 @@
 //                        when half of P is there
 // While one tile's scores are in the registers the tensor cores work on the
 // other's.  m only moves when the maximum grows by more than 2^8, so O in TMEM
-// is seldom rescaled (by the thread that owns the row; P stays below 2^8 and
-// sums are fp32, so nothing is lost).
+// is seldom rescaled (by the thread that owns the row; P stays below 2^8, or 2^15
+// in float16, see kRaised, and sums are fp32).
 //
 // Roles: warps 0-7 and 8-15 one row tile each, warp 16 issues the mma, warp 17
 // the TMA loads through a ring of two stages, each with the K of a tile and the V
@@ -42,6 +42,12 @@ constexpr int kTileThreads = 256;  // of one row tile: two per row
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 constexpr float kLazy = 8.f;  // log2 of how far P may pass 1 before O is rescaled
+// log2 of a factor on the weights (the sum has it too, so only the row's log takes
+// it off).  Below 2^-14 float16 rounds in steps of 2^-24, and 2^-25 of the maximum
+// was lost: 100k keys of that size are 0.3% of a row.  2^7 times larger, weights of
+// up to 2^8 stay below its 65504 and what is lost is 2^-32.
+template <typename T>
+constexpr float kRaised = __is_same(T, __half) ? 7.f : 0.f;
 
 // Dense keys: positions and documents of a key tile.
 struct TileStats {
@@ -685,7 +691,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // half of this tile; one that does has only scores of -inf there, and NaN
         // weights (-inf less -inf) lead it to the definition.
         const bool sees = kDense ? whole || (vis0 | vis1) != 0 : some_page;
-        const float off = (m == -INFINITY && !sees ? 0.f : m) - lift;
+        const float off = (m == -INFINITY && !sees ? 0.f : m) - lift - kRaised<T>;
         const f32x2 c2 = pack2(c, c), off2 = pack2(-off, -off);
         f32x2 l0 = pack2(0.f, 0.f), l1 = l0;
         // the weights of 32 keys, some of them by the polynomial; the product may
@@ -802,10 +808,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       if (ref.valid && half == 0) {
         if (a.slices == 0) {
-          if (a.lse) a.lse[row] = log2_of_sum(ok, m, l) * kLn2;
+          if (a.lse) a.lse[row] = log2_of_sum(ok, m - kRaised<T>, l) * kLn2;
         } else {
           a.part_lse[static_cast<long long>(slice) * a.tokens * a.heads + row] =
-              log2_of_sum(ok, m, l);
+              log2_of_sum(ok, m - kRaised<T>, l);
         }
       }
       if (!ok && row_in_tile == 0 && half == 0)

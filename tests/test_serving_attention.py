@@ -616,6 +616,61 @@ def test_prefix_kernel_scores_of_minus_infinity(form):
     assert int(hit.sum()) == H // KH
 
 
+def _tail(n, D, bits):
+    """One key whose weight is 2^bits times each of n others and whose value is
+    zero: the result is the others' share."""
+    q = torch.zeros(1, 1, D, dtype=FP)
+    q[0, 0, 0] = 8.0
+    k = torch.zeros(n + 1, 1, D, dtype=FP)
+    k[n // 3, 0, 0] = bits * math.log(2) / 8
+    v = torch.rand(n + 1, 1, D, generator=torch.Generator().manual_seed(n)).to(FP) + 1
+    v[n // 3] = 0
+    return q, k, v
+
+
+# Weights pass through float16 times 2^7: below its normal range they are off by at
+# most 2^-25 of that, 2^-32 of the largest weight, each.
+def _tail_tolerance(o, v, n):
+    return (2.0 ** -10 + 2.0 ** -14) * o.abs() + n * 2.0 ** -32 * float(v.max()) + 2.0 ** -25
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [20.3, 24.7, 25.4, 27.0])
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_position_kernel_float16_keeps_the_tail_of_a_row(form, bits):
+    Tq, Tk, H, KH, D = form
+    q, k, v = _tail(Tk - 1, D, bits)
+    o, lse = R.position_attention_ref(q, k, v, torch.tensor([Tk]), None, 1.0,
+                                      compute=torch.float64)
+    got, gl = api.position_attention(
+        q.cuda().expand(Tq, H, D), k.cuda().expand(Tk, KH, D), v.cuda().expand(Tk, KH, D),
+        torch.full((Tq,), Tk, device="cuda"), scale=1.0, return_lse=True)
+    err = (got.cpu().double() - o).abs()
+    assert bool((err <= _tail_tolerance(o, v, Tk)).all())
+    assert bool(((gl.cpu().double() - lse).abs() <= 2.0 ** -18 * (1 + lse.abs())).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [20.3, 24.7, 25.4, 27.0])
+@pytest.mark.parametrize("form", PAGED_FORMS, ids=str)
+def test_prefix_kernel_float16_keeps_the_tail_of_a_row(form, bits):
+    B, Tq, H, KH, D, P = form
+    q, k, v = _tail(P, D, bits)
+    _, kc, vc, prefix, tables, lens = _prefix_case(B, Tq, H, KH, D, 16, P, [1] * B, FP, junk=0.0)
+    at = torch.arange(P)
+    for c, x in ((kc, k), (vc, v)):
+        c[prefix.long()[at // 16], at % 16] = x[:P].expand(P, KH, D)
+        c[tables[:, 0].long(), 0] = x[P].expand(B, KH, D)
+    o, lse = R.position_attention_ref(q, k, v, torch.tensor([P]), None, 1.0,
+                                      compute=torch.float64)
+    got, gl = api.shared_prefix_attention(
+        q.cuda().expand(B, H, D), kc.cuda(), vc.cuda(), prefix.cuda(), P, tables.cuda(),
+        lens.cuda(), scale=1.0, return_lse=True)
+    err = (got.cpu().double() - o).abs()
+    assert bool((err <= _tail_tolerance(o, v, P + 1)).all())
+    assert bool(((gl.cpu().double() - lse).abs() <= 2.0 ** -18 * (1 + lse.abs())).all())
+
+
 @pytest.mark.gpu
 def test_position_kernel_unaligned_rows_and_far_positions():
     q, k, v, qp, kp, kw = _position_case(100, 300, 4, 2, 64, BF, "subset")
