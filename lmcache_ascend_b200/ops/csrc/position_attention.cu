@@ -135,6 +135,12 @@ cudaError_t launch(const PositionArgs &a, void *workspace, cudaStream_t stream) 
 
 }  // namespace
 
+PositionPasses position_passes(const PositionArgs &a) {
+  const Plan p = plan_of(a);
+  if (p.split) return {0, p.slices};
+  return {std::max(1, p.slices), 0};
+}
+
 long long position_attention_workspace(const PositionArgs &a, int dim) {
   const Plan p = plan_of(a);
   if (p.split)

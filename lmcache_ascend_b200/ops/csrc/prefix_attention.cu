@@ -117,6 +117,11 @@ cudaError_t launch(const PagedArgs &a, void *workspace, cudaStream_t stream) {
 
 }  // namespace
 
+PrefixPasses prefix_passes(const PagedArgs &a) {
+  const PrefixPlan p = plan_of(a);
+  return {p.tc_slices, p.pre_slices, p.own_slices};
+}
+
 long long shared_prefix_attention_workspace(const PagedArgs &a, int dim) {
   const PrefixPlan p = plan_of(a);
   const int slices = p.tc_slices + p.pre_slices + p.own_slices;

@@ -114,6 +114,12 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> position_attention(
     double softcap, const c10::optional<at::Tensor> &alibi_slopes,
     const c10::optional<at::Tensor> &q_documents, const c10::optional<at::Tensor> &k_documents,
     const c10::optional<at::Tensor> &q_prefix_lens, bool causal, bool return_lse);
+std::tuple<int, int, int> shared_prefix_attention_passes(int64_t batch, int64_t q_len,
+                                                         int64_t heads, int64_t kv_heads,
+                                                         int64_t block_size, int64_t prefix_len,
+                                                         int64_t width);
+std::tuple<int, int> position_attention_passes(int64_t q_tokens, int64_t k_tokens, int64_t heads,
+                                               int64_t kv_heads);
 // dma.cu
 void dma_copy_batch(const at::Tensor &dsts, const at::Tensor &srcs, const at::Tensor &sizes);
 double dma_copy_batch_timed(const at::Tensor &dsts, const at::Tensor &srcs,
@@ -244,6 +250,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("shared_prefix_attention", &shared_prefix_attention);
   m.def("position_attention", &position_attention);
   m.def("log2_of_sum", &log2_of_sum);
+  m.def("shared_prefix_attention_passes", &shared_prefix_attention_passes);
+  m.def("position_attention_passes", &position_attention_passes);
 
   m.def("layerwise_prefill_dma_copy", &dma_copy_batch);
   m.def("layerwise_prefill_dma_copy_diagnose", &dma_copy_batch_timed);

@@ -479,4 +479,27 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> position_attention(
   return {out, lse};
 }
 
+// The passes of a call of these sizes (for tests: which kernel a shape reaches).
+std::tuple<int, int, int> shared_prefix_attention_passes(int64_t batch, int64_t q_len,
+                                                         int64_t heads, int64_t kv_heads,
+                                                         int64_t block_size, int64_t prefix_len,
+                                                         int64_t width) {
+  PagedArgs a = {};
+  a.batch = static_cast<int>(batch), a.q_len = static_cast<int>(q_len);
+  a.heads = static_cast<int>(heads), a.kv_heads = static_cast<int>(kv_heads);
+  a.block_size = static_cast<int>(block_size), a.width = static_cast<int>(width);
+  a.prefix_len = prefix_len;
+  const PrefixPasses p = prefix_passes(a);
+  return {p.tensor_core, p.split_prefix, p.own};
+}
+
+std::tuple<int, int> position_attention_passes(int64_t q_tokens, int64_t k_tokens, int64_t heads,
+                                               int64_t kv_heads) {
+  PositionArgs a = {};
+  a.q_tokens = static_cast<int>(q_tokens), a.k_tokens = static_cast<int>(k_tokens);
+  a.heads = static_cast<int>(heads), a.kv_heads = static_cast<int>(kv_heads);
+  const PositionPasses p = position_passes(a);
+  return {p.tensor_core, p.split};
+}
+
 }  // namespace lmc

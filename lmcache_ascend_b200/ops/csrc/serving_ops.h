@@ -88,6 +88,16 @@ struct PositionArgs {
   float scale, softcap;
 };
 
+// Which kernels an attention call takes, in slices of the keys (0: not taken).
+struct PrefixPasses {
+  int tensor_core, split_prefix, own;  // the prefix, or else in the own pass
+};
+struct PositionPasses {
+  int tensor_core, split;  // one of them; tensor_core 1: whole, more: joined
+};
+PrefixPasses prefix_passes(const PagedArgs &a);
+PositionPasses position_passes(const PositionArgs &a);
+
 cudaError_t launch_slot_mapping(const SlotArgs &a, bool long_lens, bool long_slots,
                                 cudaStream_t stream);
 cudaError_t launch_rope_cache(const RopeArgs &a, RowType rows, RowType table, bool vec,

@@ -517,7 +517,7 @@ FORMS = [(20, 200, 8, 2, 64), (20, 300, 4, 2, 128), (1, 6000, 4, 2, 64), (400, 7
          (500, 850, 16, 2, 64), (300, 3000, 16, 2, 64)]
 # ... and paged: B, Tq, H, KH, D, P
 PAGED_FORMS = [(3, 1, 8, 2, 64, 20), (2, 1, 8, 2, 64, 500), (1, 1, 8, 2, 128, 6000),
-               (30, 1, 32, 2, 128, 1000), (40, 1, 32, 2, 64, 1700)]
+               (30, 1, 32, 2, 128, 1000), (40, 1, 32, 2, 64, 1700), (40, 1, 32, 2, 128, 1200)]
 
 
 def _check_with_nan(got, lse, want):
@@ -669,6 +669,149 @@ def test_prefix_kernel_float16_keeps_the_tail_of_a_row(form, bits):
     err = (got.cpu().double() - o).abs()
     assert bool((err <= _tail_tolerance(o, v, P + 1)).all())
     assert bool(((gl.cpu().double() - lse).abs() <= 2.0 ** -18 * (1 + lse.abs())).all())
+
+
+# The tensor-core pass over the prefix: parts of large pages and many small ones, every
+# layout, several KV heads, and a last page that ends inside a tile.
+PREFIX_TC = [
+    (40, 1, 32, 2, 64, 8, 1700, [1 + i for i in range(40)], BF, 0.0, False, "merged"),
+    (40, 1, 32, 2, 128, 16, 1705, [1 + i % 5 for i in range(40)], FP, 0.0, False, "heads"),
+    (40, 1, 32, 2, 128, 32, 1705, [3 * i for i in range(40)], FP, 30.0, True, "heads"),
+    (40, 1, 32, 2, 128, 128, 1790, [1 + i for i in range(40)], BF, 0.0, True, "merged"),
+    (44, 1, 32, 2, 64, 256, 1801, [1 + i for i in range(44)], FP, 0.0, False, "heads"),
+    (33, 4, 16, 2, 64, 384, 1000, [4 + i for i in range(33)], BF, 20.0, False, "merged"),
+    (30, 2, 64, 4, 128, 64, 700, [2 + i for i in range(30)], BF, 0.0, False, "plain"),
+]
+# Dense calls on the tensor cores whose blocks write their rows themselves.
+POSITION_WHOLE = [
+    (700, 700, 16, 2, 64, FP, 50.0, True, "documents"),
+    (700, 700, 16, 2, 128, FP, 0.0, False, "documents"),
+    (650, 650, 16, 2, 128, BF, 0.0, False, "padded"),
+    (800, 800, 8, 2, 64, BF, 0.0, True, "prefix"),
+    (600, 850, 16, 2, 128, FP, 15.0, True, "shuffled"),
+    (640, 895, 10, 2, 128, BF, 20.0, False, "interleaved"),
+    (500, 600, 16, 1, 64, FP, 0.0, True, "all"),
+    (700, 700, 8, 1, 64, BF, 0.0, False, "causal"),
+    (1000, 1300, 40, 4, 128, BF, 0.0, False, "subset"),
+    (1000, 1000, 40, 4, 64, FP, 0.0, True, "documents"),
+]
+
+
+@pytest.mark.skipif(not ops.native_available(), reason="native module not built")
+def test_shapes_reach_the_kernels_they_are_there_for():
+    dense = lambda c: ops.native().position_attention_passes(*c[:4])
+    tc, split = zip(*(dense(c) for c in FORMS))
+    assert tc[:3] == (0, 0, 0) and split[0] == 1 and 2 <= split[1] <= 8 < split[2]
+    assert split[3:] == (0, 0, 0) and tc[3:5] == (1, 1) and tc[5] > 1
+    for c in POSITION_WHOLE:
+        assert dense(c) == (1, 0), c
+    for T in (700, 850):
+        assert dense((T, T, 16, 1)) == (1, 0)
+
+    def paged(B, Tq, H, KH, D, P, bs=16, own=20):
+        return ops.native().shared_prefix_attention_passes(B, Tq, H, KH, bs, P, -(-own // bs) + 1)
+
+    got = [paged(*c) for c in PAGED_FORMS]
+    assert got[0] == (0, 0, 1) and got[1][:2] == (0, 0) and 2 <= got[1][2] <= 8
+    assert got[2][:2] == (0, 0) and got[2][2] > 8
+    assert got[3][:2] == (0, 0) and got[4][0] > 1 and got[4][1] == 0
+    assert got[5][0] == 0 and got[5][1] > 1
+    for B, Tq, H, KH, D, bs, P, own in (c[:8] for c in PREFIX_TC):
+        assert paged(B, Tq, H, KH, D, P, bs, max(own))[0] > 1
+    for bs in (8, 16, 64, 256):
+        assert paged(40, 1, 32, 2, 128, 1700, bs, 50)[0] > 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", PREFIX_TC, ids=lambda c: "-".join(str(x) for x in c[:7]))
+def test_prefix_kernel_on_the_tensor_cores(case):
+    test_prefix_kernel(case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", POSITION_WHOLE,
+                         ids=lambda c: "-".join(str(x) for x in c[:5]) + c[8])
+def test_position_kernel_whole_rows_on_the_tensor_cores(case):
+    test_position_kernel(case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("D,T", [(64, 700), (128, 850)])
+def test_position_kernel_masked_keys_hold_anything_whole_rows(value, D, T):
+    test_position_kernel_masked_keys_hold_anything(value, T, 16, D, T)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bs,bad", [(8, (3, 17, 40)), (16, (0, 30)), (64, (2, 5, 6)), (256, (1, 3)),
+                                    (16, tuple(range(8))), (64, tuple(range(27)))])
+def test_prefix_kernel_bad_pages_on_the_tensor_cores(bs, bad):
+    """Single pages, the first whole tile, every page of the prefix."""
+    B, H, KH, D, P = 40, 32, 2, 128, 1700
+    own = [20 + i % 30 for i in range(B)]
+    q, kc, vc, prefix, tables, lens = _prefix_case(B, 1, H, KH, D, bs, P, own, BF)
+    for i, page in enumerate(bad):
+        prefix[page] = (-1, kc.shape[0], 1 << 30, -(1 << 31))[i % 4]
+
+    def ref(q_, k_, v_):
+        return R.shared_prefix_attention_ref(q_, k_, v_, prefix, P, tables, lens, 0.1,
+                                             compute=torch.float64)
+
+    want = _bounds(ref, q, kc, vc, BF, 0.1, 0.0, None, P + 50)
+    st = ops.DeviceStatus("cuda")
+    got, lse = api.shared_prefix_attention(q.cuda(), kc.cuda(), vc.cuda(), prefix.cuda(), P,
+                                           tables.cuda(), lens.cuda(), scale=0.1, return_lse=True,
+                                           status=st.tensor)
+    _check(got, lse, *want)
+    assert st.read()["name"] == "bad_slot"
+
+
+@pytest.mark.gpu
+def test_prefix_kernel_large_scores_on_the_tensor_cores():
+    B, H, KH, D, P = 40, 32, 2, 64, 1700
+    q, kc, vc, prefix, tables, lens = _prefix_case(B, 1, H, KH, D, 16, P, [40] * B, BF)
+    kc[prefix.long()[2]] *= 100
+    kc[prefix.long()[70]] *= 200
+
+    def ref(q_, k_, v_):
+        return R.shared_prefix_attention_ref(q_, k_, v_, prefix, P, tables, lens, 1.0,
+                                             compute=torch.float64)
+
+    want = _bounds(ref, q, kc, vc, BF, 1.0, 0.0, None, P + 40)
+    got, lse = api.shared_prefix_attention(q.cuda(), kc.cuda(), vc.cuda(), prefix.cuda(), P,
+                                           tables.cuda(), lens.cuda(), scale=1.0, return_lse=True)
+    _check(got, lse, *want)
+
+
+@pytest.mark.gpu
+def test_prefix_kernel_on_the_tensor_cores_captured_twice():
+    B, P = 40, 1700
+    q, kc, vc, prefix, tables, lens = _prefix_case(B, 1, 32, 2, 64, 16, P, [30] * B, BF, junk=0.0)
+    d = [x.cuda() for x in (q, kc, vc, prefix, tables, lens)]
+
+    def call():
+        return api.shared_prefix_attention(d[0], d[1], d[2], d[3], P, d[4], d[5], return_lse=True)
+
+    call()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = call()
+        graphs.append((g, out))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for shift in (0, 1):
+        d[5].copy_(torch.arange(B) % 30 + shift)
+        want = call()
+        torch.cuda.synchronize()
+        for _ in range(5):  # both at once
+            for (g, _), s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
 
 
 @pytest.mark.gpu
