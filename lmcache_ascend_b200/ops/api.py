@@ -623,6 +623,7 @@ def rotary_embedding(positions: torch.Tensor, query: torch.Tensor,
     others pass through.  ``cos_sin_cache``: one row of cosines and sines per
     position (``reference.make_cos_sin_cache`` / ``make_scaled_cos_sin_cache``).
     A position outside the table gives a zero row and is reported in ``status``.
+    On the device forward only: operands that ask for gradients are refused.
     """
     if query.is_cuda:
         return native().rotary_embedding_and_cache(

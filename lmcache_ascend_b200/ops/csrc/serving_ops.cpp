@@ -2,6 +2,7 @@
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <algorithm>
@@ -40,12 +41,22 @@ at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const c10::Device 
   return at::detail::empty_cuda(sizes, dtype, dev, c10::nullopt);
 }
 
-// The operators are forward only: an input that asks for gradients would lose them.
-void check_no_grad(const char *op, std::initializer_list<const at::Tensor *> inputs) {
-  if (!at::GradMode::is_enabled()) return;
-  for (const at::Tensor *t : inputs)
-    TORCH_CHECK(!t->requires_grad(), op, ": forward only, and an input requires grad");
+// The operators are forward only: an input that asks for gradients, or carries a
+// tangent of forward differentiation, would lose them without a word.  (An operand
+// that is not given is null.)
+void check_no_grad(const char *op, std::initializer_list<const at::Tensor *> operands) {
+  const bool backward = at::GradMode::is_enabled();
+  const bool forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  for (const at::Tensor *t : operands) {
+    if (t == nullptr) continue;
+    TORCH_CHECK(!backward || !t->requires_grad(), op,
+                ": forward only, and an operand requires grad");
+    TORCH_CHECK(!forward || !t->_fw_grad(/*level=*/0).defined(), op,
+                ": forward only, and an operand carries a tangent");
+  }
 }
+
+const at::Tensor *given(const c10::optional<at::Tensor> &t) { return t.has_value() ? &*t : nullptr; }
 
 // `n` elements of `base` from `first` on, as a tensor of their own (a view without
 // the dispatcher).
@@ -218,9 +229,8 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> rotary_embedding_and_cache(
   TORCH_CHECK(query.is_cuda(), op, ": query must be on the device");
   const c10::Device dev = query.device();
   const auto dt = query.scalar_type();
-  check_no_grad(op, {&query});
-  if (key.has_value()) check_no_grad(op, {&*key});
-  if (value.has_value()) check_no_grad(op, {&*value});
+  check_no_grad(op, {&query, given(key), given(value), given(key_cache), given(value_cache),
+                     &cos_sin_cache, given(given_query_out), given(given_key_out)});
   const c10::cuda::CUDAGuard guard(dev);
   const at::Tensor query_out =
       given_query_out.has_value() ? *given_query_out : fresh(query.sizes(), dt, dev);
@@ -334,7 +344,7 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> shared_prefix_attention(
   TORCH_CHECK(query.is_cuda(), op, ": query must be on the device");
   const c10::Device dev = query.device();
   const auto dt = query.scalar_type();
-  check_no_grad(op, {&query, &key_cache, &value_cache});
+  check_no_grad(op, {&query, &key_cache, &value_cache, given(alibi_slopes)});
   TORCH_CHECK(query.dim() == 3 || query.dim() == 4, op,
               ": query must be [B, H, D] or [B, q_len, H, D]");
   const at::Tensor q4 = query.dim() == 3 ? query.unsqueeze(1) : query;
@@ -410,7 +420,7 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> position_attention(
   TORCH_CHECK(query.is_cuda(), op, ": query must be on the device");
   const c10::Device dev = query.device();
   const auto dt = query.scalar_type();
-  check_no_grad(op, {&query, &key, &value});
+  check_no_grad(op, {&query, &key, &value, given(alibi_slopes)});
   TORCH_CHECK(query.dim() == 3, op, ": query must be [Tq, H, D]");
   const int64_t Tq = query.size(0), H = query.size(1), D = query.size(2);
   TORCH_CHECK(key.dim() == 3 && key.sizes() == value.sizes() && key.size(2) == D &&

@@ -197,6 +197,32 @@ def test_kernel_no_rows_and_refusals():
 
 
 @pytest.mark.gpu
+def test_no_gradient_is_lost_without_a_word():
+    D, table = 64, R.make_cos_sin_cache(64, 64).cuda()
+    q = torch.randn(4, 2 * D, device="cuda")
+    k, v = torch.randn(4, D, device="cuda"), torch.randn(4, D, device="cuda")
+    kc, vc = torch.zeros(2, 4, 1, D, device="cuda"), torch.zeros(2, 4, 1, D, device="cuda")
+    p = torch.arange(4, device="cuda")
+    kw = dict(query=q, key=k, value=v, key_cache=kc, value_cache=vc, cos_sin_cache=table,
+              query_out=torch.zeros_like(q), key_out=torch.zeros_like(k))
+
+    def call(**more):
+        return api.rotary_embedding_and_cache(positions=p, slot_mapping=p, head_size=D,
+                                              **{**kw, **more})
+
+    call()
+    for name, t in kw.items():
+        with pytest.raises(RuntimeError, match="forward only"):
+            call(**{name: t.clone().requires_grad_()})
+        with torch.no_grad():
+            call(**{name: t.clone().requires_grad_()})
+        with torch.autograd.forward_ad.dual_level():
+            dual = torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+            with pytest.raises(RuntimeError, match="tangent"):
+                call(**{name: dual})
+
+
+@pytest.mark.gpu
 def test_kernel_on_a_side_stream_captured():
     T, H, D = 40, 8, 128
     q = torch.randn(T, H * D, device="cuda").bfloat16()

@@ -273,6 +273,34 @@ def test_inputs_that_ask_for_gradients_are_refused():
 
 
 @pytest.mark.gpu
+def test_no_gradient_is_lost_without_a_word():
+    """Slopes and caches that ask for gradients, and forward tangents of any input."""
+    q, k, v, qp, kp, _ = _position_case(8, 30, 4, 2, 64, BF, "subset")
+    d = [x.cuda() for x in (q, k, v, qp, kp)]
+    slopes = _slopes(4).cuda()
+    p = [x.cuda() for x in _prefix_case(2, 1, 4, 2, 64, 16, 32, [3, 4], BF)]
+
+    def dense(q_=d[0], k_=d[1], v_=d[2], s_=slopes):
+        return api.position_attention(q_, k_, v_, d[3], d[4], alibi_slopes=s_)
+
+    def paged(q_=p[0], k_=p[1], v_=p[2], s_=slopes):
+        return api.shared_prefix_attention(q_, k_, v_, p[3], 32, p[4], p[5], alibi_slopes=s_)
+
+    for call, tensors in ((dense, d[:3]), (paged, p[:3])):
+        want = call()
+        for name, t in zip(("q_", "k_", "v_", "s_"), tensors + [slopes]):
+            leaf = t.clone().requires_grad_()
+            with pytest.raises(RuntimeError, match="forward only"):
+                call(**{name: leaf})
+            with torch.no_grad():
+                assert torch.equal(call(**{name: leaf}), want)
+            with torch.autograd.forward_ad.dual_level():
+                dual = torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+                with torch.no_grad(), pytest.raises(RuntimeError, match="tangent"):
+                    call(**{name: dual})
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,value", [(BF, torch.finfo(BF).min), (FP, torch.finfo(FP).min),
                                          (BF, math.inf)])
 def test_prefix_kernel_unused_slots_hold_anything(dtype, value):
