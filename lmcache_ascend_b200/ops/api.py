@@ -667,10 +667,14 @@ def rotary_embedding_and_cache(positions: torch.Tensor, query: torch.Tensor, key
 
 
 def _check_scores(scale, softcap):
-    if not 0 < scale < float("inf"):
-        raise ValueError("scale must be positive and finite")
-    if not 0 <= softcap < float("inf"):
-        raise ValueError("softcap must be >= 0 (0: none)")
+    """The range in which fp32 holds both, and the cap's argument."""
+    least = torch.finfo(torch.float32).tiny
+    if not least <= scale <= 1e38:
+        raise ValueError("scale must be positive and finite (in fp32)")
+    if softcap != 0 and not least <= softcap <= 1e38:
+        raise ValueError("softcap must be >= 0 and finite (0: none)")
+    if softcap and scale / softcap > 1e37:
+        raise ValueError("softcap too small for the scale")
 
 
 def _attention_result(query, out, lse, return_lse):

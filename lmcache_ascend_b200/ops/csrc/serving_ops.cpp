@@ -127,8 +127,13 @@ at::Tensor with_vector_rows(const at::Tensor &x) {
 void check_scores(const char *op, double scale, double softcap,
                   const c10::optional<at::Tensor> &slopes, int64_t heads,
                   const c10::Device &dev) {
-  TORCH_CHECK(std::isfinite(scale) && scale > 0, op, ": scale must be positive and finite");
-  TORCH_CHECK(std::isfinite(softcap) && softcap >= 0, op, ": softcap must be >= 0 (0: none)");
+  // the kernels hold both in fp32, times log2 e and (the cap's argument) 2 scale / cap
+  const float f = static_cast<float>(scale), cap = static_cast<float>(softcap);
+  constexpr float kLeast = std::numeric_limits<float>::min(), kMost = 1e38f;
+  TORCH_CHECK(f >= kLeast && f <= kMost, op, ": scale must be positive and finite (in fp32)");
+  TORCH_CHECK(softcap == 0 || (cap >= kLeast && cap <= kMost), op,
+              ": softcap must be >= 0 and finite (0: none)");
+  TORCH_CHECK(softcap == 0 || scale / softcap <= 1e37, op, ": softcap too small for the scale");
   if (slopes.has_value()) {
     check_dense(*slopes, op, "alibi_slopes", dev, at::kFloat);
     TORCH_CHECK(slopes->dim() == 1 && slopes->numel() == heads, op,

@@ -140,6 +140,32 @@ def test_part_whose_wait_ran_out_is_not_taken_for_an_empty_one():
         assert math.isnan(log(False, m, l))
 
 
+# Scales and caps that fp32 does not hold: infinite, or zero and so no cap at all.
+OUT_OF_FP32 = [dict(scale=1e300), dict(scale=1e39), dict(scale=1e-50), dict(softcap=1e39),
+               dict(softcap=1e-50), dict(softcap=math.inf), dict(softcap=math.nan),
+               dict(scale=1e20, softcap=1e-20)]
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_scores_outside_of_fp32_are_refused(device):
+    q, k, v, qp, kp, _ = (x.to(device) if isinstance(x, torch.Tensor) else x
+                          for x in _position_case(8, 30, 4, 2, 64, BF, "subset"))
+    p = [x.to(device) for x in _prefix_case(2, 1, 4, 2, 64, 16, 32, [3, 4], BF)]
+    for kw in OUT_OF_FP32:
+        with pytest.raises((ValueError, RuntimeError)):
+            api.position_attention(q, k, v, qp, kp, **kw)
+        with pytest.raises((ValueError, RuntimeError)):
+            api.shared_prefix_attention(p[0], p[1], p[2], p[3], 32, p[4], p[5], **kw)
+    # at the borders: a cap far below the scores is a mean of the values seen
+    for kw in (dict(softcap=1e-20), dict(scale=1e-37), dict(scale=1.0, softcap=1e38)):
+        want = R.position_attention_ref(q.cpu(), k.cpu(), v.cpu(), qp.cpu(), kp.cpu(),
+                                        kw.get("scale", 0.125), kw.get("softcap", 0.0),
+                                        compute=torch.float64)[0]
+        got = api.position_attention(q, k, v, qp, kp, **kw).cpu().double()
+        # weights and result rounded to 8 bits, |v| below 5
+        assert bool(((got - want).abs() <= 2 * 2.0 ** -8 * 5).all())
+
+
 # ------------------------------------------------------------ shared prefix
 def _prefix_case(B, Tq, H, KH, D, bs, P, own, dtype, seed=0, layout="plain", junk=math.nan):
     """A paged batch whose unused slots hold ``junk``."""
