@@ -188,6 +188,13 @@ class LMCacheEngineConfig:
             return [v]
         return v
 
+    def extra_flag(self, name: str) -> bool:
+        """A truth value of ``extra_config``, also where it comes as text."""
+        v = (self.extra_config or {}).get(name, False)
+        if isinstance(v, str):
+            return v.strip().lower() in ("1", "true", "yes", "on")
+        return bool(v)
+
     def validate(self) -> None:
         if self.chunk_size <= 0:
             raise ValueError("chunk_size must be > 0")

@@ -212,7 +212,7 @@ def get_or_create_blender(instance_id: str, cache_engine, gpu_connector, config,
         from .blender import LMCBlender
 
         model = infer_model_from_vllm(VLLMModelTracker.get_model(instance_id),
-                                      bool(config.extra_config.get("blend_native_attention")))
+                                      config.extra_flag("blend_native_attention"))
         b = _blenders[instance_id] = LMCBlender(cache_engine, gpu_connector, model, config,
                                                 kv_caches=_kv_pairs(kv_caches))
     return b

@@ -17,6 +17,7 @@ from lmcache_ascend_b200.config import LMCacheEngineConfig, LMCacheEngineMetadat
 from lmcache_ascend_b200.models.llama import LlamaConfig, LlamaForBlend
 from lmcache_ascend_b200.v1.blend.blender import LMCBlender
 from lmcache_ascend_b200.v1.blend.vllm_model import (LMCVLLMModel, VLLMModelTracker,
+                                                     drop_blender, get_or_create_blender,
                                                      infer_model_from_vllm)
 from lmcache_ascend_b200.v1.cache_engine import LMCacheEngine
 from lmcache_ascend_b200.v1.gpu_connector import VLLMBufferLayerwiseGPUConnector
@@ -165,3 +166,38 @@ def test_blend_through_served_model_equals_prefill(qwen3):
 def test_unsupported_model_type_is_refused():
     with pytest.raises(NotImplementedError):
         infer_model_from_vllm(nn.Linear(2, 2))
+
+
+@pytest.mark.parametrize("value,native", [(True, True), ("true", True), ("1", True), (None, False),
+                                          ("false", False), ("0", False), (False, False)])
+def test_native_attention_of_a_served_model_is_asked_for_in_the_config(value, native):
+    _, eng, blender, kv = _setup(False)
+    ec = LMCacheEngineConfig.from_dict({"lmcache.blend_native_attention": value})
+    drop_blender("blend-test")
+    try:
+        got = get_or_create_blender("blend-test", eng, blender.gpu_connector, ec, kv)
+        assert isinstance(got.layerwise_model, LMCVLLMModel)
+        assert got.layerwise_model.native_attention is native
+    finally:
+        drop_blender("blend-test")
+
+
+@pytest.mark.parametrize("qwen3", [False, True])
+def test_blend_with_native_attention_equals_prefill(qwen3, monkeypatch):
+    """The served model's blend with ``position_attention`` (on the CPU its plain form)."""
+    from lmcache_ascend_b200.ops import api
+
+    calls = []
+    plain = api.position_attention
+    monkeypatch.setattr(api, "position_attention",
+                        lambda *a, **kw: (calls.append(a[0].shape), plain(*a, **kw))[1])
+    setup = _setup
+
+    def native(q):
+        ref, eng, blender, kv = setup(q)
+        blender.layerwise_model.native_attention = True
+        return ref, eng, blender, kv
+
+    monkeypatch.setitem(globals(), "_setup", native)
+    test_blend_through_served_model_equals_prefill(qwen3)
+    assert len(calls) == 4  # one a layer
