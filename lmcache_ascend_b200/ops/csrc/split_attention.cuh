@@ -106,14 +106,18 @@ __device__ __noinline__ void strict_paged_row(const PagedArgs &a, long long r) {
   const float slope = a.slopes ? a.slopes[h] : 0.f;
   WarpRow<T, D> row;
   row.start(static_cast<const T *>(a.q) + b * a.q_batch + i * a.q_token + h * a.q_head);
-  for (long long j = 0; j < a.prefix_len + own; ++j) {
+  const long long keys = a.prefix_len + own;
+#pragma unroll 1
+  for (long long j0 = 0; j0 < keys && !row.lost(); j0 += 32) {
+    const long long j = min(j0 + (threadIdx.x & 31), keys - 1);
     const bool shared = j < a.prefix_len;
     const unsigned at = static_cast<unsigned>(shared ? j : j - a.prefix_len);
     const unsigned col = at / static_cast<unsigned>(a.block_size);
     const int off = static_cast<int>(at - col * a.block_size);
-    const int page = shared ? a.prefix_blocks[col] : a.tables[b * a.table_stride + col];
-    if (page < 0 || page >= a.num_blocks) continue;
-    row.add(static_cast<const T *>(a.k) + page * a.k_block + off * a.k_slot + kv * a.k_head,
+    int page = shared ? a.prefix_blocks[col] : a.tables[b * a.table_stride + col];
+    const bool sees = j0 + (threadIdx.x & 31) < keys && page >= 0 && page < a.num_blocks;
+    if (!sees) page = 0;
+    row.add(sees, static_cast<const T *>(a.k) + page * a.k_block + off * a.k_slot + kv * a.k_head,
             static_cast<const T *>(a.v) + page * a.v_block + off * a.v_slot + kv * a.v_head,
             a.scale, a.softcap, slope * fabsf(static_cast<float>(pos - j)));
   }

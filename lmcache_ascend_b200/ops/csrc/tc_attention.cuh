@@ -209,10 +209,12 @@ __device__ __forceinline__ void strict_position_row(const PositionArgs &a, int t
   row.start(static_cast<const T *>(a.q) + token * a.q_token + h * a.q_head);
   const float slope = a.slopes ? a.slopes[h] : 0.f;
 #pragma unroll 1
-  for (int j = 0; j < a.k_tokens; ++j) {
+  for (int j0 = 0; j0 < a.k_tokens && !row.lost(); j0 += 32) {
+    const int j = min(j0 + static_cast<int>(threadIdx.x & 31), a.k_tokens - 1);
     const int kp = a.k_pos ? clamp_pos(position_at(a.k_pos, a.long_k_pos, j)) : j;
-    if (kp >= m.limit || (a.k_doc && a.k_doc[j] != m.doc)) continue;
-    row.add(static_cast<const T *>(a.k) + j * a.k_token + kv * a.k_head,
+    const bool sees = j0 + static_cast<int>(threadIdx.x & 31) < a.k_tokens && kp < m.limit &&
+                      (!a.k_doc || a.k_doc[j] == m.doc);
+    row.add(sees, static_cast<const T *>(a.k) + j * a.k_token + kv * a.k_head,
             static_cast<const T *>(a.v) + j * a.v_token + kv * a.v_head, a.scale, a.softcap,
             slope * fabsf(static_cast<float>(static_cast<long long>(m.pos) - kp)));
   }
@@ -821,8 +823,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (tile_any(x, wrong)) {  // what was written above is written again below
           *mine = wrong ? 1.f : 0.f;
           tile_any(x, false);
-          uint32_t again =
-              half == 0 ? __ballot_sync(0xffffffffu, *mine + *other > 0.f) : 0u;
+          // (the two warps of 32 rows take every other one)
+          uint32_t again = __ballot_sync(0xffffffffu, *mine + *other > 0.f) &
+                           (half == 0 ? 0x55555555u : 0xaaaaaaaau);
           while (again) {
             const int src = __ffs(again) - 1;
             again &= again - 1;

@@ -670,6 +670,51 @@ def test_prefix_kernel_scores_of_minus_infinity(form):
     assert int(hit.sum()) == H // KH
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("paged", [False, True])
+@pytest.mark.parametrize("form", range(len(FORMS)))
+def test_rows_computed_again_have_the_same_scores(form, paged):
+    """An infinity in the first value: every row is computed a second time, with cap
+    and distance bias, and only that column shows it."""
+    if paged:
+        B, Tq, H, KH, D, P = PAGED_FORMS[form]
+        q, kc, vc, prefix, tables, lens = _prefix_case(B, Tq, H, KH, D, 16, P, [20] * B, BF)
+        reach, slopes = P + 20, _slopes(H)
+        k, v = kc, vc
+        hit = (int(prefix[0]), 0, 0, 5)
+
+        def ref(q_, k_, v_):
+            return R.shared_prefix_attention_ref(q_, k_, v_, prefix, P, tables, lens, D ** -0.5,
+                                                 20.0, slopes, torch.float64)
+
+        def run(v_):
+            return api.shared_prefix_attention(
+                q.cuda(), kc.cuda(), v_.cuda(), prefix.cuda(), P, tables.cuda(), lens.cuda(),
+                softcap=20.0, alibi_slopes=slopes.cuda(), return_lse=True)
+    else:
+        Tq, Tk, H, KH, D = FORMS[form]
+        q, k, v, qp, kp, kw = _position_case(Tq, Tk, H, KH, D, BF, "subset")
+        reach, slopes = Tk, _slopes(H)
+        hit = (0, 0, 5)
+
+        def ref(q_, k_, v_):
+            return R.position_attention_ref(q_, k_, v_, qp, kp, D ** -0.5, 20.0, slopes,
+                                            compute=torch.float64)
+
+        def run(v_):
+            return _run_position(q, k, v_, qp, kp, {}, BF, 20.0, slopes)
+
+    o, e, tol, tl = _bounds(ref, q, k, v, BF, D ** -0.5, 20.0, slopes, reach)
+    bad = v.clone()
+    bad[hit] = math.inf
+    got, lse = run(bad)
+    rows = got.cpu().reshape(-1, H, D)[:, :H // KH]
+    assert bool((rows[..., 5] == math.inf).all())
+    mended = got.cpu().clone()
+    mended.reshape(-1, H, D)[:, :H // KH, 5] = o.reshape(-1, H, D)[:, :H // KH, 5].to(BF)
+    _check(mended, lse, o, e, tol, tl)
+
+
 def _tail(n, D, bits):
     """One key whose weight is 2^bits times each of n others and whose value is
     zero: the result is the others' share."""
