@@ -913,6 +913,97 @@ def test_prefix_kernel_on_the_tensor_cores_captured_twice():
             assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
 
 
+# Chunks of a prompt on a shared prefix: split and tensor-core prefix, more rows than
+# a tile, requests with fewer own tokens than queries.
+CHUNKS = [(2, 300, 8, 2, 64, 16, 100, [300, 700], BF, 0.0, False, "plain"),
+          (3, 129, 16, 2, 128, 32, 700, [40, 129, 500], FP, 30.0, True, "heads"),
+          (1, 1024, 4, 1, 64, 64, 300, [1024], FP, 0.0, True, "merged")]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", CHUNKS, ids=lambda c: "-".join(str(x) for x in c[:7]))
+def test_prefix_kernel_many_query_tokens(case):
+    test_prefix_kernel(case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_position_kernel_keys_and_values_of_other_strides(form):
+    """K as a slice of wider rows, V and Q head by head."""
+    Tq, Tk, H, KH, D = form
+    q, k, v, qp, kp, kw = _position_case(Tq, Tk, H, KH, D, BF, "subset")
+    want = _run_position(q, k, v, qp, kp, {}, BF, 0.0, None)
+    wide = torch.zeros(Tk, (KH + 3) * D, dtype=BF, device="cuda")
+    wide[:, 2 * D:(KH + 2) * D] = k.flatten(1).cuda()
+    dk = wide[:, 2 * D:(KH + 2) * D].unflatten(1, (KH, D))
+    dv = v.transpose(0, 1).contiguous().cuda().transpose(0, 1)
+    dq = q.transpose(0, 1).contiguous().cuda().transpose(0, 1)
+    got, lse = api.position_attention(dq, dk, dv, qp.cuda(), kp.cuda(), return_lse=True)
+    assert torch.equal(got, want[0]) and torch.equal(lse, want[1])
+
+
+@pytest.mark.gpu
+def test_prefix_kernel_caches_of_other_strides():
+    for form in PAGED_FORMS:
+        B, Tq, H, KH, D, P = form
+        q, kc, vc, *rest = _prefix_case(B, Tq, H, KH, D, 16, P, [20] * B, BF)
+        rest = [x.cuda() for x in rest]
+        a = (rest[0], P, rest[1], rest[2])
+        want = api.shared_prefix_attention(q.cuda(), *_on_device(kc, vc, "plain"), *a)
+        dk = _on_device(kc, vc, "merged")[0]
+        dv = _on_device(kc, vc, "heads")[1]
+        assert torch.equal(api.shared_prefix_attention(q.cuda(), dk, dv, *a), want)
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once():
+    cases = [_position_case(Tq, Tk, H, KH, D, BF, "subset") for Tq, Tk, H, KH, D in FORMS[2:]]
+    dev = [[x.cuda() for x in c[:5]] for c in cases]
+    want = [api.position_attention(*d) for d in dev]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(3):
+        for i, d in enumerate(dev):
+            for s in streams:
+                with torch.cuda.stream(s):
+                    got.append((i, api.position_attention(*d)))
+    torch.cuda.synchronize()
+    for i, g in got:
+        assert torch.equal(g, want[i])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", [PAGED_FORMS[i] for i in (1, 2, 4, 5)], ids=str)
+def test_offsets_of_a_long_cache_pass_32_bits(form):
+    """The same pages at the end of caches of 2^31 elements and more."""
+    from lmcache_ascend_b200.ops.reference import make_cos_sin_cache
+
+    B, Tq, H, KH, D, P = form
+    q, kc, vc, prefix, tables, lens = (x.cuda() for x in _prefix_case(
+        B, Tq, H, KH, D, 16, P, [20] * B, BF, junk=0.0))
+    want = api.shared_prefix_attention(q, kc, vc, prefix, P, tables, lens)
+    first = (1 << 31) // (16 * KH * D) + 7
+    long_k, long_v = (torch.empty(first + c.shape[0], 16, KH, D, dtype=BF, device="cuda")
+                      for c in (kc, vc))
+    long_k[first:], long_v[first:] = kc, vc
+    got = api.shared_prefix_attention(q, long_k, long_v, prefix + first, P, tables + first, lens)
+    assert torch.equal(got, want)
+    # rows written there, by the slots of a slot map
+    st = ops.DeviceStatus("cuda")
+    new = torch.full((B,), 3, dtype=torch.int32, device="cuda")
+    small, far = (api.build_slot_mapping(lens, new, t, 16, 3 * B, num_blocks=nb, status=st.tensor)
+                  for t, nb in ((tables, kc.shape[0]), (tables + first, long_k.shape[0])))
+    st.check()
+    assert torch.equal(far.slot_mapping, small.slot_mapping + first * 16)
+    x = torch.randn(3 * B, KH * D, device="cuda").to(BF)
+    table = make_cos_sin_cache(64, D).cuda()
+    args = (small.positions, x, x, x)
+    api.rotary_embedding_and_cache(*args, kc, vc, small.slot_mapping, D, table)
+    api.rotary_embedding_and_cache(*args, long_k, long_v, far.slot_mapping, D, table)
+    assert torch.equal(long_k[first:], kc) and torch.equal(long_v[first:], vc)
+
+
 @pytest.mark.gpu
 def test_position_kernel_unaligned_rows_and_far_positions():
     q, k, v, qp, kp, kw = _position_case(100, 300, 4, 2, 64, BF, "subset")
