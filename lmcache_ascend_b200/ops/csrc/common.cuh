@@ -1,10 +1,10 @@
 // Device-side building blocks shared by every kernel of the extension.
 //
-// All kernels here are bandwidth or latency bound (no GEMM-shaped work), so
-// the Blackwell features that matter are: 16-byte vector loads/stores, the
-// TMA bulk engine (`cp.async.bulk`, NON-multicast only) completing on an
-// mbarrier, and system-scope release/acquire operations for flags that cross
-// NVLink.  Every spin-wait in this file takes an iteration budget and reports
+// The kernels that move, code and place KV are bandwidth or latency bound (the
+// GEMM-shaped work is in tc_attention.cuh), so the Blackwell features that matter
+// to them are: 16-byte vector loads/stores, the TMA bulk engine
+// (`cp.async.bulk`, NON-multicast only) completing on an mbarrier, and
+// system-scope release/acquire operations for flags that cross NVLink.  Every spin-wait in this file takes an iteration budget and reports
 // failure instead of hanging the GPU.
 #pragma once
 

@@ -51,9 +51,17 @@ struct Plan {
 };
 
 // Blocks of 16 rows times steps of 64 keys up to which the split kernel is taken.
-// Measured (B200, 32/8 heads of 128, split / tensor cores, us): 38 rows on 257 keys
-// (400 steps) 11.2 / 14.8, 128 on 512 (2048) 16.1 / 16.5, 1 on 16384 (2048)
-// 20.2 / 24.7, 8 on 16384 (4096) 30.7 / 26.0, 256 on 512 (4096) 29.0 / 16.5.
+// Measured (B200, 32/8 heads, split / tensor cores, us, replayed without host calls):
+//                         steps  D 128        D 64         D 128, cap and bias
+//   38 rows on 257 keys     400   9.3 / 15.0   7.1 / 12.0  11.1 / 20.3
+//   128 on 512             2048  14.9 / 18.4  10.6 / 15.8  17.7 / 28.2
+//   1 on 16384             2048  20.7 / 23.0  14.9 / 20.1  19.9 / 33.6
+//   256 on 512             4096  27.9 / 17.6  20.2 / 14.8  32.8 / 27.7
+//   8 at the end of 16384  4096  27.2 / 24.5  18.4 / 20.8  32.4 / 36.4
+//   8 spread over 16384    4096  28.2 / 48.8  19.5 / 46.7  33.4 / 61.6
+// Rows far apart cost the tensor-core kernel its masks (nearly every tile is in part
+// visible to a warp's rows), which the sizes do not tell; the border is where rows
+// next to one another break even.
 constexpr long long kSplitSteps = 2048;
 
 // The keys are split when the blocks would not fill the GPU: towards one block

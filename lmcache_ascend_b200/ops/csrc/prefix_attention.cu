@@ -17,13 +17,18 @@ struct PrefixPlan {
 };
 
 // Blocks of 16 rows times steps of 64 keys up to which the split pass reads the
-// prefix.  Measured (B200, 32/8 heads of 128, split / tensor cores, us): 250 steps
-// 11.8 / 15.9, 1024 steps 17.5 / 20.3 and 22.2 / 24.8, 2000 steps 20.1 / 25.0
-// (one request), 4096 steps 36.1 / 26.4.
+// prefix.  Measured (B200, 32/8 heads, split / tensor cores, us, replayed without
+// host calls):          steps  D 128        D 64         D 128, cap and bias
+//   8 requests on 4096   1024  17.9 / 19.6  16.0 / 17.9  20.0 / 24.1
+//   1 on 16000           2000  21.7 / 24.6  20.6 / 22.1  24.8 / 32.1
+//   64 on 1024           2048  23.9 / 22.2  17.8 / 18.2  28.8 / 27.3
+//   32 on 4096           4096  29.2 / 21.5  21.1 / 18.9  36.4 / 25.6
 constexpr long long kSplitSteps = 2000;
-// ... and up to which every request reads it with its own keys, in one pass (16 on
-// 500 tokens, 1024 steps: 11.0 us against 11.2 in two passes, with one launch for
-// three; 4 on 500: 7.8 against 9.6).
+// ... and up to which every request reads it with its own keys, in one pass and one
+// launch instead of two and three (one / two passes: 4 on 500 tokens, 256 steps,
+// 7.9 / 10.2, D 64 6.4 / 9.0, capped 9.9 / 12.2; 16 on 500, 1024 steps, 11.0 / 11.6,
+// 8.0 / 10.1, 12.8 / 13.8; 16 on 1024, 2048 steps, 15.0 / 13.3, 10.6 / 11.6,
+// 18.7 / 14.9).
 constexpr long long kFewSteps = 1200;
 
 PrefixPlan plan_of(const PagedArgs &a) {

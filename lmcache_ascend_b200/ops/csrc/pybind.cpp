@@ -86,13 +86,12 @@ void rotary_embedding_k_fused_layers(const at::Tensor &old_positions,
                                      const std::vector<at::Tensor> &keys, int64_t head_size,
                                      const at::Tensor &cos_sin_cache, bool is_neox,
                                      const c10::optional<at::Tensor> &slot_mapping);
-// slot_kernels.cu
+// serving_ops.cpp (slot maps, rotary with cache writes, attention)
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>
 build_slot_mapping(const at::Tensor &context_lens, const at::Tensor &new_lens,
                    at::Tensor &block_tables, int64_t block_size, int64_t num_tokens,
                    const c10::optional<at::Tensor> &free_blocks, int64_t num_blocks,
                    bool long_slots, const c10::optional<at::Tensor> &status);
-// rope_cache_kernels.cu
 std::tuple<at::Tensor, c10::optional<at::Tensor>> rotary_embedding_and_cache(
     const at::Tensor &positions, const at::Tensor &query, const c10::optional<at::Tensor> &key,
     const c10::optional<at::Tensor> &value, const c10::optional<at::Tensor> &key_cache,
@@ -101,7 +100,6 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> rotary_embedding_and_cache(
     const c10::optional<at::Tensor> &given_query_out,
     const c10::optional<at::Tensor> &given_key_out, bool new_key_out,
     const c10::optional<at::Tensor> &status);
-// attention_kernels.cu
 std::tuple<at::Tensor, c10::optional<at::Tensor>> shared_prefix_attention(
     const at::Tensor &query, const at::Tensor &key_cache, const at::Tensor &value_cache,
     const at::Tensor &prefix_blocks, int64_t prefix_len, const at::Tensor &block_tables,

@@ -17,8 +17,8 @@
 // a unit costs no division and a row's cosines and sines are loaded once for
 // several heads; blocks get equal work for one row or many.  The loads in flight
 // come from many threads with one unit each (five blocks of 256 per SM), not from
-// several units a thread: 16385 rows of 64/8 heads of 128 (680 MB) take 113 us
-// (6.0 TB/s) so, 150 us with two units a thread in four blocks, 126 us in six
+// several units a thread: 16385 rows of 64/8 heads of 128 (680 MB) take 117 us
+// (5.8 TB/s) so, 150 us with two units a thread in four blocks, 126 us in six
 // blocks (spills).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -632,9 +632,12 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
 // Towards one wave of three blocks per SM, with 128 keys or more each; eight parts
 // rather than up to sixteen, because a cluster joins them in the same launch.
 // Measured (us, 8 KV heads of 128): 16 requests on 500 tokens 15.8 in one part, 11.0
-// in parts of 128; one row on 1024 keys 19.4 / 6.9; one row on 257 keys 7.8 / 7.0,
-// but 38 rows of 32 heads on them (80 blocks) 9.4 / 10.0.  A deeper ring (six stages)
-// changed none of these: a step's own chain of instructions takes its 0.8 us.
+// in parts of 128; one row on 1024 keys 19.4 / 6.9.  Between 256 and 384 keys two
+// parts pay while their blocks have an SM each (one / two parts, 260 keys: 72 blocks
+// 9.1 / 8.6, 80 blocks 9.2 / 10.2, 200 blocks 11.6 / 12.5; D 64 7.0 / 7.0, 7.0 / 7.7,
+// 8.3 / 9.1; capped 11.1 / 10.1, 11.0 / 11.5, 13.6 / 14.6; 383 keys alike).  A deeper
+// ring (six stages) changed none of these: a step's own chain of instructions takes
+// its 0.8 us.
 inline int split_slices(long long blocks, long long keys) {
   if (keys < 256 || (keys < 384 && blocks > 74)) return 1;
   long long want = std::min(444 / std::max(1ll, blocks), keys / 128);

@@ -10,7 +10,7 @@ CPU test tier).  They implement the same formats as the CUDA kernels:
 * RoPE delta re-rotation (``pos_kernels.cu``);
 * slot maps from request lengths, rotary positions with cache writes, and the
   attention operators (``slot_kernels.cu``, ``rope_cache_kernels.cu``,
-  ``attention_kernels.cu``).
+  ``prefix_attention.cu``, ``position_attention.cu``).
 """
 
 from __future__ import annotations
