@@ -65,7 +65,8 @@ struct JoinedRow {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(128)
-    join_position_kernel(PositionArgs a, const float *part_o, const float *part_lse, int slices) {
+    join_position_kernel(const __grid_constant__ PositionArgs a, const float *part_o,
+                         const float *part_lse, int slices) {
   const long long rows = static_cast<long long>(a.q_tokens) * a.heads;
   const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
   wait_for_previous();
@@ -75,7 +76,8 @@ __global__ void __launch_bounds__(128)
   if (r.finite())
     r.store(static_cast<T *>(a.out), a.lse, row);
   else
-    strict_position_row<T, D>(a, static_cast<int>(row / a.heads), static_cast<int>(row % a.heads));
+    strict_position_row_again<T, D>(a, static_cast<int>(row / a.heads),
+                                    static_cast<int>(row % a.heads));
 }
 
 // Score constants of the tensor-core kernel.

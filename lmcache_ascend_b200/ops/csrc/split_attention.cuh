@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
              __reduce_max_sync(0xffffffffu, kp_all) < all_limit;
     else
       open = j0 + kSplitKeys <= all_last && bad_keys == 0;
-    bool sees0 = open, sees1 = open;  // one of this lane's keys
+    uint32_t sees = open ? 3 : 0;  // which of its rows see one of this lane's keys
     if (!open) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
           }
           if (out0) sc[t][e] = -INFINITY;
           if (out1) sc[t][2 + e] = -INFINITY;
-          sees0 = sees0 || !out0, sees1 = sees1 || !out1;
+          sees |= (out0 ? 0 : 1) | (out1 ? 0 : 2);  // (as two flags: 4% of a short call)
         }
       }
     }
@@ -471,8 +471,8 @@ __global__ void __launch_bounds__(kSplitWarps * 32, 3)
     }
     // no finite score yet: zero weights, or NaN ones for keys that are seen and have
     // scores of -inf (they lead the row to the definition)
-    const float off0 = (m0 == -INFINITY && !sees0 ? 0.f : m0) - kRaised<T>;
-    const float off1 = (m1 == -INFINITY && !sees1 ? 0.f : m1) - kRaised<T>;
+    const float off0 = (m0 == -INFINITY && !(sees & 1) ? 0.f : m0) - kRaised<T>;
+    const float off1 = (m1 == -INFINITY && !(sees & 2) ? 0.f : m1) - kRaised<T>;
     uint32_t p[4];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {

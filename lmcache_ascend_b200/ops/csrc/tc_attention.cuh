@@ -223,6 +223,13 @@ __device__ __forceinline__ void strict_position_row(const PositionArgs &a, int t
   row.finish(static_cast<T *>(a.out) + r * D, a.lse ? a.lse + r : nullptr);
 }
 
+// The same as a call of its own, for the join (inlined, its registers and code cost a
+// join of 27 parts 0.3 of 16.7 us).
+template <typename T, int D>
+__device__ __noinline__ void strict_position_row_again(const PositionArgs &a, int token, int h) {
+  strict_position_row<T, D>(a, token, h);
+}
+
 // The key tiles of a block, in order; every role walks them alike.
 template <bool kDense>
 struct TileScan {
