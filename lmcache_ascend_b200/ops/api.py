@@ -704,15 +704,14 @@ def shared_prefix_attention(query: torch.Tensor, key_cache: torch.Tensor,
 
     Returns [B, ..., H, D] and, with ``return_lse``, the fp32 log of each row's
     sum.  A row that sees no key is zero with -inf; one whose scores are all -inf
-    is NaN.  Keys in a block outside the
-    cache, or past the end of a table row, are left out and reported in
-    ``status``.  On the device: bfloat16 or float16, D of 64 or 128, 16-byte
+    is NaN.  Keys in a block outside the cache, or past the end of a table row, are
+    left out and reported in ``status``.  On the device: bfloat16 or float16, D of 64 or 128, 16-byte
     aligned cache rows, forward only (operands that ask for gradients are
     refused).  There the weights are rounded to the rows' type for the product
     with the values, as tensor cores take them: beside its own rounding an element
     is off by at most 2^-8 (float16: 2^-11) of the weighted mean of |v|, less where
-    many keys count.  Statistics, sums and joins are fp32.  A row that sees an infinity or NaN is
-    computed a second time, which is slow where many do.
+    many keys count.  Statistics, sums and joins are fp32.  A row that sees an
+    infinity or NaN is computed a second time, which is slow where many do.
     """
     if scale is None:
         scale = query.shape[-1] ** -0.5

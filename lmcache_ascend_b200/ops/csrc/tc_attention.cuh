@@ -24,7 +24,7 @@
 // (four warps) the tensor cores idled half the time.
 // 256 rows a block because a K/V tile then feeds 256 flop a byte from L2.
 //
-// Measured: 16384 x 16384 rows of 64/8 heads of 128, causal, 3.9 ms (1.12 PFLOP/s,
+// Measured: 16384 x 16384 rows of 64/8 heads of 128, causal, 3.9 ms (1.1 PFLOP/s,
 // 0.68 of the measured product).  At D = 128 two row tiles take all of tensor memory
 // (at 64 three quarters, and a third buffer for scores is not there yet), so a
 // tile's next scores wait for its last weights: a turn is about 3250 cycles
