@@ -219,6 +219,17 @@ def make_cos_sin_cache(max_pos: int, rot_dim: int, base: float = 10000.0,
     return torch.cat([f.cos(), f.sin()], dim=-1).to(dtype)
 
 
+_ROPE_KEYS = {
+    "default": {"factor", "original_max_position_embeddings"},  # of no effect
+    "linear": {"factor", "original_max_position_embeddings"},
+    "dynamic": {"factor", "original_max_position_embeddings"},
+    "llama3": {"factor", "original_max_position_embeddings", "low_freq_factor",
+               "high_freq_factor"},
+    "yarn": {"factor", "original_max_position_embeddings", "beta_fast", "beta_slow", "truncate",
+             "attention_factor", "mscale", "mscale_all_dim"},
+}
+
+
 def make_scaled_cos_sin_cache(max_pos: int, rot_dim: int, base: float = 10000.0,
                               scaling: Optional[Dict[str, Any]] = None,
                               dtype=torch.float32) -> torch.Tensor:
@@ -232,11 +243,21 @@ def make_scaled_cos_sin_cache(max_pos: int, rot_dim: int, base: float = 10000.0,
       original context kept, of fewer than ``low_freq_factor`` divided by
       ``factor``, a ramp between;
     * ``yarn``: a ramp over the dimensions between ``beta_fast`` and ``beta_slow``
-      turns, and a gain of ``attention_factor`` (default 0.1 ln(factor) + 1) on
-      the cosines and sines.
+      turns (rounded outwards unless ``truncate`` is false), and a gain on the
+      cosines and sines: ``attention_factor``, or with ``mscale`` and
+      ``mscale_all_dim`` the quotient of 0.1 m ln(factor) + 1 for each, or that for
+      m = 1.
+
+    A key that would change the table and is not known here is refused.
     """
     scaling = dict(scaling or {})
     kind = scaling.get("rope_type", scaling.get("type", "default"))
+    unknown = {k for k, v in scaling.items() if v is not None} - _ROPE_KEYS.get(kind, set()) \
+        - {"rope_type", "type", "rope_theta"}
+    if kind in _ROPE_KEYS and unknown:
+        raise ValueError(f"{kind} rope scaling does not know {sorted(unknown)}")
+    if float(scaling.get("rope_theta") or base) != float(base):
+        raise ValueError(f"rope_theta {scaling['rope_theta']} is not the base {base}")
     dims = torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim
     gain = 1.0
     if kind == "default":
@@ -262,14 +283,26 @@ def make_scaled_cos_sin_cache(max_pos: int, rot_dim: int, base: float = 10000.0,
         def dim_of(turns: float) -> float:
             return rot_dim * math.log(orig / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-        lo = max(math.floor(dim_of(float(scaling.get("beta_fast", 32.0)))), 0)
-        hi = min(math.ceil(dim_of(float(scaling.get("beta_slow", 1.0)))), rot_dim - 1)
+        lo = dim_of(float(scaling.get("beta_fast") or 32.0))
+        hi = dim_of(float(scaling.get("beta_slow") or 1.0))
+        if scaling.get("truncate") in (None, True):
+            lo, hi = math.floor(lo), math.ceil(hi)
+        lo, hi = max(lo, 0), min(hi, rot_dim - 1)
         ramp = ((torch.arange(rot_dim // 2, dtype=torch.float64) - lo)
                 / max(hi - lo, 0.001)).clamp(0, 1)
         inv = base ** -dims
         inv = inv / f * ramp + inv * (1 - ramp)
-        given = scaling.get("attention_factor")
-        gain = float(given) if given is not None else (0.1 * math.log(f) + 1.0 if f > 1 else 1.0)
+
+        def gain_of(m: float) -> float:
+            return 0.1 * m * math.log(f) + 1.0 if f > 1 else 1.0
+
+        m, m_all = scaling.get("mscale"), scaling.get("mscale_all_dim")
+        if scaling.get("attention_factor") is not None:
+            gain = float(scaling["attention_factor"])
+        elif m and m_all:
+            gain = gain_of(float(m)) / gain_of(float(m_all))
+        else:
+            gain = gain_of(1.0)
     else:
         raise ValueError(f"unknown rope scaling {kind!r}")
     a = torch.outer(torch.arange(max_pos, dtype=torch.float64), inv)

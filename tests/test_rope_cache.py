@@ -52,6 +52,42 @@ def test_unknown_scaling_is_refused():
         R.make_scaled_cos_sin_cache(16, 8, scaling={"rope_type": "other", "factor": 2.0})
 
 
+def test_yarn_gains_and_untruncated_ramp():
+    n, rot, base, f, orig = 64, 64, 10000.0, 40.0, 4096
+    yarn = {"rope_type": "yarn", "factor": f, "original_max_position_embeddings": orig}
+    gain = lambda m: 0.1 * m * math.log(f) + 1
+
+    def first(**more):  # cosine of angle 0: the gain
+        return float(R.make_scaled_cos_sin_cache(n, rot, base, {**yarn, **more},
+                                                 torch.float64)[0, 0])
+
+    assert abs(first() - gain(1)) < 1e-12
+    assert abs(first(mscale=1.0, mscale_all_dim=1.0) - 1) < 1e-12
+    assert abs(first(mscale=0.707, mscale_all_dim=1.5) - gain(0.707) / gain(1.5)) < 1e-12
+    assert abs(first(attention_factor=1.25, mscale=1.0, mscale_all_dim=1.0) - 1.25) < 1e-12
+    lo, hi = (rot * math.log(orig / (t * 2 * math.pi)) / (2 * math.log(base)) for t in (16, 2))
+    table = R.make_scaled_cos_sin_cache(n, rot, base, {**yarn, "beta_fast": 16, "beta_slow": 2,
+                                                       "truncate": False,
+                                                       "attention_factor": 1.0}, torch.float64)
+    for i in range(rot // 2):
+        w = base ** (-2 * i / rot)
+        mix = min(1.0, max(0.0, (i - lo) / (hi - lo)))
+        w = mix * w / f + (1 - mix) * w
+        assert abs(float(table[63, rot // 2 + i]) - math.sin(63 * w)) < 1e-9
+
+
+def test_scaling_keys_that_are_not_known_are_refused():
+    for bad in ({"rope_type": "linear", "factor": 2.0, "mscale": 1.0},
+                {"rope_type": "yarn", "factor": 2.0, "original_max_position_embeddings": 64,
+                 "partial_rotary_factor": 0.5},
+                {"rope_type": "llama3", "factor": 8.0, "rope_theta": 500000.0}):
+        with pytest.raises(ValueError):
+            R.make_scaled_cos_sin_cache(16, 8, 10000.0, bad)
+    same = {"rope_type": "default", "rope_theta": 10000.0, "mscale": None}
+    assert torch.equal(R.make_scaled_cos_sin_cache(16, 8, 10000.0, same),
+                       R.make_cos_sin_cache(16, 8))
+
+
 def test_oracle_is_a_rotation_and_undone_by_the_opposite():
     T, H, D, rot = 9, 3, 32, 16
     x = torch.randn(T, H * D, dtype=torch.float64)
