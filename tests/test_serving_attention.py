@@ -927,6 +927,29 @@ def test_prefix_kernel_many_query_tokens(case):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("width", [3, 20, 600, 4096])
+@pytest.mark.parametrize("form", PAGED_FORMS, ids=str)
+def test_prefix_kernel_tables_wider_than_the_requests(form, width):
+    """Most parts of a row are empty where a table has room for long requests."""
+    B, Tq, H, KH, D, P = form
+    q, kc, vc, prefix, tables, lens = _prefix_case(B, Tq, H, KH, D, 16, P, [20] * B, BF)
+    wide = torch.full((B, width), -1, dtype=torch.int32)
+    wide[:, :tables.shape[1]] = tables
+
+    def ref(q_, k_, v_):
+        return R.shared_prefix_attention_ref(q_, k_, v_, prefix, P, tables, lens, D ** -0.5,
+                                             compute=torch.float64)
+
+    want = _bounds(ref, q, kc, vc, BF, D ** -0.5, 0.0, None, P + 20)
+    st = ops.DeviceStatus("cuda")
+    got, lse = api.shared_prefix_attention(q.cuda(), kc.cuda(), vc.cuda(), prefix.cuda(), P,
+                                           wide.cuda(), lens.cuda(), return_lse=True,
+                                           status=st.tensor)
+    _check(got, lse, *want)
+    st.check()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("form", FORMS, ids=str)
 def test_position_kernel_keys_and_values_of_other_strides(form):
     """K as a slice of wider rows, V and Q head by head."""
