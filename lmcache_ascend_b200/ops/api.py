@@ -594,7 +594,7 @@ def build_slot_mapping(context_lens: torch.Tensor, new_lens: torch.Tensor,
     if dtype not in (torch.int32, torch.int64):
         raise ValueError(f"slots are int32 or int64, not {dtype}")
     if num_blocks is None:
-        num_blocks = ((1 << 31) - 1) // (block_size if dtype == torch.int32 else 1)
+        num_blocks = ((1 << 31) - 1) // (max(1, block_size) if dtype == torch.int32 else 1)
     if block_tables.is_cuda:
         return SlotMapping(*native().build_slot_mapping(
             context_lens, new_lens, block_tables, block_size, num_tokens, free_blocks,
@@ -725,6 +725,10 @@ def shared_prefix_attention(query: torch.Tensor, key_cache: torch.Tensor,
         raise ValueError("query must be [B, H, D] or [B, q_len, H, D] with whole head groups")
     if prefix_len < 0 or prefix_blocks.numel() * key_cache.shape[1] < prefix_len:
         raise ValueError("prefix_blocks do not hold the prefix")
+    if seq_lens.shape != (query.shape[0],) or block_tables.shape[0] < query.shape[0]:
+        raise ValueError("seq_lens must be [batch] and block_tables [>= batch, width]")
+    if alibi_slopes is not None and alibi_slopes.shape != (query.shape[-2],):
+        raise ValueError("alibi_slopes must be [heads]")
     out, lse = R.shared_prefix_attention_ref(query, key_cache, value_cache, prefix_blocks,
                                              prefix_len, block_tables, seq_lens, scale, softcap,
                                              alibi_slopes)
@@ -769,6 +773,15 @@ def position_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tens
         raise ValueError("query [Tq, H, D] and key [Tk, KV heads, D] with whole head groups")
     if (q_documents is None) != (k_documents is None):
         raise ValueError("q_documents and k_documents go together")
+    for name, x, n in (("q_positions", q_positions, query.shape[0]),
+                       ("k_positions", k_positions, key.shape[0]),
+                       ("q_documents", q_documents, query.shape[0]),
+                       ("k_documents", k_documents, key.shape[0]),
+                       ("q_prefix_lens", q_prefix_lens, query.shape[0])):
+        if x is not None and (x.shape != (n,) or x.dtype not in (torch.int32, torch.int64)):
+            raise ValueError(f"{name} must be integers, {n} of them")
+    if alibi_slopes is not None and alibi_slopes.shape != (query.shape[1],):
+        raise ValueError("alibi_slopes must be [heads]")
     out, lse = R.position_attention_ref(query, key, value, q_positions, k_positions, scale,
                                         softcap, alibi_slopes, q_documents, k_documents,
                                         q_prefix_lens, causal)

@@ -140,6 +140,26 @@ def test_part_whose_wait_ran_out_is_not_taken_for_an_empty_one():
         assert math.isnan(log(False, m, l))
 
 
+def test_cpu_forms_refuse_marks_that_do_not_fit():
+    """What would be broadcast, or compared as a fraction."""
+    q, k = torch.randn(2, 4, 8), torch.randn(5, 2, 8)
+    p = torch.tensor([0, 4])
+    for bad in (dict(q_positions=p.float()), dict(q_positions=p[:1]),
+                dict(k_positions=torch.tensor([3])), dict(k_positions=torch.arange(5) / 2),
+                dict(q_prefix_lens=torch.tensor([1])), dict(alibi_slopes=torch.ones(6)),
+                dict(q_documents=p[:1].int(), k_documents=torch.zeros(5, dtype=torch.int32))):
+        with pytest.raises(ValueError):
+            api.position_attention(**{**dict(query=q, key=k, value=k, q_positions=p), **bad})
+    kc, one = torch.randn(3, 4, 2, 8), torch.zeros(1, dtype=torch.int32)
+    kw = dict(query=q, key_cache=kc, value_cache=kc, prefix_blocks=one, prefix_len=4,
+              block_tables=torch.tensor([[1], [2]], dtype=torch.int32),
+              seq_lens=torch.tensor([1, 3], dtype=torch.int32))
+    for bad in (dict(seq_lens=torch.tensor([1, 3, 2])), dict(block_tables=kw["block_tables"][:1]),
+                dict(alibi_slopes=torch.ones(5))):
+        with pytest.raises(ValueError):
+            api.shared_prefix_attention(**{**kw, **bad})
+
+
 # Scales and caps that fp32 does not hold: infinite, or zero and so no cap at all.
 OUT_OF_FP32 = [dict(scale=1e300), dict(scale=1e39), dict(scale=1e-50), dict(softcap=1e39),
                dict(softcap=1e-50), dict(softcap=math.inf), dict(softcap=math.nan),

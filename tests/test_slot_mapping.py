@@ -65,6 +65,13 @@ def test_cpu_refusals():
             api.build_slot_mapping(**kw)
 
 
+def test_block_size_of_zero_is_refused_for_both_slot_types():
+    z, t = torch.zeros(2, dtype=torch.int32), torch.zeros(2, 2, dtype=torch.int32)
+    for dtype in (torch.int32, torch.int64):
+        with pytest.raises(ValueError):
+            api.build_slot_mapping(z, z, t, 0, 2, dtype=dtype)
+
+
 def _compare(got, want, tables, tables_ref):
     for a, b in zip(got, want):
         assert a.dtype == b.dtype and torch.equal(a.cpu(), b)
