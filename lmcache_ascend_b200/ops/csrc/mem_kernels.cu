@@ -467,6 +467,9 @@ void kv_transfer(const PagedLayout &paged, const c10::optional<at::Tensor> &chun
     TORCH_CHECK(chunk_ptrs->is_cuda() && chunk_ptrs->scalar_type() == at::kLong,
                 "chunk_ptrs must be a device int64 tensor");
     TORCH_CHECK(chunk_tokens > 0, "chunk_tokens must be > 0");
+    const int64_t tokens = chunk_idx.has_value() ? chunk_idx_limit : slots.numel();
+    TORCH_CHECK(tokens <= chunk_ptrs->numel() * chunk_tokens, "chunk_ptrs: ", tokens,
+                " tokens need more than ", chunk_ptrs->numel(), " chunks of ", chunk_tokens);
     j.chunk.chunk_ptrs = chunk_ptrs->data_ptr<int64_t>();
     j.chunk.chunk_tokens = static_cast<int32_t>(chunk_tokens);
   } else {

@@ -148,11 +148,14 @@ class VLLMPagedMemGPUConnector(GPUConnectorInterface):
         return slot_mapping
 
     def _contiguous_batch(self, objs, starts, ends) -> bool:
+        """Whether token t of the range lies in object t // chunk_size, so that one
+        launch moves them all: full chunks, the last one full or shorter.  (A segment
+        of CacheBlend is one object however long it is.)"""
         cs = self.config.chunk_size
         for i, (s, e) in enumerate(zip(starts, ends)):
             if i > 0 and s != ends[i - 1]:
                 return False
-            if (e - s) != cs and i != len(starts) - 1:
+            if e - s > cs or (e - s != cs and i != len(starts) - 1):
                 return False
             if objs[i].get_num_tokens() != e - s:
                 return False

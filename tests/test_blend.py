@@ -102,3 +102,61 @@ def test_blend_partial_recompute_selects_topk():
     # layers 0-1 before selection see all tokens; after the check layer 25 % remain
     assert picked[0] == T and picked[1] == int(T * 0.25) and picked[-1] == int(T * 0.25)
     eng.close()
+
+
+def test_segments_longer_than_a_chunk_do_not_move_as_chunks():
+    """A pointer table of chunks holds token t at entry t // chunk_size: one object of
+    more tokens than a chunk has no second entry."""
+    conn = _setup(1.0, [0])[2]
+
+    class Obj:
+        def __init__(self, n):
+            self.n = n
+
+        def get_num_tokens(self):
+            return self.n
+
+    def tiles(*lens):
+        ends = [sum(lens[:i + 1]) for i in range(len(lens))]
+        return conn._contiguous_batch([Obj(n) for n in lens],
+                                      [e - n for e, n in zip(ends, lens)], ends)
+
+    assert tiles(256) and tiles(100) and tiles(256, 256) and tiles(256, 1)
+    assert not tiles(300) and not tiles(256, 300) and not tiles(100, 256) and not tiles(512, 10)
+
+
+@pytest.mark.gpu
+def test_long_segments_stored_from_the_gpu():
+    model, eng, conn, blender, kv = _setup(1.0, [0], "cuda")
+    for n, seed in ((300, 1), (256, 2), (257, 3), (511, 4)):
+        doc = torch.randint(0, 900, (n,), generator=torch.Generator().manual_seed(seed))
+        slots = torch.randperm(NB * BS, generator=torch.Generator().manual_seed(seed + 10))
+        slots = slots[:n].cuda()
+        model.prefill(doc, kv, slots)
+        want = [[_rows(kv, slots, l, w).clone() for w in range(2)] for l in range(4)]
+        for _ in eng.store_layer(doc, slot_mapping=slots):
+            pass
+        for layer in kv:
+            for t in layer:
+                t.zero_()
+        got = blender.blend(doc, slot_mapping=slots)
+        assert int(got.sum()) == n
+        torch.cuda.synchronize()
+        for l in range(4):  # every row is computed again: the same up to fp32's roundings
+            for w in range(2):
+                assert torch.allclose(_rows(kv, slots, l, w), want[l][w], atol=1e-3, rtol=1e-3)
+
+
+@pytest.mark.gpu
+def test_pointer_table_too_short_for_the_tokens_is_refused():
+    from lmcache_ascend_b200 import ops
+
+    conn = _setup(1.0, [0], "cuda")[2]
+    chunk = torch.zeros(2, 4, 256, 64, device="cuda")
+    table = torch.tensor([chunk.data_ptr()], dtype=torch.int64, device="cuda")
+    slots = torch.arange(300, device="cuda")
+    with pytest.raises(RuntimeError, match="need more than 1 chunks of 256"):
+        conn._native_xfer(None, slots, True, chunk_ptrs=table, chunk_tokens=256)
+    conn._native_xfer(None, slots[:256], True, chunk_ptrs=table, chunk_tokens=256)
+    torch.cuda.synchronize()
+    assert ops.native_available()
