@@ -141,17 +141,37 @@ def batched_fused_sparse_single_layer_kv_transfer(stagings, layout, layer, slot_
 
 
 # ----------------------------------------------------------------- K4 / N5
+def _chunk_tokens(chunks: Sequence[torch.Tensor], chunk_size: int) -> int:
+    """Tokens of chunk objects that make up a range: all full but the last."""
+    lens = [c.shape[2] for c in chunks]
+    if any(n != chunk_size for n in lens[:-1]) or not 0 < lens[-1] <= chunk_size:
+        raise ValueError(f"chunks of {lens} tokens are not full chunks of {chunk_size} "
+                         "(the last one full or shorter)")
+    return sum(lens)
+
+
+def _check_range(slots: torch.Tensor, tokens: int, chunk_size: int) -> None:
+    """A launch over a chunk table takes the chunk of its last token for as long as
+    the range says: the slots cover whole objects."""
+    n = slots.numel()
+    if n != tokens and (n > tokens or n % chunk_size):
+        raise ValueError(f"{n} slots do not cover whole chunks of {tokens} tokens")
+
+
 def dense_mla_dsa_batched_direct_kv_transfer(chunks: Sequence[torch.Tensor], layout,
                                              slot_mapping: torch.Tensor, chunk_size: int,
                                              direction: bool) -> None:
     """All layers of N chunk objects (host-pinned or device) in ONE launch
     through a device pointer table; token t lives in chunk t // chunk_size
     (reference mem_kernels.cpp:1036-1307, the 'direct' staging-free path)."""
+    _check_range(slot_mapping, _chunk_tokens(chunks, chunk_size), chunk_size)
     if layout.device.type != "cuda":
         s = 0
         for c in chunks:
             n = c.shape[2]
-            (layout.gather_ref if direction else layout.scatter_ref)(c, slot_mapping[s:s + n])
+            if s + n <= slot_mapping.numel():
+                (layout.gather_ref if direction else layout.scatter_ref)(
+                    c, slot_mapping[s:s + n])
             s += n
         return
     on_dev = chunks[0].is_cuda
@@ -172,6 +192,7 @@ class DirectTransferState:
         self.layout = layout
         self.chunk_size = int(chunk_size)
         self.chunks = list(chunks)
+        self.tokens = _chunk_tokens(self.chunks, self.chunk_size)
         self.on_device = chunks[0].is_cuda
         self.ptrs = torch.tensor([c.data_ptr() for c in chunks], dtype=torch.int64,
                                  device=layout.device)
@@ -187,6 +208,7 @@ def dense_mla_dsa_batched_direct_kv_transfer_prepared(state: DirectTransferState
         dense_mla_dsa_batched_direct_kv_transfer(state.chunks, state.layout, slot_mapping,
                                                  state.chunk_size, direction)
         return
+    _check_range(slot_mapping, state.tokens, state.chunk_size)
     _xfer(state.layout, None, slot_mapping, direction, chunk_ptrs=state.ptrs,
           chunk_tokens=state.chunk_size, chunk_on_device=state.on_device,
           mode=MODE_AUTO if state.on_device else MODE_SIMT)
@@ -220,9 +242,10 @@ def mla_dsa_sparse_multi_chunk_kv_transfer(chunks: Sequence[torch.Tensor], layou
                                            selected_token_idx: torch.Tensor,
                                            chunk_size: int) -> None:
     """paged[slot_mapping_packed[i]] = token selected_token_idx[i] of the chunk
-    sequence (token t in chunk t // chunk_size), all layers, straight from
-    pinned host or device chunks (reference mem_kernels.h:82-154 sparse
-    multi-chunk kernels)."""
+    sequence (token t in chunk t // chunk_size, the last one full or shorter), all
+    layers, straight from pinned host or device chunks (reference
+    mem_kernels.h:82-154 sparse multi-chunk kernels)."""
+    tokens = _chunk_tokens(chunks, chunk_size)
     if layout.device.type != "cuda":
         full = torch.cat(list(chunks), dim=2)
         rows = full.index_select(2, selected_token_idx.long().cpu())
@@ -233,7 +256,7 @@ def mla_dsa_sparse_multi_chunk_kv_transfer(chunks: Sequence[torch.Tensor], layou
     idx = selected_token_idx.to(layout.device, slot_mapping_packed.dtype)
     _xfer(layout, None, slot_mapping_packed.to(layout.device), False, chunk_ptrs=ptrs,
           chunk_tokens=chunk_size, chunk_on_device=on_dev, chunk_idx=idx,
-          chunk_idx_limit=len(chunks) * chunk_size,
+          chunk_idx_limit=tokens,
           mode=MODE_AUTO if on_dev else MODE_SIMT)
 
 

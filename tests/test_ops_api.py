@@ -123,6 +123,55 @@ def test_direct_fast_prepared_and_sparse_multi_chunk(dev):
         api.multi_layer_kv_transfer_unilateral()
 
 
+@pytest.mark.parametrize("dev", _devs())
+def test_direct_and_sparse_transfers_with_a_short_last_chunk(dev):
+    kv = make_separate_kv(2, 64, 16, 2, 64, torch.bfloat16, dev, seed=9)
+    lay = PagedKVLayout(kv)
+    cs, lens = 128, (128, 128, 45)
+    T = sum(lens)
+    slots = block_slots(T, 16, 64, seed=10, device=dev)
+    pin = dev == "cuda"
+    mk = lambda: [(lambda c: c.pin_memory() if pin else c)(
+        torch.zeros(lay.chunk_shape(n), dtype=torch.bfloat16)) for n in lens]
+    ref = torch.zeros(lay.chunk_shape(T), dtype=torch.bfloat16, device=dev)
+    lay.gather_ref(ref, slots)
+    chunks = mk()
+    api.dense_mla_dsa_batched_direct_kv_transfer(chunks, lay, slots, cs, True)
+    if pin:
+        torch.cuda.synchronize()
+    assert torch.equal(torch.cat([c.to(dev) for c in chunks], dim=2), ref)
+    # tokens of the last chunk among others
+    kv2 = [(torch.zeros_like(x), torch.zeros_like(y)) for x, y in kv]
+    lay2 = PagedKVLayout(kv2)
+    sel = torch.randperm(T, generator=torch.Generator().manual_seed(11))[:120]
+    dst = random_slots(120, 64 * 16, seed=12, device=dev)
+    api.mla_dsa_sparse_multi_chunk_kv_transfer(chunks, lay2, dst, sel.to(dev), cs)
+    if pin:
+        torch.cuda.synchronize()
+    for layer in range(2):
+        for plane in range(2):
+            got = kv2[layer][plane].reshape(-1, 128)[dst.long()]
+            assert torch.equal(got.cpu(), ref[plane, layer][sel].cpu())
+    # whole chunks of a longer list are a range; part of one, or more than all, is not
+    front = mk()
+    api.dense_mla_dsa_batched_direct_kv_transfer(front, lay, slots[:256], cs, True)
+    if pin:
+        torch.cuda.synchronize()
+    assert torch.equal(torch.cat([c.to(dev) for c in front[:2]], dim=2), ref[:, :, :256])
+    more = block_slots(T + 1, 16, 64, seed=10, device=dev)
+    state = api.DirectTransferState(chunks, lay, cs)
+    for bad in (slots[:200], slots[:300], more):
+        with pytest.raises(ValueError):
+            api.dense_mla_dsa_batched_direct_kv_transfer(chunks, lay, bad, cs, True)
+        with pytest.raises(ValueError):
+            api.dense_mla_dsa_batched_direct_kv_transfer_prepared(state, bad, True)
+    for bad in (chunks[::-1], [chunks[2], chunks[2]]):
+        with pytest.raises(ValueError):
+            api.dense_mla_dsa_batched_direct_kv_transfer(bad, lay, slots, cs, True)
+        with pytest.raises(ValueError):
+            api.mla_dsa_sparse_multi_chunk_kv_transfer(bad, lay2, dst, sel.to(dev), cs)
+
+
 @GPU
 def test_sparse_graph_capture_replay():
     kv = make_separate_kv(1, 64, 16, 4, 64, torch.bfloat16, "cuda", seed=9)
