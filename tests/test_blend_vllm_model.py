@@ -201,3 +201,54 @@ def test_blend_with_native_attention_equals_prefill(qwen3, monkeypatch):
     monkeypatch.setitem(globals(), "_setup", native)
     test_blend_through_served_model_equals_prefill(qwen3)
     assert len(calls) == 4  # one a layer
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ratio", [1.0, 0.3])
+def test_blend_with_native_attention_on_the_gpu(ratio):
+    """The served model's blend with the kernel and with PyTorch's attention leaves the
+    same pages, up to float16's roundings."""
+    cfg = LlamaConfig.tiny(vocab_size=1000, hidden_size=128, num_layers=3, num_heads=4,
+                           num_kv_heads=2, head_dim=64, intermediate_size=256, max_position=4096)
+    ref = LlamaForBlend(cfg, "cuda", torch.float16)
+    served = _served(ref, cfg, False)
+    g = torch.Generator().manual_seed(0)
+    docs = [torch.randint(0, 900, (n,), generator=g) for n in (300, 170)]
+    prompt = torch.cat([docs[0], torch.tensor(SEP), docs[1]])
+    nb = 80
+    got = {}
+    for native in (False, True):
+        kv = [tuple(torch.zeros(nb, BS, 2, 64, device="cuda", dtype=torch.float16)
+                    for _ in range(2)) for _ in range(3)]
+        ec = LMCacheEngineConfig.from_defaults(
+            chunk_size=256, enable_blending=True, use_layerwise=True, max_local_cpu_size=0.05,
+            blend_recompute_ratios=[ratio], blend_check_layers=[1 if ratio < 1 else 0],
+            extra_config={"blend_native_attention": native})
+        md = LMCacheEngineMetadata("tiny", 1, 0, "vllm", torch.float16)
+        conn = VLLMBufferLayerwiseGPUConnector(ec, kvcaches=kv)
+        eng = LMCacheEngine(ec, md, conn, token_database=SegmentTokenDatabase(ec, md, SEP))
+        name = f"blend-gpu-{native}"
+        VLLMModelTracker.unregister(name)
+        VLLMModelTracker.register_model(name, served)
+        try:
+            blender = get_or_create_blender(name, eng, conn, ec, kv)
+            assert blender.layerwise_model.native_attention is native
+            for i, doc in enumerate(docs):
+                slots = torch.randperm(nb * BS, generator=torch.Generator().manual_seed(i))
+                slots = slots[:len(doc)].cuda()
+                ref.prefill(doc, kv, slots)
+                for _ in eng.store_layer(doc, slot_mapping=slots):
+                    pass
+            slots = torch.randperm(nb * BS, generator=torch.Generator().manual_seed(9))
+            slots = slots[:len(prompt)].cuda()
+            assert int(blender.blend(prompt, slot_mapping=slots).sum()) == 470
+            torch.cuda.synchronize()
+            got[native] = [[c.view(nb * BS, -1)[slots].double() for c in layer] for layer in kv]
+        finally:
+            drop_blender(name)
+            VLLMModelTracker.unregister(name)
+    # up to two layers of attention apart: some 16 roundings of 2^-11 a layer and side
+    for a, b in zip(got[False], got[True]):
+        for x, y in zip(a, b):
+            err = (x - y).norm(dim=-1) / x.norm(dim=-1)
+            assert float(err.max()) <= 2 * 32 * 2.0 ** -11
